@@ -1,0 +1,343 @@
+// Rows of an embedding table, scaled on the way out, and the table's gradient.
+//
+//   forward    result[t, :] = scale * weight[index[t], :]
+//   gradient   grad_weight[r, :] (+)= scale * sum over the tokens t with index[t] = r of grad_output[t, :]
+//
+// The gradient adds the tokens of a row in token order, in double (float for half, as the reductions of this library):
+// the tokens are sorted by row (keysort.cu), a CTA walks a fixed chunk of the sorted list, and a row whose tokens cross
+// chunks is joined from the chunks' partial sums in chunk order.  No atomics on data: results repeat bit for bit, where
+// indexAdd adds in any order and, for half, rounds every addend to 11 bits.
+#include <cuda_fp16.h>
+
+#include "context.h"
+#include "core.cuh"
+#include "keysort.h"
+#include "plan.h"
+#include "rows.cuh"
+
+namespace thcb {
+namespace {
+
+constexpr int kLookThreads = 256;
+constexpr int kLookUnroll = 4;
+
+// One vector of V elements per item, kLookUnroll items per thread: the positions come first, then all row loads are in
+// flight together.
+template <typename T, int V>
+__global__ void __launch_bounds__(kLookThreads)
+embedding_kernel(T *out, const T *weight, const int64_t *index, FastDiv32 vecs32, uint64_t vecs, uint64_t items,
+                 int64_t index_stride, int64_t rows, int64_t row_stride, int64_t col_stride, int64_t out_stride, typename TypeTraits<T>::Math scale,
+                 unsigned int *errors) {
+  pdl_prologue();
+  const uint64_t base = (uint64_t)blockIdx.x * (kLookThreads * kLookUnroll) + threadIdx.x;
+  uint64_t tok[kLookUnroll], col[kLookUnroll];
+  int64_t row[kLookUnroll];
+#pragma unroll
+  for (int u = 0; u < kLookUnroll; ++u) {
+    const uint64_t i = base + (uint64_t)u * kLookThreads;
+    row[u] = -1;
+    if (i >= items) continue;
+    if (items <= 0xffffffffull) {
+      uint32_t q, r;
+      vecs32.divmod((uint32_t)i, q, r);
+      tok[u] = q;
+      col[u] = r;
+    } else {
+      tok[u] = i / vecs;
+      col[u] = i - tok[u] * vecs;
+    }
+    const int64_t k = index[(int64_t)tok[u] * index_stride] - 1;   // positions are 1-based (TH_INDEX_BASE)
+    if ((uint64_t)k < (uint64_t)rows) row[u] = k;
+    else if (col[u] == 0) atomicAdd(errors, 1u);
+  }
+  Pack<T, V> x[kLookUnroll];
+#pragma unroll
+  for (int u = 0; u < kLookUnroll; ++u)
+    if (row[u] >= 0) x[u] = load_pack<T, V>(weight + row[u] * row_stride + (int64_t)(col[u] * V) * col_stride);
+#pragma unroll
+  for (int u = 0; u < kLookUnroll; ++u) {
+    if (row[u] < 0) continue;
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[u].e[e] = from_math<T>(to_math(x[u].e[e]) * scale);
+    store_pack<T, V>(out + (int64_t)tok[u] * out_stride + (int64_t)(col[u] * V), x[u]);
+  }
+}
+
+// ---- gradient ----------------------------------------------------------------------------------
+constexpr int kGradThreads = 256;
+constexpr int kGradBatch = 8;        // rows in flight per thread
+constexpr int kGradMaxChunk = 64;    // sorted tokens per CTA
+constexpr int kZeroRows = 32;        // table rows a CTA checks and clears
+
+template <typename T> struct GradArgs {
+  T *table;
+  const T *grad;
+  const uint32_t *key, *pos;
+  typename TypeTraits<T>::Acc *partial;      // [chunk][head, tail][width]
+  int64_t tokens, width, rows;
+  int64_t grad_stride, grad_col, table_stride;
+  uint32_t chunk, chunks;
+  int accumulate;
+  typename TypeTraits<T>::Acc scale;
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void write_row(const GradArgs<T> &a, uint32_t key, int64_t col, const typename TypeTraits<T>::Acc (&acc)[V]) {
+  using Acc = typename TypeTraits<T>::Acc;
+  T *p = a.table + (int64_t)key * a.table_stride + col;
+  Pack<T, V> out;
+  if (a.accumulate) {
+    out = load_pack<T, V>(p);
+#pragma unroll
+    for (int e = 0; e < V; ++e) out.e[e] = round_from<T>((Acc)to_math(out.e[e]) + acc[e] * a.scale);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) out.e[e] = round_from<T>(acc[e] * a.scale);
+  }
+  store_pack<T, V>(p, out);
+}
+
+// CTAs 0 .. chunks-1 sum the rows named in their chunk of the sorted tokens; the ones behind clear the rows no token
+// names (accumulate = 0).
+template <typename T, int V>
+__global__ void __launch_bounds__(kGradThreads)
+embedding_grad_kernel(GradArgs<T> a) {
+  using Acc = typename TypeTraits<T>::Acc;
+  pdl_prologue();
+  const int64_t col = ((int64_t)blockIdx.y * kGradThreads + threadIdx.x) * V;
+  if (blockIdx.x >= a.chunks) {
+    __shared__ int used[kZeroRows];
+    const int64_t row0 = (int64_t)(blockIdx.x - a.chunks) * kZeroRows;
+    if (threadIdx.x < kZeroRows) {
+      const int64_t row = row0 + threadIdx.x;
+      // first sorted key that is not below the row
+      int64_t lo = 0, hi = a.tokens;
+      while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if ((int64_t)a.key[mid] < row) lo = mid + 1; else hi = mid;
+      }
+      used[threadIdx.x] = row >= a.rows || (lo < a.tokens && (int64_t)a.key[lo] == row);
+    }
+    __syncthreads();
+    if (col >= a.width) return;
+    Pack<T, V> zero;
+#pragma unroll
+    for (int e = 0; e < V; ++e) zero.e[e] = round_from<T>((Acc)0);
+    for (int r = 0; r < kZeroRows; ++r)
+      if (!used[r]) store_pack<T, V>(a.table + (row0 + r) * a.table_stride + col, zero);
+    return;
+  }
+  __shared__ uint32_t skey[kGradMaxChunk + 2], spos[kGradMaxChunk];
+  const int64_t begin = (int64_t)blockIdx.x * a.chunk;
+  const uint32_t count = (uint32_t)min((int64_t)a.chunk, a.tokens - begin);
+  // skey[0]: the key in front of the chunk; skey[count + 1]: the one behind it (a sentinel stands behind the last)
+  for (uint32_t i = threadIdx.x; i < count + 2; i += kGradThreads) {
+    const int64_t p = begin + (int64_t)i - 1;
+    skey[i] = p < 0 ? 0xfffffffeu : a.key[p];
+    if (i >= 1 && i <= count) spos[i - 1] = a.pos[p];
+  }
+  __syncthreads();
+  if (col >= a.width) return;
+  const uint32_t none = (uint32_t)a.rows;
+  Acc acc[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0;
+  const uint32_t first = skey[1];
+  const bool head_open = skey[0] == first;                      // the first row began in an earlier chunk
+  const bool tail_open = skey[count] == skey[count + 1];        // the last row goes on in the next
+  for (uint32_t i = 0; i < count; i += kGradBatch) {
+    Pack<T, V> x[kGradBatch];
+#pragma unroll
+    for (int u = 0; u < kGradBatch; ++u)
+      if (i + u < count && skey[i + u + 1] != none)
+        x[u] = load_pack<T, V>(a.grad + (int64_t)spos[i + u] * a.grad_stride + col * a.grad_col);
+#pragma unroll
+    for (int u = 0; u < kGradBatch; ++u) {
+      if (i + u >= count) break;
+      const uint32_t key = skey[i + u + 1];
+      if (key == none) return;                                  // items without a row come last
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += (Acc)to_math(x[u].e[e]);
+      if (i + u + 1 < count ? skey[i + u + 2] == key : false) continue;
+      const bool head = key == first && head_open, tail = i + u + 1 == count && tail_open;
+      if (head || tail) {
+        Acc *p = a.partial + ((int64_t)blockIdx.x * 2 + (head ? 0 : 1)) * a.width + col;
+#pragma unroll
+        for (int e = 0; e < V; ++e) p[e] = acc[e];
+      } else {
+        write_row<T, V>(a, key, col, acc);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] = 0;
+    }
+  }
+}
+
+// Joins the rows whose tokens cross chunks: the CTA of the chunk a row begins in adds the partial sums of the chunks
+// behind it, in order.
+template <typename T, int V>
+__global__ void __launch_bounds__(kGradThreads)
+embedding_grad_join_kernel(GradArgs<T> a) {
+  using Acc = typename TypeTraits<T>::Acc;
+  pdl_prologue();
+  const int64_t begin = (int64_t)blockIdx.x * a.chunk, end = begin + a.chunk;
+  if (end >= a.tokens) return;
+  const uint32_t key = a.key[end - 1];
+  if (key != a.key[end] || key == (uint32_t)a.rows) return;
+  if (begin > 0 && a.key[begin - 1] == key) return;             // began earlier (and fills this chunk)
+  const int64_t col = ((int64_t)blockIdx.y * kGradThreads + threadIdx.x) * V;
+  if (col >= a.width) return;
+  Acc acc[V];
+  const Acc *p = a.partial + ((int64_t)blockIdx.x * 2 + 1) * a.width + col;
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = p[e];
+  for (int64_t c = (int64_t)blockIdx.x + 1; c < a.chunks && a.key[c * a.chunk] == key; ++c) {
+    p = a.partial + c * 2 * a.width + col;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] += p[e];
+  }
+  write_row<T, V>(a, key, col, acc);
+}
+
+// ---- host --------------------------------------------------------------------------------------
+template <typename T>
+int run_embedding(thcb200_ctx *ctx, const MatView &out, const MatView &w, const int64_t *index, int64_t index_stride, double scale,
+                  cudaStream_t st) {
+  using Math = typename TypeTraits<T>::Math;
+  unsigned int *errors = index_errors(ctx);
+  constexpr int VB = 16 / sizeof(T);
+  const bool vec = mat_vec(out, sizeof(T), 16) && mat_vec(w, sizeof(T), 16);
+  const uint64_t vecs = vec ? (uint64_t)out.cols / VB : (uint64_t)out.cols;
+  const uint64_t items = vecs * (uint64_t)out.rows;
+  const uint64_t blocks = (items + kLookThreads * kLookUnroll - 1) / (kLookThreads * kLookUnroll);
+  if (blocks >= (1ull << 31) || vecs >= (1ull << 31)) { set_error("embedding: tensor too large"); return THCB200_ERR_LIMIT; }
+  const FastDiv32 div((uint32_t)vecs);
+  if (vec)
+    launch_pdl(embedding_kernel<T, VB>, (unsigned)blocks, kLookThreads, 0, st, (T *)out.data, (const T *)w.data, index, div, vecs,
+               items, index_stride, w.rows, w.row_stride, (int64_t)1, out.row_stride, (Math)scale, errors);
+  else
+    launch_pdl(embedding_kernel<T, 1>, (unsigned)blocks, kLookThreads, 0, st, (T *)out.data, (const T *)w.data, index, div, vecs,
+               items, index_stride, w.rows, w.row_stride, w.col_stride, out.row_stride, (Math)scale, errors);
+  count_launch();
+  THCB_CUDA_TRY(cudaGetLastError());
+  return 0;
+}
+
+uint32_t grad_chunk(int64_t tokens) {
+  // long chunks leave fewer partial sums, short ones give every SM a CTA
+  uint32_t c = kGradMaxChunk;
+  while (c > 8 && tokens / c < 8 * kNumSM_B200) c >>= 1;
+  return c;
+}
+
+template <typename T>
+int run_embedding_grad(thcb200_ctx *ctx, const MatView &table, const MatView &grad, const SortInput &in, double scale, int accumulate,
+                       cudaStream_t st) {
+  using Acc = typename TypeTraits<T>::Acc;
+  constexpr int VB = 16 / sizeof(T);
+  const bool vec = mat_vec(table, sizeof(T), 16) && mat_vec(grad, sizeof(T), 16);
+  const uint32_t chunk = grad_chunk(in.n);
+  const int64_t chunks = (in.n + chunk - 1) / chunk;
+  const int64_t zero = accumulate ? 0 : (table.rows + kZeroRows - 1) / kZeroRows;
+  const int64_t slabs = ((vec ? table.cols / VB : table.cols) + kGradThreads - 1) / kGradThreads;
+  if (chunks + zero >= (1ll << 31) || slabs > 65535) { set_error("embeddingAccGrad: tensor too large"); return THCB200_ERR_LIMIT; }
+  const size_t nk = ((size_t)(in.n + 1) * 4 + 255) & ~(size_t)255, np = ((size_t)in.n * 4 + 255) & ~(size_t)255;
+  const size_t pb = (size_t)chunks * 2 * (size_t)table.cols * sizeof(Acc);
+  Workspace ws(ctx, nk + np + ((pb + 255) & ~(size_t)255) + sort_by_key_bytes(in.n, in.limit), st);
+  if (!ws.ok) return THCB200_ERR_NOMEM;
+  GradArgs<T> a;
+  a.key = (uint32_t *)ws.data;
+  a.pos = (uint32_t *)(ws.data + nk);
+  a.partial = (Acc *)(ws.data + nk + np);
+  int rc = sort_by_key(in, (uint32_t *)a.key, (uint32_t *)a.pos, ws.data + nk + np + ((pb + 255) & ~(size_t)255), st);
+  if (rc) return rc;
+  a.table = (T *)table.data;
+  a.grad = (const T *)grad.data;
+  a.tokens = in.n;
+  a.width = table.cols;
+  a.rows = table.rows;
+  a.grad_stride = grad.row_stride;
+  a.grad_col = vec ? 1 : grad.col_stride;
+  a.table_stride = table.row_stride;
+  a.chunk = chunk;
+  a.chunks = (uint32_t)chunks;
+  a.accumulate = accumulate;
+  a.scale = (Acc)scale;
+  const dim3 grid((unsigned)(chunks + zero), (unsigned)slabs), join((unsigned)chunks, (unsigned)slabs);
+  if (vec) {
+    launch_pdl(embedding_grad_kernel<T, VB>, grid, kGradThreads, 0, st, a);
+    if (chunks > 1) launch_pdl(embedding_grad_join_kernel<T, VB>, join, kGradThreads, 0, st, a);
+  } else {
+    launch_pdl(embedding_grad_kernel<T, 1>, grid, kGradThreads, 0, st, a);
+    if (chunks > 1) launch_pdl(embedding_grad_join_kernel<T, 1>, join, kGradThreads, 0, st, a);
+  }
+  count_launch(chunks > 1 ? 2 : 1);
+  THCB_CUDA_TRY(cudaGetLastError());
+  return 0;
+}
+
+}  // namespace
+}  // namespace thcb
+
+using namespace thcb;
+
+extern "C" {
+
+int thcb200_embedding(thcb200_ctx *ctx, const thcb200_tensor *result, const thcb200_tensor *weight, const thcb200_tensor *index, double scale,
+                      void *stream) {
+  if (!ctx) { set_error("embedding: null context"); return THCB200_ERR_ARG; }
+  MatView out, w;
+  HostView vi;
+  int rc = to_mat_view(result, &out, "embedding result");
+  if (!rc) rc = to_mat_view(weight, &w, "embedding weight");
+  if (!rc) rc = to_host_view(index, &vi, "embedding index");
+  if (rc) return rc;
+  if (!floating(w.dtype) || out.dtype != w.dtype) { set_error("embedding: weight and result must be of one floating-point type"); return THCB200_ERR_ARG; }
+  if (vi.dtype != THCB200_I64 || vi.ndim != 1) { set_error("embedding: the index must be a vector of I64"); return THCB200_ERR_ARG; }
+  if (out.cols != w.cols || out.rows != vi.sizes[0]) { set_error("embedding: sizes do not match"); return THCB200_ERR_SIZE; }
+  if (!dense_rows(out)) { set_error("embedding: the result must have dense rows that do not overlap"); return THCB200_ERR_ARG; }
+  if (out.rows == 0 || out.cols == 0) return THCB200_OK;
+  cudaStream_t st = (cudaStream_t)stream;
+  set_plan_name("embedding");
+  switch (w.dtype) {
+    case THCB200_F16: return run_embedding<__half>(ctx, out, w, (const int64_t *)vi.data, vi.strides[0], scale, st);
+    case THCB200_F32: return run_embedding<float>(ctx, out, w, (const int64_t *)vi.data, vi.strides[0], scale, st);
+    default: return run_embedding<double>(ctx, out, w, (const int64_t *)vi.data, vi.strides[0], scale, st);
+  }
+}
+
+int thcb200_embedding_grad(thcb200_ctx *ctx, const thcb200_tensor *grad_weight, const thcb200_tensor *grad_output, const thcb200_tensor *index,
+                           double scale, int64_t padding_index, int accumulate, void *stream) {
+  if (!ctx) { set_error("embedding_grad: null context"); return THCB200_ERR_ARG; }
+  MatView table, grad;
+  HostView vi;
+  int rc = to_mat_view(grad_weight, &table, "embedding_grad gradient");
+  if (!rc) rc = to_mat_view(grad_output, &grad, "embedding_grad output gradient");
+  if (!rc) rc = to_host_view(index, &vi, "embedding_grad index");
+  if (rc) return rc;
+  if (!floating(table.dtype) || grad.dtype != table.dtype) { set_error("embedding_grad: both gradients must be of one floating-point type"); return THCB200_ERR_ARG; }
+  if (vi.dtype != THCB200_I64 || vi.ndim != 1) { set_error("embedding_grad: the index must be a vector of I64"); return THCB200_ERR_ARG; }
+  if (grad.cols != table.cols || grad.rows != vi.sizes[0]) { set_error("embedding_grad: sizes do not match"); return THCB200_ERR_SIZE; }
+  if (padding_index < 0 || padding_index > table.rows) { set_error("embedding_grad: padding index out of range"); return THCB200_ERR_ARG; }
+  if (!dense_rows(table)) { set_error("embedding_grad: the table's gradient must have dense rows that do not overlap"); return THCB200_ERR_ARG; }
+  if (table.rows == 0 || table.cols == 0 || (grad.rows == 0 && accumulate)) return THCB200_OK;
+  if (table.rows > kSortMaxKeys || grad.rows > kSortMaxItems) { set_error("embedding_grad: more than 2^31 rows or tokens"); return THCB200_ERR_LIMIT; }
+  THCB_CTX_LOCK(ctx);
+  SortInput in;
+  in.index = (const int64_t *)vi.data;
+  in.stride = vi.strides[0];
+  in.n = grad.rows;
+  in.limit = table.rows;
+  in.skip = padding_index;
+  in.zero_is_none = 0;
+  in.errors = index_errors(ctx);
+  cudaStream_t st = (cudaStream_t)stream;
+  set_plan_name("embedding_grad");
+  switch (table.dtype) {
+    case THCB200_F16: return run_embedding_grad<__half>(ctx, table, grad, in, scale, accumulate, st);
+    case THCB200_F32: return run_embedding_grad<float>(ctx, table, grad, in, scale, accumulate, st);
+    default: return run_embedding_grad<double>(ctx, table, grad, in, scale, accumulate, st);
+  }
+}
+
+}  // extern "C"

@@ -1,0 +1,392 @@
+// Tokens sorted by the experts they are routed to, and back.
+//
+//   sort      expert[t, k] in 1..E (0: not routed) -> slot[t, k], order[p], offsets[e], stable by (expert, t, k)
+//   dispatch  rows[slot[t, k], :] = (w[t, k] *) x[t, :]
+//   combine   y[t, :] = sum over k of (w[t, k] *) rows[slot[t, k], :]
+//   gradient  grad_rows[slot[t, k], :] = w[t, k] * grad_y[t, :],  grad_w[t, k] = <grad_y[t, :], rows[slot[t, k], :]>
+//
+// Combine without weights is the gradient of dispatch, and dispatch with weights the row part of combine's gradient.
+// All four walk the tokens, not the sorted places: a token's row is read once for its k copies, sums run over k in order
+// (no atomics, results repeat bit for bit), and every access to the sorted side is a whole row.  They are bound by HBM.
+#include <cuda_fp16.h>
+
+#include "context.h"
+#include "core.cuh"
+#include "keysort.h"
+#include "plan.h"
+#include "rows.cuh"
+
+namespace thcb {
+namespace {
+
+constexpr int kRowThreads = 256;
+
+// Routing weights and sums over k: float beside half and float, double beside double; sums as the library's reductions.
+template <typename T> struct Weight { using type = float; };
+template <> struct Weight<double> { using type = double; };
+
+template <typename T> struct RouteArgs {
+  T *dst;
+  const T *src;            // token rows (dispatch) or sorted rows (combine)
+  const int64_t *slot;     // [tokens][chosen]
+  const typename Weight<T>::type *weight;
+  uint64_t vecs, items;    // vectors per row; tokens * vecs
+  FastDiv32 vecs32;
+  int chosen;
+  int64_t places;          // rows on the sorted side
+  int64_t dst_stride, src_stride, src_col;
+  unsigned int *errors;
+};
+
+template <typename T>
+__device__ __forceinline__ void split_item(const RouteArgs<T> &a, uint64_t i, int64_t *token, int64_t *vec) {
+  if (a.items <= 0xffffffffull) {
+    uint32_t q, r;
+    a.vecs32.divmod((uint32_t)i, q, r);
+    *token = q;
+    *vec = r;
+  } else {
+    *token = (int64_t)(i / a.vecs);
+    *vec = (int64_t)(i - (uint64_t)*token * a.vecs);
+  }
+}
+
+// Place of a slot on the sorted side, or -1; a slot that is neither 0 nor a place is counted once.
+__device__ __forceinline__ int64_t place_of(int64_t slot, int64_t places, bool count, unsigned int *errors) {
+  const int64_t p = slot - 1;
+  if ((uint64_t)p < (uint64_t)places) return p;
+  if (slot != 0 && count) atomicAdd(errors, 1u);
+  return -1;
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kRowThreads)
+dispatch_kernel(RouteArgs<T> a) {
+  pdl_prologue();
+  const uint64_t i = (uint64_t)blockIdx.x * kRowThreads + threadIdx.x;
+  if (i >= a.items) return;
+  int64_t token, vec;
+  split_item(a, i, &token, &vec);
+  const Pack<T, V> x = load_pack<T, V>(a.src + token * a.src_stride + vec * V * a.src_col);
+  for (int k = 0; k < a.chosen; ++k) {
+    const int64_t p = place_of(a.slot[token * a.chosen + k], a.places, vec == 0, a.errors);
+    if (p < 0) continue;
+    T *q = a.dst + p * a.dst_stride + vec * V;
+    if (a.weight) {
+      using Math = typename TypeTraits<T>::Math;
+      const Math w = (Math)a.weight[token * a.chosen + k];
+      Pack<T, V> y;
+#pragma unroll
+      for (int e = 0; e < V; ++e) y.e[e] = from_math<T>(to_math(x.e[e]) * w);
+      store_pack<T, V>(q, y);
+    } else {
+      store_pack<T, V>(q, x);
+    }
+  }
+}
+
+constexpr int kCombineBatch = 4;
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kRowThreads)
+combine_kernel(RouteArgs<T> a) {
+  using Acc = typename TypeTraits<T>::Acc;
+  pdl_prologue();
+  const uint64_t i = (uint64_t)blockIdx.x * kRowThreads + threadIdx.x;
+  if (i >= a.items) return;
+  int64_t token, vec;
+  split_item(a, i, &token, &vec);
+  Acc acc[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0;
+  for (int k0 = 0; k0 < a.chosen; k0 += kCombineBatch) {
+    Pack<T, V> x[kCombineBatch];
+    int64_t p[kCombineBatch];
+    Acc w[kCombineBatch];
+#pragma unroll
+    for (int u = 0; u < kCombineBatch; ++u) {
+      p[u] = k0 + u < a.chosen ? place_of(a.slot[token * a.chosen + k0 + u], a.places, vec == 0, a.errors) : -1;
+      w[u] = p[u] >= 0 && a.weight ? (Acc)a.weight[token * a.chosen + k0 + u] : (Acc)1;
+    }
+#pragma unroll
+    for (int u = 0; u < kCombineBatch; ++u)
+      if (p[u] >= 0) x[u] = load_pack<T, V>(a.src + p[u] * a.src_stride + vec * V * a.src_col);
+#pragma unroll
+    for (int u = 0; u < kCombineBatch; ++u) {
+      if (p[u] < 0) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += (Acc)to_math(x[u].e[e]) * w[u];
+    }
+  }
+  Pack<T, V> y;
+#pragma unroll
+  for (int e = 0; e < V; ++e) y.e[e] = round_from<T>(acc[e]);
+  store_pack<T, V>(a.dst + token * a.dst_stride + vec * V, y);
+}
+
+template <typename T> struct CombineGradArgs {
+  T *grad_rows;                                // may be null
+  typename Weight<T>::type *grad_weight;       // may be null
+  const T *grad, *rows;
+  const int64_t *slot;
+  const typename Weight<T>::type *weight;      // may be null: ones
+  uint64_t pairs;
+  int64_t vecs;
+  FastDiv32 chosen;
+  int64_t places;
+  int64_t out_stride, grad_stride, grad_col, rows_stride, rows_col;
+  unsigned int *errors;
+};
+
+// A warp per (token, choice): the token's gradient row is read by the warps of its choices, which sit side by side in the
+// CTA, so all but the first find it in the L1.
+template <typename T, int V>
+__global__ void __launch_bounds__(kRowThreads)
+combine_grad_kernel(CombineGradArgs<T> a) {
+  using Acc = typename TypeTraits<T>::Acc;
+  using Math = typename TypeTraits<T>::Math;
+  pdl_prologue();
+  const uint32_t lane = threadIdx.x & 31;
+  const uint64_t pair = (uint64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+  if (pair >= a.pairs) return;
+  const int64_t token = a.chosen.div((uint32_t)pair);
+  const int64_t p = place_of(a.slot[pair], a.places, lane == 0, a.errors);
+  Acc dot = 0;
+  if (p >= 0) {
+    const Math w = a.weight ? (Math)a.weight[pair] : (Math)1;
+    const T *g = a.grad + token * a.grad_stride, *r = a.rows + p * a.rows_stride;
+    T *o = a.grad_rows ? a.grad_rows + p * a.out_stride : nullptr;
+#pragma unroll 4
+    for (int64_t v = lane; v < a.vecs; v += 32) {
+      const Pack<T, V> x = *reinterpret_cast<const Pack<T, V> *>(g + v * V * a.grad_col);
+      if (a.grad_weight) {
+        const Pack<T, V> y = load_pack<T, V>(r + v * V * a.rows_col);
+#pragma unroll
+        for (int e = 0; e < V; ++e) dot += (Acc)to_math(x.e[e]) * (Acc)to_math(y.e[e]);
+      }
+      if (o) {
+        Pack<T, V> y;
+#pragma unroll
+        for (int e = 0; e < V; ++e) y.e[e] = from_math<T>(to_math(x.e[e]) * w);
+        store_pack<T, V>(o + v * V, y);
+      }
+    }
+  }
+  if (!a.grad_weight) return;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(~0u, dot, d);
+  if (lane == 0) a.grad_weight[pair] = (typename Weight<T>::type)dot;
+}
+
+// ---- host --------------------------------------------------------------------------------------
+struct SlotView {
+  const int64_t *data;
+  int64_t tokens, chosen;
+};
+
+bool dense(const HostView &v) {
+  int64_t run = 1;
+  for (int d = v.ndim - 1; d >= 0; --d) {
+    if (v.sizes[d] != 1 && v.strides[d] != run) return false;
+    run *= v.sizes[d];
+  }
+  return true;
+}
+
+int slot_view(const thcb200_tensor *t, SlotView *s, const char *what) {
+  HostView v;
+  const int rc = to_host_view(t, &v, what);
+  if (rc) return rc;
+  if (v.dtype != THCB200_I64 || v.ndim != 2 || !dense(v)) { set_error("%s: expected a contiguous matrix of I64", what); return THCB200_ERR_ARG; }
+  s->data = (const int64_t *)v.data;
+  s->tokens = v.sizes[0];
+  s->chosen = v.sizes[1];
+  if (s->chosen > kSortMaxItems || (s->chosen > 0 && s->tokens > kSortMaxItems / s->chosen)) { set_error("%s: more than 2^31 choices", what); return THCB200_ERR_LIMIT; }
+  return 0;
+}
+
+// A routing weight matrix shaped like the slots, in the type that goes with the rows' type.
+int weight_view(const thcb200_tensor *t, int rows_dtype, const SlotView &s, void **data, const char *what) {
+  *data = nullptr;
+  if (!t) return 0;
+  HostView v;
+  const int rc = to_host_view(t, &v, what);
+  if (rc) return rc;
+  if (v.dtype != (rows_dtype == THCB200_F64 ? THCB200_F64 : THCB200_F32)) { set_error("%s: weights are F32, or F64 beside F64 rows", what); return THCB200_ERR_ARG; }
+  if (v.ndim != 2 || !dense(v)) { set_error("%s: expected a contiguous matrix", what); return THCB200_ERR_ARG; }
+  if (v.sizes[0] != s.tokens || v.sizes[1] != s.chosen) { set_error("%s: weights and slots differ in size", what); return THCB200_ERR_SIZE; }
+  *data = v.data;
+  return 0;
+}
+
+template <typename T>
+int run_route(thcb200_ctx *ctx, bool dispatch, const MatView &dst, const MatView &src, const SlotView &s, const void *weight, cudaStream_t st) {
+  constexpr int VB = 16 / sizeof(T);
+  const bool vec = mat_vec(dst, sizeof(T), 16) && mat_vec(src, sizeof(T), 16);
+  RouteArgs<T> a;
+  a.dst = (T *)dst.data;
+  a.src = (const T *)src.data;
+  a.slot = s.data;
+  a.weight = (const typename Weight<T>::type *)weight;
+  a.vecs = (uint64_t)(vec ? dst.cols / VB : dst.cols);
+  a.items = a.vecs * (uint64_t)s.tokens;
+  const uint64_t blocks = (a.items + kRowThreads - 1) / kRowThreads;
+  if (blocks >= (1ull << 31) || a.vecs >= (1ull << 31)) { set_error("expert rows: tensor too large"); return THCB200_ERR_LIMIT; }
+  a.vecs32 = FastDiv32((uint32_t)a.vecs);
+  a.chosen = (int)s.chosen;
+  a.places = dispatch ? dst.rows : src.rows;
+  a.dst_stride = dst.row_stride;
+  a.src_stride = src.row_stride;
+  a.src_col = vec ? 1 : src.col_stride;
+  a.errors = index_errors(ctx);
+  if (dispatch) {
+    if (vec) launch_pdl(dispatch_kernel<T, VB>, (unsigned)blocks, kRowThreads, 0, st, a);
+    else launch_pdl(dispatch_kernel<T, 1>, (unsigned)blocks, kRowThreads, 0, st, a);
+  } else {
+    if (vec) launch_pdl(combine_kernel<T, VB>, (unsigned)blocks, kRowThreads, 0, st, a);
+    else launch_pdl(combine_kernel<T, 1>, (unsigned)blocks, kRowThreads, 0, st, a);
+  }
+  count_launch();
+  THCB_CUDA_TRY(cudaGetLastError());
+  return 0;
+}
+
+template <typename T>
+int run_combine_grad(thcb200_ctx *ctx, const MatView *out, void *grad_weight, const MatView &grad, const MatView &rows, const SlotView &s,
+                     const void *weight, cudaStream_t st) {
+  constexpr int VB = 16 / sizeof(T);
+  const bool vec = (!out || mat_vec(*out, sizeof(T), 16)) && mat_vec(grad, sizeof(T), 16) && mat_vec(rows, sizeof(T), 16);
+  CombineGradArgs<T> a;
+  a.grad_rows = out ? (T *)out->data : nullptr;
+  a.grad_weight = (typename Weight<T>::type *)grad_weight;
+  a.grad = (const T *)grad.data;
+  a.rows = (const T *)rows.data;
+  a.slot = s.data;
+  a.weight = (const typename Weight<T>::type *)weight;
+  a.pairs = (uint64_t)(s.tokens * s.chosen);
+  a.vecs = vec ? grad.cols / VB : grad.cols;
+  a.chosen = FastDiv32((uint32_t)s.chosen);
+  a.places = rows.rows;
+  a.out_stride = out ? out->row_stride : 0;
+  a.grad_stride = grad.row_stride;
+  a.grad_col = vec ? 1 : grad.col_stride;
+  a.rows_stride = rows.row_stride;
+  a.rows_col = vec ? 1 : rows.col_stride;
+  a.errors = index_errors(ctx);
+  const unsigned blocks = (unsigned)((a.pairs + kRowThreads / 32 - 1) / (kRowThreads / 32));
+  if (vec) launch_pdl(combine_grad_kernel<T, VB>, blocks, kRowThreads, 0, st, a);
+  else launch_pdl(combine_grad_kernel<T, 1>, blocks, kRowThreads, 0, st, a);
+  count_launch();
+  THCB_CUDA_TRY(cudaGetLastError());
+  return 0;
+}
+
+int route(thcb200_ctx *ctx, bool dispatch, const thcb200_tensor *dst_t, const thcb200_tensor *src_t, const thcb200_tensor *slot,
+          const thcb200_tensor *weight, void *stream) {
+  const char *name = dispatch ? "expert_dispatch" : "expert_combine";
+  if (!ctx) { set_error("%s: null context", name); return THCB200_ERR_ARG; }
+  MatView dst, src;
+  SlotView s;
+  void *w = nullptr;
+  int rc = to_mat_view(dst_t, &dst, name);
+  if (!rc) rc = to_mat_view(src_t, &src, name);
+  if (!rc) rc = slot_view(slot, &s, name);
+  if (!rc && (!floating(dst.dtype) || src.dtype != dst.dtype)) { set_error("%s: both matrices must be of one floating-point type", name); rc = THCB200_ERR_ARG; }
+  if (!rc) rc = weight_view(weight, dst.dtype, s, &w, name);
+  if (rc) return rc;
+  if (dst.cols != src.cols || (dispatch ? src.rows : dst.rows) != s.tokens) { set_error("%s: sizes do not match", name); return THCB200_ERR_SIZE; }
+  if (!dense_rows(dst)) { set_error("%s: the result must have dense rows that do not overlap", name); return THCB200_ERR_ARG; }
+  if (s.tokens == 0 || dst.cols == 0 || (dispatch && s.chosen == 0)) return THCB200_OK;
+  cudaStream_t st = (cudaStream_t)stream;
+  set_plan_name(name);
+  switch (dst.dtype) {
+    case THCB200_F16: return run_route<__half>(ctx, dispatch, dst, src, s, w, st);
+    case THCB200_F32: return run_route<float>(ctx, dispatch, dst, src, s, w, st);
+    default: return run_route<double>(ctx, dispatch, dst, src, s, w, st);
+  }
+}
+
+}  // namespace
+}  // namespace thcb
+
+using namespace thcb;
+
+extern "C" {
+
+int thcb200_expert_sort(thcb200_ctx *ctx, const thcb200_tensor *slot, const thcb200_tensor *order, const thcb200_tensor *offsets,
+                        const thcb200_tensor *expert, void *stream) {
+  if (!ctx) { set_error("expert_sort: null context"); return THCB200_ERR_ARG; }
+  HostView vs, vo, vf, ve;
+  int rc = to_host_view(slot, &vs, "expert_sort slots");
+  if (!rc) rc = to_host_view(order, &vo, "expert_sort order");
+  if (!rc) rc = to_host_view(offsets, &vf, "expert_sort offsets");
+  if (!rc) rc = to_host_view(expert, &ve, "expert_sort experts");
+  if (rc) return rc;
+  for (const HostView *v : {&vs, &vo, &vf, &ve})
+    if (v->dtype != THCB200_I64 || !dense(*v)) { set_error("expert_sort: every argument is a contiguous I64 tensor"); return THCB200_ERR_ARG; }
+  if (vs.numel != ve.numel || vo.numel != ve.numel || vf.ndim != 1) { set_error("expert_sort: sizes do not match"); return THCB200_ERR_SIZE; }
+  const int64_t experts = vf.sizes[0] - 1;
+  if (experts < 1 || experts >= kSortMaxBins) { set_error("expert_sort: between 1 and %d experts", kSortMaxBins - 1); return THCB200_ERR_LIMIT; }
+  if (ve.numel > kSortMaxItems) { set_error("expert_sort: more than 2^31 choices"); return THCB200_ERR_LIMIT; }
+  THCB_CTX_LOCK(ctx);
+  SortInput in;
+  in.index = (const int64_t *)ve.data;
+  in.stride = 1;
+  in.n = ve.numel;
+  in.limit = experts;
+  in.skip = 0;
+  in.zero_is_none = 1;
+  in.errors = index_errors(ctx);
+  cudaStream_t st = (cudaStream_t)stream;
+  set_plan_name("expert_sort");
+  Workspace ws(ctx, sort_to_slots_bytes(in.n, in.limit), st);
+  if (!ws.ok) return THCB200_ERR_NOMEM;
+  return sort_to_slots(in, (int64_t *)vs.data, (int64_t *)vo.data, (int64_t *)vf.data, ws.data, st);
+}
+
+int thcb200_expert_dispatch(thcb200_ctx *ctx, const thcb200_tensor *rows, const thcb200_tensor *src, const thcb200_tensor *slot,
+                            const thcb200_tensor *weight, void *stream) {
+  return route(ctx, true, rows, src, slot, weight, stream);
+}
+
+int thcb200_expert_combine(thcb200_ctx *ctx, const thcb200_tensor *result, const thcb200_tensor *rows, const thcb200_tensor *slot,
+                           const thcb200_tensor *weight, void *stream) {
+  return route(ctx, false, result, rows, slot, weight, stream);
+}
+
+int thcb200_expert_combine_grad(thcb200_ctx *ctx, const thcb200_tensor *grad_rows, const thcb200_tensor *grad_weight,
+                                const thcb200_tensor *grad_result, const thcb200_tensor *rows, const thcb200_tensor *slot,
+                                const thcb200_tensor *weight, void *stream) {
+  const char *name = "expert_combine_grad";
+  if (!ctx) { set_error("%s: null context", name); return THCB200_ERR_ARG; }
+  MatView out, grad, r;
+  SlotView s;
+  void *w = nullptr, *gw = nullptr;
+  int rc = grad_rows ? to_mat_view(grad_rows, &out, name) : 0;
+  if (!rc) rc = to_mat_view(grad_result, &grad, name);
+  if (!rc) rc = to_mat_view(rows, &r, name);
+  if (!rc) rc = slot_view(slot, &s, name);
+  if (!rc && (!floating(grad.dtype) || r.dtype != grad.dtype || (grad_rows && out.dtype != grad.dtype))) {
+    set_error("%s: the matrices must be of one floating-point type", name);
+    rc = THCB200_ERR_ARG;
+  }
+  if (!rc) rc = weight_view(weight, grad.dtype, s, &w, name);
+  if (!rc) rc = weight_view(grad_weight, grad.dtype, s, &gw, name);
+  if (rc) return rc;
+  if (grad.rows != s.tokens || r.cols != grad.cols || (grad_rows && (out.cols != r.cols || out.rows != r.rows))) {
+    set_error("%s: sizes do not match", name);
+    return THCB200_ERR_SIZE;
+  }
+  if (grad_rows && !dense_rows(out)) { set_error("%s: the rows' gradient must have dense rows that do not overlap", name); return THCB200_ERR_ARG; }
+  if (s.tokens == 0 || s.chosen == 0 || (!grad_rows && !grad_weight)) return THCB200_OK;
+  cudaStream_t st = (cudaStream_t)stream;
+  set_plan_name(name);
+  const MatView *o = grad_rows ? &out : nullptr;
+  switch (grad.dtype) {
+    case THCB200_F16: return run_combine_grad<__half>(ctx, o, gw, grad, r, s, w, st);
+    case THCB200_F32: return run_combine_grad<float>(ctx, o, gw, grad, r, s, w, st);
+    default: return run_combine_grad<double>(ctx, o, gw, grad, r, s, w, st);
+  }
+}
+
+}  // extern "C"

@@ -14,6 +14,7 @@
 #include <atomic>
 #include <mutex>
 #include <new>
+#include <optional>
 #include <set>
 #include <type_traits>
 #include <utility>
@@ -80,6 +81,9 @@ void record_failure(const THFailure &f) {
 #define API_BEGIN try {
 #define API_END } catch (const THFailure &f) { record_failure(f); }
 #define API_END_RET(v) } catch (const THFailure &f) { record_failure(f); return v; }
+// for entry points that keep lists on the host
+#define API_END_HOST } catch (const THFailure &f) { record_failure(f); } \
+  catch (const std::bad_alloc &) { record_failure(THFailure{"out of host memory", 0}); }
 
 }  // namespace
 
@@ -1643,6 +1647,372 @@ template <typename R> void nonzero(THCState *state, LongT *out, TensorT<R> *self
   tensor_free<unsigned char>(state, mask);
 }
 
+// ---- embedding tables, expert routing, optimiser steps ----------------------------------------
+// A tensor held for the length of a call: itself, or a contiguous copy of it.
+template <typename R> struct Held {
+  THCState *state;
+  TensorT<R> *t;
+  TensorT<R> *back;       // where a copy's elements go after the call
+  explicit Held(THCState *st) : state(st), t(nullptr), back(nullptr) {}
+  Held(const Held &) = delete;
+  Held(Held &&o) noexcept : state(o.state), t(o.t), back(o.back) { o.t = nullptr; o.back = nullptr; }
+  ~Held() { if (t) tensor_free<R>(state, t); }
+  void in(TensorT<R> *x, bool as_is) {
+    if (as_is) { __sync_fetch_and_add(&x->refcount, 1); t = x; }
+    else t = tensor_new_contiguous<R>(state, x);
+  }
+  void inout(TensorT<R> *x, bool as_is, int arg) {
+    in(x, as_is);
+    if (t == x) return;
+    thcb200_tensor d = describe<R>(x);
+    THArgCheck(!thcb200_overlapping(&d), arg, "elements of the result share memory");
+    back = x;
+  }
+  void finish() { if (back) tensor_copy<R>(state, back, t); }
+};
+
+// The leading dims of a tensor as the rows of a matrix; false when they are not evenly spaced.
+template <typename R> bool as_matrix(const TensorT<R> *t, thcb200_tensor *d) {
+  const thcb200_tensor v = describe<R>(t);
+  if (v.ndim < 1) return false;
+  const int last = v.ndim - 1;
+  int64_t rows = 1, stride = 0;
+  for (int k = last - 1; k >= 0; --k) {
+    if (v.sizes[k] != 1) {
+      if (rows == 1) stride = v.strides[k];
+      else if (v.strides[k] != rows * stride) return false;
+    }
+    rows *= v.sizes[k];
+  }
+  d->data = v.data;
+  d->dtype = v.dtype;
+  d->ndim = 2;
+  d->sizes[0] = rows;
+  d->sizes[1] = v.sizes[last];
+  d->strides[0] = rows > 1 ? stride : v.sizes[last];
+  d->strides[1] = v.sizes[last] > 1 ? v.strides[last] : 1;
+  return true;
+}
+bool writable_rows(const thcb200_tensor &d) {
+  return d.strides[1] == 1 && (d.sizes[0] <= 1 || d.strides[0] >= d.sizes[1]);
+}
+
+template <typename R> struct RowsIn : Held<R> {
+  thcb200_tensor d;
+  RowsIn(THCState *state, TensorT<R> *x) : Held<R>(state) {
+    memset(&d, 0, sizeof(d));
+    this->in(x, as_matrix<R>(x, &d));
+    if (this->t != x) as_matrix<R>(this->t, &d);
+  }
+};
+template <typename R> struct RowsOut : Held<R> {
+  thcb200_tensor d;
+  RowsOut(THCState *state, TensorT<R> *x, int arg) : Held<R>(state) {
+    memset(&d, 0, sizeof(d));
+    const bool as_is = as_matrix<R>(x, &d) && writable_rows(d);
+    this->inout(x, as_is, arg);
+    if (this->t != x) as_matrix<R>(this->t, &d);
+  }
+};
+// A contiguous tensor as a vector (rows = 0) or as a matrix of so many rows.
+template <typename R> struct Dense : Held<R> {
+  thcb200_tensor d;
+  Dense(THCState *state, TensorT<R> *x, int64_t rows, int out_arg = 0) : Held<R>(state) {
+    if (out_arg) this->inout(x, tensor_is_contiguous<R>(x), out_arg);
+    else this->in(x, false);
+    d = describe<R>(this->t);
+    const int64_t n = (int64_t)tensor_nelement<R>(this->t);
+    d.ndim = rows ? 2 : 1;
+    d.sizes[0] = rows ? rows : n;
+    d.sizes[1] = rows ? n / rows : 1;
+    d.strides[0] = rows ? d.sizes[1] : 1;
+    d.strides[1] = 1;
+  }
+};
+
+// A tensor of positions as a vector.
+struct Positions : Held<long> {
+  thcb200_tensor d;
+  Positions(THCState *state, TensorT<long> *x) : Held<long>(state) {
+    in(x, x->nDimension == 1);
+    d = describe<long>(t);
+    if (d.ndim != 1) { d.sizes[0] = (int64_t)tensor_nelement<long>(t); d.strides[0] = 1; d.ndim = 1; }
+  }
+};
+
+// Results must not share memory with anything else a call is given.
+struct Span { const char *lo, *hi; };
+template <typename R> Span span_of(const TensorT<R> *t) {
+  if (!t || !t->storage || !t->storage->data || tensor_nelement<R>(t) == 0) return Span{nullptr, nullptr};
+  ptrdiff_t lo = 0, hi = 0;
+  for (int d = 0; d < t->nDimension; ++d) {
+    const ptrdiff_t reach = (ptrdiff_t)(t->size[d] - 1) * t->stride[d];
+    if (reach > 0) hi += reach; else lo += reach;
+  }
+  const R *p = t->storage->data + t->storageOffset;
+  return Span{(const char *)(p + lo), (const char *)(p + hi + 1)};
+}
+void check_apart(int arg, Span out, std::initializer_list<Span> others) {
+  if (!out.lo) return;
+  for (const Span &s : others)
+    if (s.lo && out.lo < s.hi && s.lo < out.hi) th_arg_error(arg, "the result shares memory with another argument");
+}
+
+void resize2(THCState *state, TensorT<long> *t, long a) { tensor_raw_resize<long>(state, t, 1, &a, nullptr); }
+
+template <typename R> void embedding(THCState *state, TensorT<R> *result, TensorT<R> *weight, LongT *index, double scale) {
+  check_gpu<R>(state, {result, weight});
+  check_gpu<long>(state, {index});
+  THArgCheck(weight->nDimension == 2, 3, "expecting a matrix of rows");
+  THArgCheck(index->nDimension >= 1, 4, "expecting a tensor of positions");
+  THArgCheck(index->nDimension < THCB200_MAX_DIMS, 4, CUTORCH_DIM_WARNING);
+  long sz[THCB200_MAX_DIMS];
+  for (int d = 0; d < index->nDimension; ++d) sz[d] = index->size[d];
+  sz[index->nDimension] = weight->size[1];
+  tensor_raw_resize<R>(state, result, index->nDimension + 1, sz, nullptr);
+  check_apart(2, span_of<R>(result), {span_of<R>(weight), span_of<long>(index)});
+  if (tensor_nelement<R>(result) == 0) return;
+  RowsOut<R> out(state, result, 2);
+  RowsIn<R> w(state, weight);
+  Positions ix(state, index);
+  check_core(thcb200_embedding(state_ctx(state), &out.d, &w.d, &ix.d, scale, (void *)state_stream(state)));
+  out.finish();
+}
+
+template <typename R>
+void embedding_acc_grad(THCState *state, TensorT<R> *grad_weight, TensorT<R> *grad_output, LongT *index, double scale, long padding, int accumulate) {
+  check_gpu<R>(state, {grad_weight, grad_output});
+  check_gpu<long>(state, {index});
+  THArgCheck(grad_weight->nDimension == 2, 2, "expecting a matrix of rows");
+  THArgCheck(padding >= 0 && padding <= grad_weight->size[0], 6, "paddingIndex out of range");
+  THArgCheck(index->nDimension >= 1, 4, "expecting a tensor of positions");
+  THArgCheck(grad_output->nDimension == index->nDimension + 1, 3, "gradOutput must have the sizes of index and the table's columns");
+  for (int d = 0; d < index->nDimension; ++d)
+    THArgCheck(grad_output->size[d] == index->size[d], 3, "gradOutput must have the sizes of index and the table's columns");
+  THArgCheck(grad_output->size[index->nDimension] == grad_weight->size[1], 3, "gradOutput must have the sizes of index and the table's columns");
+  check_apart(2, span_of<R>(grad_weight), {span_of<R>(grad_output), span_of<long>(index)});
+  if (tensor_nelement<R>(grad_weight) == 0) return;
+  RowsOut<R> table(state, grad_weight, 2);
+  RowsIn<R> grad(state, grad_output);
+  Positions ix(state, index);
+  check_core(thcb200_embedding_grad(state_ctx(state), &table.d, &grad.d, &ix.d, scale, padding, accumulate, (void *)state_stream(state)));
+  table.finish();
+}
+
+void expert_sort(THCState *state, LongT *slot, LongT *order, LongT *offsets, LongT *expert, long experts) {
+  check_gpu<long>(state, {slot, order, offsets, expert});
+  THArgCheck(experts >= 1, 6, "nExperts must be positive");
+  THArgCheck(expert->nDimension >= 1, 5, "expecting a tensor of experts");
+  THArgCheck(slot != expert && order != expert && offsets != expert && slot != order && slot != offsets && order != offsets, 2,
+             "the results must be different tensors");
+  if (experts >= 2048) th_arg_error(6, "at most 2047 experts");
+  tensor_resize_as<long>(state, slot, expert);
+  resize2(state, order, (long)tensor_nelement<long>(expert));
+  resize2(state, offsets, experts + 1);
+  const Span s = span_of<long>(slot), o = span_of<long>(order), f = span_of<long>(offsets), e = span_of<long>(expert);
+  check_apart(2, s, {o, f, e});
+  check_apart(3, o, {f, e});
+  check_apart(4, f, {e});
+  Dense<long> ds(state, slot, 0, 2), dord(state, order, 0, 3), df(state, offsets, 0, 4), de(state, expert, 0);
+  check_core(thcb200_expert_sort(state_ctx(state), &ds.d, &dord.d, &df.d, &de.d, (void *)state_stream(state)));
+  ds.finish();
+  dord.finish();
+  df.finish();
+}
+
+template <typename A> void check_weight(TensorT<A> *weight, LongT *slot, int arg) {
+  if (!weight) return;
+  THArgCheck(weight->nDimension == slot->nDimension, arg, "weight and slot must have the same sizes");
+  for (int d = 0; d < slot->nDimension; ++d) THArgCheck(weight->size[d] == slot->size[d], arg, "weight and slot must have the same sizes");
+}
+void check_slot(LongT *slot, int arg) { THArgCheck(slot->nDimension == 1 || slot->nDimension == 2, arg, "slot must be a vector or a matrix"); }
+
+template <typename R, typename A> void expert_dispatch(THCState *state, TensorT<R> *rows, TensorT<R> *src, LongT *slot, TensorT<A> *weight) {
+  check_gpu<R>(state, {rows, src});
+  check_gpu<long>(state, {slot});
+  if (weight) check_gpu<A>(state, {weight});
+  THArgCheck(src->nDimension == 2, 3, "expecting a matrix of rows");
+  check_slot(slot, 4);
+  THArgCheck(slot->size[0] == src->size[0], 4, "slot must have a row for each row of src");
+  check_weight<A>(weight, slot, 5);
+  const long n = (long)tensor_nelement<long>(slot);
+  if (rows->nDimension != 2 || rows->size[1] != src->size[1] || rows->size[0] < n) {
+    const long sz[2] = {n, src->size[1]};
+    tensor_raw_resize<R>(state, rows, 2, sz, nullptr);
+  }
+  check_apart(2, span_of<R>(rows), {span_of<R>(src), span_of<long>(slot), span_of<A>(weight)});
+  if (n == 0 || src->size[1] == 0) return;
+  RowsOut<R> out(state, rows, 2);
+  RowsIn<R> in(state, src);
+  Dense<long> s(state, slot, slot->size[0]);
+  if (weight) {
+    Dense<A> w(state, weight, slot->size[0]);
+    check_core(thcb200_expert_dispatch(state_ctx(state), &out.d, &in.d, &s.d, &w.d, (void *)state_stream(state)));
+  } else {
+    check_core(thcb200_expert_dispatch(state_ctx(state), &out.d, &in.d, &s.d, nullptr, (void *)state_stream(state)));
+  }
+  out.finish();
+}
+
+template <typename R, typename A> void expert_combine(THCState *state, TensorT<R> *result, TensorT<R> *rows, LongT *slot, TensorT<A> *weight) {
+  check_gpu<R>(state, {result, rows});
+  check_gpu<long>(state, {slot});
+  if (weight) check_gpu<A>(state, {weight});
+  THArgCheck(rows->nDimension == 2, 3, "expecting a matrix of rows");
+  check_slot(slot, 4);
+  check_weight<A>(weight, slot, 5);
+  const long sz[2] = {slot->size[0], rows->size[1]};
+  tensor_raw_resize<R>(state, result, 2, sz, nullptr);
+  check_apart(2, span_of<R>(result), {span_of<R>(rows), span_of<long>(slot), span_of<A>(weight)});
+  if (sz[0] == 0 || sz[1] == 0) return;
+  RowsOut<R> out(state, result, 2);
+  RowsIn<R> in(state, rows);
+  Dense<long> s(state, slot, slot->size[0]);
+  if (weight) {
+    Dense<A> w(state, weight, slot->size[0]);
+    check_core(thcb200_expert_combine(state_ctx(state), &out.d, &in.d, &s.d, &w.d, (void *)state_stream(state)));
+  } else {
+    check_core(thcb200_expert_combine(state_ctx(state), &out.d, &in.d, &s.d, nullptr, (void *)state_stream(state)));
+  }
+  out.finish();
+}
+
+template <typename R, typename A>
+void expert_combine_grad(THCState *state, TensorT<R> *grad_rows, TensorT<A> *grad_weight, TensorT<R> *grad_result, TensorT<R> *rows, LongT *slot,
+                         TensorT<A> *weight) {
+  check_gpu<R>(state, {grad_rows, grad_result, rows});
+  check_gpu<long>(state, {slot});
+  check_gpu<A>(state, {grad_weight, weight});
+  THArgCheck(grad_result->nDimension == 2, 4, "expecting a matrix of rows");
+  THArgCheck(rows->nDimension == 2 && rows->size[1] == grad_result->size[1], 5, "expecting a matrix of as many columns");
+  check_slot(slot, 6);
+  THArgCheck(slot->size[0] == grad_result->size[0], 6, "slot must have a row for each row of gradResult");
+  check_weight<A>(weight, slot, 7);
+  if (grad_rows) tensor_resize_as<R>(state, grad_rows, rows);
+  if (grad_weight) tensor_raw_resize<A>(state, grad_weight, slot->nDimension, slot->size, nullptr);
+  const Span gr = span_of<R>(grad_rows), gw = span_of<A>(grad_weight);
+  check_apart(2, gr, {gw, span_of<R>(grad_result), span_of<R>(rows), span_of<long>(slot), span_of<A>(weight)});
+  check_apart(3, gw, {span_of<R>(grad_result), span_of<R>(rows), span_of<long>(slot), span_of<A>(weight)});
+  if (tensor_nelement<long>(slot) == 0) return;
+  if (rows->size[1] == 0 || rows->size[0] == 0) {   // no rows to multiply with
+    if (grad_weight) pointwise<A>(state, THCB200_OP_FILL, grad_weight, nullptr, nullptr, nullptr, kZero, kZero);
+    return;
+  }
+  RowsIn<R> grad(state, grad_result), in(state, rows);
+  Dense<long> s(state, slot, slot->size[0]);
+  std::optional<RowsOut<R>> out;
+  std::optional<Dense<A>> gwd, wd;
+  if (grad_rows) out.emplace(state, grad_rows, 2);
+  if (grad_weight) gwd.emplace(state, grad_weight, slot->size[0], 3);
+  if (weight) wd.emplace(state, weight, slot->size[0]);
+  check_core(thcb200_expert_combine_grad(state_ctx(state), out ? &out->d : nullptr, gwd ? &gwd->d : nullptr, &grad.d, &in.d, &s.d,
+                                         wd ? &wd->d : nullptr, (void *)state_stream(state)));
+  if (out) out->finish();
+  if (gwd) gwd->finish();
+}
+
+// A list's tensors, contiguous for the call.
+template <typename R> struct HeldList {
+  std::vector<Held<R>> v;
+  R *add(THCState *state, TensorT<R> *t, ptrdiff_t n, bool written, int arg, int i) {
+    if (!t) th_arg_error(arg, "tensor %d is missing", i + 1);
+    check_gpu<R>(state, {t});
+    if (tensor_nelement<R>(t) != n) th_arg_error(arg, "tensor %d has %ld elements, expected %ld", i + 1, (long)tensor_nelement<R>(t), (long)n);
+    if (n == 0) return nullptr;
+    const bool dense = tensor_is_contiguous<R>(t);
+    if (!dense) {
+      v.emplace_back(state);
+      if (written) v.back().inout(t, false, arg); else v.back().in(t, false);
+      t = v.back().t;
+    }
+    return (R *)describe<R>(t).data;
+  }
+  void finish() { for (Held<R> &h : v) h.finish(); }
+};
+
+long unit_count(ptrdiff_t n) { return (long)((n + THCB200_ADAMW_BLOCK - 1) / THCB200_ADAMW_BLOCK); }
+
+template <typename R, typename A>
+void adamw(THCState *state, TensorT<R> **param, TensorT<R> **grad, TensorT<A> **m, TensorT<A> **v, TensorT<A> **master, int n, thcb200_adamw_args args) {
+  THArgCheck(n >= 0 && (n == 0 || (param && grad && m && v)), 2, "expecting lists of tensors");
+  std::vector<thcb200_adamw_tensor> list((size_t)n);
+  HeldList<R> hp;
+  HeldList<A> ha;
+  for (int i = 0; i < n; ++i) {
+    THArgCheck(param[i] != nullptr, 2, "tensor %d is missing", i + 1);
+    const ptrdiff_t k = tensor_nelement<R>(param[i]);
+    thcb200_adamw_tensor &t = list[(size_t)i];
+    t = thcb200_adamw_tensor{};
+    t.numel = k;
+    t.param = hp.add(state, param[i], k, true, 2, i);
+    t.grad = hp.add(state, grad[i], k, false, 3, i);
+    t.m = ha.add(state, m[i], k, true, 4, i);
+    t.v = ha.add(state, v[i], k, true, 5, i);
+    if (master) t.master = ha.add(state, master[i], k, true, 6, i);
+  }
+  check_core(thcb200_adamw(state_ctx(state), RealTraits<R>::dtype, 32, list.data(), n, &args, (void *)state_stream(state)));
+  hp.finish();
+  ha.finish();
+}
+
+template <typename R, typename A>
+void adamw8bit(THCState *state, TensorT<R> **param, TensorT<R> **grad, TensorT<char> **m, TensorT<unsigned char> **v, TensorT<float> **m_unit,
+               TensorT<float> **v_unit, TensorT<A> **master, int n, thcb200_adamw_args args) {
+  THArgCheck(n >= 0 && (n == 0 || (param && grad && m && v && m_unit && v_unit)), 2, "expecting lists of tensors");
+  std::vector<thcb200_adamw_tensor> list((size_t)n);
+  HeldList<R> hp;
+  HeldList<A> ha;
+  HeldList<char> hm;
+  HeldList<unsigned char> hv;
+  HeldList<float> hu;
+  for (int i = 0; i < n; ++i) {
+    THArgCheck(param[i] != nullptr, 2, "tensor %d is missing", i + 1);
+    const ptrdiff_t k = tensor_nelement<R>(param[i]);
+    thcb200_adamw_tensor &t = list[(size_t)i];
+    t = thcb200_adamw_tensor{};
+    t.numel = k;
+    t.param = hp.add(state, param[i], k, true, 2, i);
+    t.grad = hp.add(state, grad[i], k, false, 3, i);
+    t.m = hm.add(state, m[i], k, true, 4, i);
+    t.v = hv.add(state, v[i], k, true, 5, i);
+    t.m_unit = hu.add(state, m_unit[i], unit_count(k), true, 6, i);
+    t.v_unit = hu.add(state, v_unit[i], unit_count(k), true, 7, i);
+    if (master) t.master = ha.add(state, master[i], k, true, 8, i);
+  }
+  check_core(thcb200_adamw(state_ctx(state), RealTraits<R>::dtype, 8, list.data(), n, &args, (void *)state_stream(state)));
+  hp.finish();
+  ha.finish();
+  hm.finish();
+  hv.finish();
+  hu.finish();
+}
+
+void adamw_values(THCState *state, TensorT<float> **m_value, TensorT<float> **v_value, TensorT<char> **m, TensorT<unsigned char> **v,
+                  TensorT<float> **m_unit, TensorT<float> **v_unit, int n) {
+  THArgCheck(n >= 0 && (n == 0 || (m_value && v_value && m && v && m_unit && v_unit)), 2, "expecting lists of tensors");
+  std::vector<thcb200_adamw_tensor> list((size_t)n);
+  HeldList<float> hf;
+  HeldList<char> hm;
+  HeldList<unsigned char> hv;
+  for (int i = 0; i < n; ++i) {
+    THArgCheck(m[i] != nullptr && v[i] != nullptr && m_value[i] != nullptr && v_value[i] != nullptr, 2, "tensor %d is missing", i + 1);
+    const ptrdiff_t k = tensor_nelement<char>(m[i]);
+    if (tensor_nelement<float>(m_value[i]) != k) tensor_raw_resize<float>(state, m_value[i], m[i]->nDimension, m[i]->size, nullptr);
+    if (tensor_nelement<float>(v_value[i]) != k) tensor_raw_resize<float>(state, v_value[i], m[i]->nDimension, m[i]->size, nullptr);
+    thcb200_adamw_tensor &t = list[(size_t)i];
+    t = thcb200_adamw_tensor{};
+    t.numel = k;
+    t.param = hf.add(state, m_value[i], k, true, 2, i);
+    t.master = hf.add(state, v_value[i], k, true, 3, i);
+    t.m = hm.add(state, m[i], k, false, 4, i);
+    t.v = hv.add(state, v[i], k, false, 5, i);
+    t.m_unit = hf.add(state, m_unit[i], unit_count(k), false, 6, i);
+    t.v_unit = hf.add(state, v_unit[i], unit_count(k), false, 7, i);
+  }
+  check_core(thcb200_adamw_values(state_ctx(state), list.data(), n, (void *)state_stream(state)));
+  hf.finish();
+}
+
 // The index* calls with a CPU LongTensor of positions (lib/THC/generic/THCTensorIndex.cu:5-15,
 // 133-143,261-272,383-394): the positions go up into a temporary CudaLongTensor, then the call
 // with device indices runs.
@@ -1783,5 +2153,18 @@ int THCudaByteTensor_logicalany(THCState *state, THCudaByteTensor *self) {
   API_BEGIN
   return (int)reduce_all_i<unsigned char>(state, THCB200_RED_ANY, THCB200_PRE_IDENTITY, kZero, (TensorT<unsigned char> *)self);
   API_END_RET(0)
+}
+void THCudaLongTensor_expertSort(THCState *state, THCudaLongTensor *slot, THCudaLongTensor *order, THCudaLongTensor *offsets,
+                                 THCudaLongTensor *expert, long nExperts) {
+  API_BEGIN
+  expert_sort(state, (LongT *)slot, (LongT *)order, (LongT *)offsets, (LongT *)expert, nExperts);
+  API_END_HOST
+}
+void THCudaTensor_adamwValues(THCState *state, THCudaTensor **mValue, THCudaTensor **vValue, THCudaCharTensor **m, THCudaByteTensor **v,
+                              THCudaTensor **mUnit, THCudaTensor **vUnit, int n) {
+  API_BEGIN
+  adamw_values(state, (TensorT<float> **)mValue, (TensorT<float> **)vValue, (TensorT<char> **)m, (TensorT<unsigned char> **)v,
+               (TensorT<float> **)mUnit, (TensorT<float> **)vUnit, n);
+  API_END_HOST
 }
 }

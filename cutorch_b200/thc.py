@@ -71,8 +71,9 @@ class CpuTensor:
     def ptr(self):
         return C.byref(self._tensor)
 FLOATING = ("Half", "Float", "Double")
+ACC_KIND = {"Half": "Float", "Float": "Float", "Double": "Double"}   # the tensor of a floating type's accreal
 
-# Argument codes: T tensor of the receiver's type, L LongTensor, C / M CPU Long / Byte tensor (CpuTensor), r real, l long, i int, S sizes.
+# Argument codes: T tensor of the receiver's type, L LongTensor, A tensor of the receiver's accreal (None: NULL), f accreal, C / M CPU Long / Byte tensor (CpuTensor), r real, l long, i int, S sizes.
 # Return codes: v void, a accreal, R real, n int.
 _UNARY = ["sigmoid", "log", "lgamma", "log1p", "exp", "cos", "acos", "cosh", "sin", "asin", "sinh", "tan", "atan",
           "tanh", "sqrt", "rsqrt", "ceil", "floor", "round", "trunc", "frac", "cinv", "neg", "abs", "sign"]
@@ -109,6 +110,9 @@ SIGNATURES.update({
     "indexFill_long": ("v", "TiCr"),
     "gather": ("v", "TTiL"), "scatter": ("v", "TiLT"), "scatterAdd": ("v", "TiLT"), "scatterFill": ("v", "TiLr"),
     "cumsum": ("v", "TTl"), "cumprod": ("v", "TTl"),
+    # rows of an embedding table and their gradient, rows to the experts and back
+    "embedding": ("v", "TTLf"), "embeddingAccGrad": ("v", "TTLfli"), "expertSort": ("v", "TTTTl"),
+    "expertDispatch": ("v", "TTLA"), "expertCombine": ("v", "TTLA"), "expertCombineGrad": ("v", "TATTLA"),
     "maskedFill": ("v", "TBr"), "maskedCopy": ("v", "TBT"), "maskedSelect": ("v", "TTB"),
 })
 # comparisons: <op>Value / <op>Tensor write a Byte tensor ("B"), the ...T forms the operands' type
@@ -427,40 +431,41 @@ class Tensor:
             raise TypeError(f"{name} takes {len(spec)} arguments ({spec}), got {len(args)}")
         f = self.state.fn(self.kind, name)
         creal, cacc = KINDS[self.kind][2], KINDS[self.kind][3]
-        argtypes, cargs = [C.c_void_p], [self.state.ptr]
+        if not hasattr(f, "prototype"):
+            # a function object belongs to one symbol: its prototype is set once
+            codes = {"r": creal, "l": C.c_long, "f": cacc}
+            f.argtypes = [C.c_void_p] + [codes.get(c, C.c_int if c == "i" else C.c_void_p) for c in spec]
+            f.restype = {"v": None, "a": cacc, "R": creal, "n": C.c_int, "p": C.c_ssize_t}[ret]
+            f.prototype = spec
+        cargs = [self.state.ptr]
         storages = []
         for code, a in zip(spec, args):
             if code == "S":
                 sz = self._long_storage(tuple(a))
                 storages.append(sz)
-                argtypes.append(C.c_void_p)
                 cargs.append(sz)
                 continue
-            if code in "TLB":
+            if code in "TLBA":
+                if a is None and code == "A":
+                    cargs.append(None)
+                    continue
                 if not isinstance(a, Tensor):
                     raise TypeError(f"{name}: expected a tensor")
-                want = {"L": "Long", "B": "Byte"}.get(code, self.kind)
+                want = {"L": "Long", "B": "Byte", "A": ACC_KIND.get(self.kind)}.get(code, self.kind)
                 if a.kind != want:
                     raise TypeError(f"{name}: expected a {want} tensor, got {a.kind}")
-                argtypes.append(C.c_void_p)
                 cargs.append(a.ptr)
             elif code in "CM":
                 want = "Long" if code == "C" else "Byte"
                 if not isinstance(a, CpuTensor) or a.kind != want:
                     raise TypeError(f"{name}: expected a CPU {want} tensor")
-                argtypes.append(C.c_void_p)
                 cargs.append(a.ptr)
             elif code == "r":
-                argtypes.append(creal)
                 cargs.append(self._real(a))
-            elif code == "l":
-                argtypes.append(C.c_long)
-                cargs.append(int(a))
+            elif code == "f":
+                cargs.append(float(a))
             else:
-                argtypes.append(C.c_int)
                 cargs.append(int(a))
-        f.argtypes = argtypes
-        f.restype = {"v": None, "a": cacc, "R": creal, "n": C.c_int, "p": C.c_ssize_t}[ret]
         r = f(*cargs)
         for sz in storages:
             self.state.lib.THLongStorage_free(sz)
@@ -533,3 +538,55 @@ class Tensor:
         if name in SIGNATURES:
             return lambda *args: self.call(name, self, *args)
         raise AttributeError(name)
+
+
+class TensorList:
+    """Handles of several tensors of one kind, as the calls over lists of tensors take them: an optimiser keeps one for its
+    parameters, one for their gradients and one for each moment."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        if not self.tensors:
+            raise ValueError("an empty list of tensors")
+        self.state, self.kind = self.tensors[0].state, self.tensors[0].kind
+        if any(t.kind != self.kind for t in self.tensors):
+            raise TypeError("tensors of different kinds in one list")
+        self.array = (C.c_void_p * len(self.tensors))(*[t.ptr for t in self.tensors])
+
+    def __len__(self):
+        return len(self.tensors)
+
+    def _call(self, name, lists, kinds, scalars=(), scalar_types=()):
+        for what, want in zip(lists, kinds):
+            if what is None:
+                continue
+            if not isinstance(what, TensorList):
+                raise TypeError(f"{name}: expected a TensorList")
+            if what.kind != want:
+                raise TypeError(f"{name}: expected {want} tensors, got {what.kind}")
+            if len(what) != len(self):
+                raise ValueError(f"{name}: lists of {len(self)} and {len(what)} tensors")
+        f = self.state.fn(self.kind, name)
+        if not hasattr(f, "prototype"):
+            f.argtypes = [C.c_void_p] * (1 + len(lists)) + [C.c_int, *scalar_types]
+            f.restype = None
+            f.prototype = name
+        f(self.state.ptr, *[None if x is None else x.array for x in lists], len(self), *scalars)
+        self.state.check()
+
+    def adamw(self, grad, m, v, *, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, grad_scale=1.0, master=None):
+        """One AdamW step of these parameters (THCTensor_(adamw)); m, v and master are of the parameters' accreal."""
+        acc = ACC_KIND.get(self.kind)
+        self._call("adamw", (self, grad, m, v, master), (self.kind, self.kind, acc, acc, acc),
+                   (step, lr, beta1, beta2, eps, weight_decay, grad_scale), (C.c_long, *[C.c_double] * 6))
+
+    def adamw8bit(self, grad, m, v, m_unit, v_unit, *, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, grad_scale=1.0,
+                  master=None):
+        """The same with the moments in 8 bits (THCTensor_(adamw8bit)): Char and Byte codes, a float unit per 256 elements."""
+        self._call("adamw8bit", (self, grad, m, v, m_unit, v_unit, master),
+                   (self.kind, self.kind, "Char", "Byte", "Float", "Float", ACC_KIND.get(self.kind)),
+                   (step, lr, beta1, beta2, eps, weight_decay, grad_scale), (C.c_long, *[C.c_double] * 6))
+
+    def adamwValues(self, v_value, m, v, m_unit, v_unit):
+        """The floats that 8-bit moments stand for: these tensors receive the first moment's, v_value's the second's."""
+        self._call("adamwValues", (self, v_value, m, v, m_unit, v_unit), ("Float", "Float", "Char", "Byte", "Float", "Float"))

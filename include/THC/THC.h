@@ -181,11 +181,23 @@ THCB200_DECLARE_TH_TENSOR(Double)
 #define THC_B200_DECLARE_STRUCTS
 #include "THCForEachType.h"
 #undef THC_B200_DECLARE_STRUCTS
+/* the tensor of each floating type's accreal */
+typedef THCudaTensor THCudaHalfAccTensor;
+typedef THCudaTensor THCudaAccTensor;
+typedef THCudaDoubleTensor THCudaDoubleAccTensor;
 #define THC_B200_DECLARE_API
 #include "THCForEachType.h"
 #undef THC_B200_DECLARE_API
 
 THC_API int THCudaByteTensor_logicalall(THCState *state, THCudaByteTensor *self);
 THC_API int THCudaByteTensor_logicalany(THCState *state, THCudaByteTensor *self);
+
+/* Choices sorted by expert (no counterpart in cutorch): slot becomes expert's sizes, order expert's element count, offsets
+ * nExperts + 1; see thcb200_expert_sort. */
+THC_API void THCudaLongTensor_expertSort(THCState *state, THCudaLongTensor *slot, THCudaLongTensor *order, THCudaLongTensor *offsets,
+                                         THCudaLongTensor *expert, long nExperts);
+/* What n tensors of 8-bit moments (adamw8bit) stand for, as floats: mValue and vValue become as large as m and v. */
+THC_API void THCudaTensor_adamwValues(THCState *state, THCudaTensor **mValue, THCudaTensor **vValue, THCudaCharTensor **m, THCudaByteTensor **v,
+                                      THCudaTensor **mUnit, THCudaTensor **vUnit, int n);
 
 #endif /* THCB200_THC_H */

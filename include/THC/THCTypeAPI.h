@@ -327,6 +327,32 @@ THC_API void THCTensor_(scatter)(THCState *state, THCTensor *tensor, int dim, st
 THC_API void THCTensor_(scatterAdd)(THCState *state, THCTensor *tensor, int dim, struct THCudaLongTensor *index, THCTensor *src);
 THC_API void THCTensor_(scatterFill)(THCState *state, THCTensor *tensor, int dim, struct THCudaLongTensor *index, real value);
 
+/* ---- embedding tables, expert routing, optimiser steps: no counterpart in cutorch, whose programs compose them from
+ * indexSelect / indexAdd, gather / scatter and cmul / addcmul / addcdiv.  Positions are 1-based; one that is out of range is
+ * skipped and counted (thcb200_take_index_errors).  THCAccTensor is the tensor of accreal. ---- */
+#if THC_T_FLOATING
+#define THCAccTensor TH_CONCAT_3(TH, CReal, AccTensor)
+/* result[.., :] = scale * weight[index[..], :]; result becomes index's sizes by weight's columns */
+THC_API void THCTensor_(embedding)(THCState *state, THCTensor *result, THCTensor *weight, struct THCudaLongTensor *index, accreal scale);
+/* gradWeight[r, :] (+)= scale * sum of the gradOutput rows whose index is r, except r = paddingIndex (0: none); without
+ * accumulate the other rows become zero.  gradWeight has the table's sizes already. */
+THC_API void THCTensor_(embeddingAccGrad)(THCState *state, THCTensor *gradWeight, THCTensor *gradOutput, struct THCudaLongTensor *index, accreal scale, long paddingIndex, int accumulate);
+/* rows[slot[t, k], :] = src[t, :] (times weight[t, k] unless weight is NULL).  rows becomes slot's element count by src's
+ * columns unless it is a matrix of these columns and at least as many rows; rows no slot names are left as they are. */
+THC_API void THCTensor_(expertDispatch)(THCState *state, THCTensor *rows, THCTensor *src, struct THCudaLongTensor *slot, THCAccTensor *weight);
+/* result[t, :] = sum over k of weight[t, k] * rows[slot[t, k], :] (weight NULL: ones) */
+THC_API void THCTensor_(expertCombine)(THCState *state, THCTensor *result, THCTensor *rows, struct THCudaLongTensor *slot, THCAccTensor *weight);
+/* gradRows[slot[t, k], :] = weight[t, k] * gradResult[t, :] and gradWeight[t, k] = <gradResult[t, :], rows[slot[t, k], :]>;
+ * gradRows or gradWeight may be NULL.  gradRows becomes as large as rows (rows no slot names are left as they are). */
+THC_API void THCTensor_(expertCombineGrad)(THCState *state, THCTensor *gradRows, THCAccTensor *gradWeight, THCTensor *gradResult, THCTensor *rows, struct THCudaLongTensor *slot, THCAccTensor *weight);
+/* One AdamW step over n tensors (thcb200_adamw): arrays of n handles; tensors at the same place have the same element
+ * count.  master: NULL, or float copies of half parameters.  The 8-bit form (Half, Float) keeps codes and, per 256
+ * elements, a float unit for each moment. */
+THC_API void THCTensor_(adamw)(THCState *state, THCTensor **param, THCTensor **grad, THCAccTensor **m, THCAccTensor **v, THCAccTensor **master, int n, long step, double lr, double beta1, double beta2, double eps, double weightDecay, double gradScale);
+THC_API void THCTensor_(adamw8bit)(THCState *state, THCTensor **param, THCTensor **grad, struct THCudaCharTensor **m, struct THCudaByteTensor **v, THCudaTensor **mUnit, THCudaTensor **vUnit, THCAccTensor **master, int n, long step, double lr, double beta1, double beta2, double eps, double weightDecay, double gradScale);
+#undef THCAccTensor
+#endif
+
 /* ---- triangles of a matrix (lib/THC/generic/THCTensorMath.h: tril, triu) ---- */
 THC_API void THCTensor_(tril)(THCState *state, THCTensor *self, THCTensor *src, long k);
 THC_API void THCTensor_(triu)(THCState *state, THCTensor *self, THCTensor *src, long k);

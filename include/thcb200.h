@@ -409,6 +409,75 @@ THCB200_API int thcb200_mask_coords(thcb200_ctx *ctx, const thcb200_tensor *out_
                         const thcb200_tensor *mask_u8, const int64_t *sizes, int nd,
                         void *stream, int flags);
 
+/* ---- embedding tables, expert routing, optimiser steps -------------------------------------
+ *
+ * cutorch leaves these to chains of its tensor calls (indexSelect and mul, indexAdd, one cmul / addcmul / addcdiv per
+ * tensor and operation); here each is one call.  They take F16, F32 and F64 matrices with any row stride; results need
+ * dense rows that do not overlap.  Positions are 1-based; one that is out of range is skipped and counted
+ * (thcb200_take_index_errors).  Sums run in a fixed order, in double (F16: float), and are rounded once: results repeat
+ * bit for bit.  A result must not share memory with an input. */
+
+/* result[t, :] = scale * weight[index[t], :].  `index` is an I64 vector (any stride); a row whose position is out of
+ * range is left as it was. */
+THCB200_API int thcb200_embedding(thcb200_ctx *ctx, const thcb200_tensor *result, const thcb200_tensor *weight,
+                      const thcb200_tensor *index, double scale, void *stream);
+/* grad_weight[r, :] = scale * sum over t with index[t] = r of grad_output[t, :], in token order; rows no token names
+ * become zero.  accumulate != 0 adds the sums to what is there and leaves the other rows alone.  Tokens whose position is
+ * padding_index (0: none) are left out.  Uses the context's workspace: about 24 bytes per token and the partial sums of
+ * rows whose tokens are cut by a chunk boundary. */
+THCB200_API int thcb200_embedding_grad(thcb200_ctx *ctx, const thcb200_tensor *grad_weight, const thcb200_tensor *grad_output,
+                           const thcb200_tensor *index, double scale, int64_t padding_index, int accumulate, void *stream);
+
+/* Stable order of choices by expert.  expert[t, k] in 1..E, 0 = not routed.  slot (as many entries as expert): the 1-based
+ * place of a choice among all routed ones, experts one after the other, inside one in the order of (t, k); 0 = not
+ * routed.  order (as many): the 1-based flat choice t * K + k + 1 at each place, 0 behind the last.  offsets (E + 1): choices of
+ * experts up to e, so expert e has places offsets[e - 1] + 1 .. offsets[e].  Contiguous I64 tensors, 1 <= E <= 2047. */
+THCB200_API int thcb200_expert_sort(thcb200_ctx *ctx, const thcb200_tensor *slot, const thcb200_tensor *order,
+                        const thcb200_tensor *offsets, const thcb200_tensor *expert, void *stream);
+/* rows[slot[t, k], :] = src[t, :], times weight[t, k] when a weight is given.  Rows no slot names are left as they were; no
+ * two slots may name the same row.  slot: contiguous I64 [T, K]; weight: contiguous [T, K], F32 (F64 beside F64). */
+THCB200_API int thcb200_expert_dispatch(thcb200_ctx *ctx, const thcb200_tensor *rows, const thcb200_tensor *src,
+                            const thcb200_tensor *slot, const thcb200_tensor *weight, void *stream);
+/* result[t, :] = sum over k of weight[t, k] * rows[slot[t, k], :] (weight NULL: ones); a token without a slot gets zeros.
+ * Without weights this is the gradient of thcb200_expert_dispatch. */
+THCB200_API int thcb200_expert_combine(thcb200_ctx *ctx, const thcb200_tensor *result, const thcb200_tensor *rows,
+                           const thcb200_tensor *slot, const thcb200_tensor *weight, void *stream);
+/* Gradient of thcb200_expert_combine: grad_rows[slot[t, k], :] = weight[t, k] * grad_result[t, :] (rows no slot names are left
+ * as they were) and grad_weight[t, k] = <grad_result[t, :], rows[slot[t, k], :]> (0 for a choice that is not routed).  Either
+ * may be NULL. */
+THCB200_API int thcb200_expert_combine_grad(thcb200_ctx *ctx, const thcb200_tensor *grad_rows, const thcb200_tensor *grad_weight,
+                                const thcb200_tensor *grad_result, const thcb200_tensor *rows,
+                                const thcb200_tensor *slot, const thcb200_tensor *weight, void *stream);
+
+/* One AdamW step over n contiguous tensors:
+ *   g = grad_scale * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps)
+ * dtype: the type of param and grad.  bits = 32: m and v are float (double for F64).  bits = 8 (F16, F32): m holds int8 and
+ * v uint8 codes, and every THCB200_ADAMW_BLOCK elements share one float in m_unit and one in v_unit; all zero is the start.
+ * A code c of m stands for c|c| * unit, one of v for c^4 * unit; values between two codes are rounded up or down by a hash of
+ * the element's place and the step, so that averages keep their expectation.  A NaN or infinite gradient makes its
+ * block's moments NaN.  master (F16; all tensors or none): float copies the step is computed from.
+ * No element may be written twice: a list whose written arrays share memory is refused.  The arguments, step among them, are
+ * fixed when a call is captured into a graph. */
+#define THCB200_ADAMW_BLOCK 256
+typedef struct thcb200_adamw_tensor {
+  void *param;
+  const void *grad;
+  void *m, *v;
+  float *m_unit, *v_unit;
+  void *master;
+  int64_t numel;
+} thcb200_adamw_tensor;
+typedef struct thcb200_adamw_args {
+  double lr, beta1, beta2, eps, weight_decay, grad_scale;
+  int64_t step;
+} thcb200_adamw_args;
+THCB200_API int thcb200_adamw(thcb200_ctx *ctx, int dtype, int bits, const thcb200_adamw_tensor *tensors, int n,
+                  const thcb200_adamw_args *args, void *stream);
+/* The floats that 8-bit moments stand for: param receives the first moment's values, master the second's (both float, numel
+ * elements); grad is not used. */
+THCB200_API int thcb200_adamw_values(thcb200_ctx *ctx, const thcb200_adamw_tensor *tensors, int n, void *stream);
+
 /* ---- sharded reductions: one rank per GPU of a box, NCCL over NVLink ---------------------
  *
  * cutorch drives several GPUs from one process and has no collective layer
