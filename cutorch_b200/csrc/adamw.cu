@@ -15,8 +15,13 @@
 // nothing is drawn, the same call gives the same codes.  A second moment that is not zero never takes code 0: a zero
 // below the root would blow its element's step up.
 //
-// Every step here is one IEEE operation (the library is compiled without contraction), so codes do not depend on the
-// compiler's choice of fused operations.
+// Moments and codes take one IEEE operation after the other (the library is compiled without contraction), so they do not
+// depend on the compiler's choice of fused operations; the 8-bit form's parameter takes the approximate root and reciprocal.
+//
+// Both are bound by HBM in principle.  200 M float elements in 290 tensors, B200: 32-bit moments 804 us, 5.6 GB, 6970 GB/s (the
+// box's copy: 6558).  8-bit moments, 3.2 GB: 860 us, 3.7 TB/s, bound by instruction issue (105 per element, 75 % of the issue
+// slots; 1310 us with scalar instructions, IEEE roots and byte conversions, 925 us packed, 890 us with the spills of 64 registers
+// taken for a fourth CTA, 860 us with the next tile prefetched into the L2).
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -201,78 +206,246 @@ adamw_kernel(const __grid_constant__ StepTable<N> table, const StepScalars<typen
 }
 
 // ---- 8-bit codes ---------------------------------------------------------------------------------
-__device__ __forceinline__ float first_value(int c) { return (float)(c * abs(c)); }
-__device__ __forceinline__ float second_value(int c) { const float f = (float)(c * c); return f * f; }
-__device__ __forceinline__ uint32_t dither_of(uint32_t place, uint32_t step) {
-  uint32_t h = place * 0x9E3779B9u + step;
-  h = (h ^ h >> 16) * 0x9E3779B9u;
-  h = (h ^ h >> 15) * 0x9E3779B9u;
+// Codes are handled as floats: c * |c| and (c c)(c c) are the products the definition names, and bytes become floats and
+// back by their place in the significand of 2^23 + c (an exact addition) instead of conversion instructions.  Neighbouring
+// elements share the packed float instructions (two IEEE operations each).
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pair(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__host__ __device__ __forceinline__ F2 both(float a) {
+#ifdef __CUDA_ARCH__
+  return pair(a, a);
+#else
+  uint32_t b;
+  memcpy(&b, &a, 4);
+  return (F2)b << 32 | b;
+#endif
+}
+__device__ __forceinline__ float lo_of(F2 x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float hi_of(F2 x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+// The two products, as a * b + z with z = -0 from the kernel's arguments: the assembler contracts a packed product and the
+// packed sum behind it into one operation (a last bit of a moment differed), whatever it is told; a value it does not know to be
+// zero stops it.
+__device__ __forceinline__ F2 mul2(F2 a, F2 b, F2 z) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(z)); return r; }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+// The step's scalars, as pairs.
+struct StepPairs {
+  F2 grad_scale, beta1, one_minus_beta1, beta2, one_minus_beta2, keep, minus_size, root, eps;
+  F2 minus_zero;
+  uint32_t dither;
+};
+__device__ __forceinline__ F2 sub2(F2 a, F2 b) { return fma2(b, both(-1.0f), a); }   // no instruction for the sign
+__device__ __forceinline__ F2 fma2_down(F2 a, F2 b, F2 c) { F2 r; asm("fma.rm.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+
+// Byte k of a word as 2^23 + byte.
+__device__ __forceinline__ float byte_magic(uint32_t word, int k) { return __uint_as_float(__byte_perm(word, 0x4b000000u, 0x7440 | k)); }
+// Half k of a word as 2^7 + half / 65536.
+__device__ __forceinline__ float half_magic(uint32_t word, int k) { return __uint_as_float(__byte_perm(word, 0x43000000u, k ? 0x7432 : 0x7410)); }
+constexpr float kMagic = 8388608.0f, kByteMagic = 12582912.0f;      // 1.5 * 2^23: -128..255 end up in the low byte
+__device__ __forceinline__ float first_value(float c) { return c * fabsf(c); }
+__device__ __forceinline__ float second_value(float c) { const float f = c * c; return f * f; }
+constexpr uint32_t kDitherPlace = 0x9E3779B9u;         // 2^32 over the golden ratio; the step's hash is added to place * this
+__device__ __forceinline__ uint32_t dither_of(uint32_t h) {
+  h = (h ^ h >> 16) * kDitherPlace;
+  h = (h ^ h >> 15) * kDitherPlace;
   return h ^ h >> 16;
 }
-// The last code of 0..TOP whose value is at most x, or by the dither the next.
-template <int TOP, float VALUE(int)>
-__device__ __forceinline__ int code_of(float x, float guess, float dither) {
-  int k = min(max((int)guess, 0), TOP);
-  if (VALUE(k) > x) --k;
-  else if (k < TOP && VALUE(k + 1) <= x) ++k;
-  if (k < TOP && dither * (VALUE(k + 1) - VALUE(k)) < x - VALUE(k)) ++k;
+__device__ __forceinline__ float root_near(float x) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float inverse_near(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_of(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float one_if_below(float a, float b) {
+  float r;
+  asm("set.lt.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// The last code of 0..TOP whose value is at most x, or by the dither (0..65535 of 65536) the next.
+template <int TOP, bool FOURTH>
+__device__ __forceinline__ float code_exact(float x, float root, float dither) {
+  auto value = [](float k) { return FOURTH ? second_value(k) : k * k; };
+  float k = fminf(floorf(root), (float)TOP);
+  if (value(k) > x) k -= 1.0f;
+  if (k < (float)TOP && value(k + 1.0f) <= x) k += 1.0f;
+  if (k < (float)TOP && dither * 0x1p-16f * (value(k + 1.0f) - value(k)) < x - value(k)) k += 1.0f;
   return k;
 }
-// Largest of non-negative floats over a warp; a NaN, whose bits are above infinity's, wins.
-__device__ __forceinline__ float warp_most(float x) { return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(x) & 0x7fffffffu)); }
+// The same for two elements without the corrections.  `root` is within 2^-21 of the code as a real number, so the integer
+// part k of root (1 - 2^-20) is the code or, next to a border, the one before (and below the top code even for the block's
+// largest).  If x has reached k + 1, the dither picks k + 1, which is right unless the dither is so small that k + 2
+// is due: the distance x - value(k + 1) is below 2^-10 of a step there.  `rare` becomes positive for a superset of those.
+template <bool FOURTH>
+__device__ __forceinline__ F2 codes_near(F2 x, F2 root, F2 dither, float &rare, const StepPairs &c) {
+  const F2 k = add2(fma2_down(root, both(1.0f - 0x1p-20f), both(kMagic)), both(-kMagic)), next = add2(k, both(1.0f));
+  F2 low = mul2(k, k, c.minus_zero), high = mul2(next, next, c.minus_zero);
+  if constexpr (FOURTH) { low = mul2(low, low, c.minus_zero); high = mul2(high, high, c.minus_zero); }
+  const F2 step = sub2(high, low), above = sub2(x, low), bar = mul2(dither, step, c.minus_zero);
+  const F2 over = fma2(step, both(-(1.0f - 0x1p-9f)), sub2(above, bar));
+  rare = max_of(rare, lo_of(over), hi_of(over));
+  return add2(k, pair(one_if_below(lo_of(bar), lo_of(above)), one_if_below(hi_of(bar), hi_of(above))));
+}
 
 constexpr float kFirstTop = (float)(1.0 / 16129.0), kSecondTop = (float)(1.0 / (255.0 * 255.0 * 255.0 * 255.0));
 // Blocks whose largest value is below these (where a unit would leave the normal floats) are stored as zero.
 constexpr float kFirstLeast = 1e-30f, kSecondLeast = 1e-28f;
 
+// The thread's eight codes, as two words.
+template <typename T>
+__device__ __forceinline__ void load_codes(uint32_t (&w)[2], const T *p, const Place &q) {
+  Eight<T> x;
+  load_eight(x, p, q);
+  memcpy(w, &x, 8);
+}
+template <typename T>
+__device__ __forceinline__ void store_codes(T *p, const uint32_t (&w)[2], const Place &q) {
+  Eight<T> x;
+  memcpy(&x, w, 8);
+  store_eight(p, x, q);
+}
+
+// m and v of elements j and j + 1 from their codes.
+__device__ __forceinline__ F2 first_pair(const uint32_t (&c)[2], int j, F2 unit, const StepPairs &p) {
+  const F2 k = add2(pair(byte_magic(c[j / 4], j % 4), byte_magic(c[j / 4], j % 4 + 1)), both(-(kMagic + 128.0f)));
+  return mul2(pair(first_value(lo_of(k)), first_value(hi_of(k))), unit, p.minus_zero);
+}
+__device__ __forceinline__ F2 second_pair(const uint32_t (&c)[2], int j, F2 unit, const StepPairs &p) {
+  const F2 k = add2(pair(byte_magic(c[j / 4], j % 4), byte_magic(c[j / 4], j % 4 + 1)), both(-kMagic)), f = mul2(k, k, p.minus_zero);
+  return mul2(mul2(f, f, p.minus_zero), unit, p.minus_zero);
+}
+
+// Asks for the tile that this CTA's successor on the SM will work on: the loads of a short-lived CTA with many instructions
+// between them otherwise leave the memory idle while its warps compute.
+constexpr uint32_t kTilesAhead = 4 * kNumSM_B200;
+__device__ __forceinline__ void prefetch_ahead(const void *base, size_t esz, const StepEntry &e, uint32_t tile) {
+  const int64_t at = (int64_t)(tile - e.first_tile + kTilesAhead) * kStepTile;
+  const char *p = (const char *)base + at * esz;
+  if (at + kStepTile <= e.n && ((uintptr_t)p & 15) == 0)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p), "r"((uint32_t)(kStepTile * esz)) : "memory");
+}
+
 template <typename T, bool MASTER, int N>
-__global__ void __launch_bounds__(kStepThreads)
-adamw8_kernel(const __grid_constant__ StepTable<N> table, const StepScalars<float> s) {
+__global__ void __launch_bounds__(kStepThreads, 4)
+adamw8_kernel(const __grid_constant__ StepTable<N> table, const __grid_constant__ StepPairs c) {
   pdl_prologue();
   const StepEntry &e = entry_of(table, blockIdx.x);
   const Place q = place_of(e, blockIdx.x);
   const int64_t block = (int64_t)(blockIdx.x - e.first_tile) * (kStepThreads / 32) + (threadIdx.x >> 5);
   if (block * kUnitItems >= e.n) return;      // whole warps
-  Eight<float> p, m, v;
+  Eight<float> p;
   Eight<T> g;
-  Eight<int8_t> cm;
-  Eight<uint8_t> cv;
+  uint32_t cm[2], cv[2];
   load_param<T, MASTER>(p, e, q);
   load_eight(g, (const T *)e.grad, q);
-  load_eight(cm, (const int8_t *)e.m, q);
-  load_eight(cv, (const uint8_t *)e.v, q);
-  const float mu = e.m_unit[block], vu = e.v_unit[block];
-  float mm = 0, vm = 0;
-  bool mnan = false;
+  load_codes(cm, (const int8_t *)e.m, q);
+  load_codes(cv, (const uint8_t *)e.v, q);
+  if (threadIdx.x == 0) prefetch_ahead(MASTER ? e.master : e.param, MASTER ? 4 : sizeof(T), e, blockIdx.x);
+  if (threadIdx.x == 64) prefetch_ahead(e.grad, sizeof(T), e, blockIdx.x);
+  if (threadIdx.x == 128) prefetch_ahead(e.m, 1, e, blockIdx.x);
+  if (threadIdx.x == 192) prefetch_ahead(e.v, 1, e, blockIdx.x);
+  const F2 mu = both(e.m_unit[block]), vu = both(e.v_unit[block]);
+  cm[0] ^= 0x80808080u;                       // signed codes as 128 + c
+  cm[1] ^= 0x80808080u;
+  F2 m[kStepItems / 2], v[kStepItems / 2];
 #pragma unroll
-  for (int j = 0; j < kStepItems; ++j) {
-    m.e[j] = first_value(cm.e[j]) * mu;
-    v.e[j] = second_value(cv.e[j]) * vu;
-    advance<float>(p.e[j], m.e[j], v.e[j], to_math(g.e[j]), s);
-    if (!q.wide && q.at(j) >= q.n) m.e[j] = v.e[j] = 0;
-    mnan = mnan || !(m.e[j] == m.e[j]) || !(v.e[j] == v.e[j]);
-    mm = fmaxf(mm, fabsf(m.e[j]));
-    vm = fmaxf(vm, v.e[j]);
+  for (int i = 0; i < kStepItems / 2; ++i) {
+    const F2 gi = mul2(pair(to_math(g.e[2 * i]), to_math(g.e[2 * i + 1])), c.grad_scale, c.minus_zero);
+    m[i] = add2(mul2(first_pair(cm, 2 * i, mu, c), c.beta1, c.minus_zero), mul2(gi, c.one_minus_beta1, c.minus_zero));
+    v[i] = add2(mul2(second_pair(cv, 2 * i, vu, c), c.beta2, c.minus_zero), mul2(mul2(gi, c.one_minus_beta2, c.minus_zero), gi, c.minus_zero));
+    // the approximate root flushes what is below the normal floats: 2^-126 is nothing beside any other v
+    const F2 vr = add2(v[i], both(0x1p-126f));
+    const F2 den = fma2(pair(root_near(lo_of(vr)), root_near(hi_of(vr))), c.root, c.eps);
+    const F2 ratio = mul2(m[i], pair(inverse_near(lo_of(den)), inverse_near(hi_of(den))), c.minus_zero);
+    const F2 pi = fma2(c.minus_size, ratio, mul2(pair(p.e[2 * i], p.e[2 * i + 1]), c.keep, c.minus_zero));
+    p.e[2 * i] = lo_of(pi);
+    p.e[2 * i + 1] = hi_of(pi);
   }
   store_param<T, MASTER>(p, e, q);
-  if (mnan) mm = vm = __int_as_float(0x7fffffff);
-  mm = warp_most(mm);
-  vm = warp_most(vm);
-  // not (x < least): a NaN stays
-  const float nmu = mm < kFirstLeast ? 0.0f : mm * kFirstTop, nvu = vm < kSecondLeast ? 0.0f : vm * kSecondTop;
-  const float mi = nmu > 0 ? 1.0f / nmu : 0.0f, vi = nvu > 0 ? 1.0f / nvu : 0.0f;
+  if (!q.wide) {
 #pragma unroll
-  for (int j = 0; j < kStepItems; ++j) {
-    const uint32_t h = dither_of((uint32_t)q.at(j), s.dither);
-    const float xm = fabsf(m.e[j]) * mi, xv = v.e[j] * vi;
-    const int km = code_of<127, first_value>(xm, sqrtf(xm), (float)(h >> 16) * (1.0f / 65536.0f));
-    int kv = code_of<255, second_value>(xv, sqrtf(sqrtf(xv)), (float)(h & 0xffffu) * (1.0f / 65536.0f));
-    if (v.e[j] > 0 && kv == 0) kv = 1;
-    cm.e[j] = (int8_t)(m.e[j] < 0 ? -km : km);
-    cv.e[j] = (uint8_t)kv;
+    for (int i = 0; i < kStepItems / 2; ++i) {
+      if (q.at(2 * i) >= q.n) m[i] = v[i] = 0;
+      else if (q.at(2 * i + 1) >= q.n) { m[i] = pair(lo_of(m[i]), 0.0f); v[i] = pair(lo_of(v[i]), 0.0f); }
+    }
   }
-  store_eight((int8_t *)e.m, cm, q);
-  store_eight((uint8_t *)e.v, cv, q);
+  float mmost = 0, vmost = 0;
+#pragma unroll
+  for (int i = 0; i < kStepItems / 2; ++i) {
+    mmost = max_or_nan(mmost, fabsf(lo_of(m[i])), fabsf(hi_of(m[i])));
+    vmost = max_or_nan(vmost, lo_of(v[i]), hi_of(v[i]));
+  }
+  // over the warp by the bits: a NaN's are above infinity's and win
+  mmost = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(mmost)));
+  vmost = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(vmost)));
+  // not (x < least): a NaN stays
+  const float nmu = mmost < kFirstLeast ? 0.0f : mmost * kFirstTop, nvu = vmost < kSecondLeast ? 0.0f : vmost * kSecondTop;
+  const float mi = nmu > 0 ? 1.0f / nmu : 0.0f, vi = nvu > 0 ? 1.0f / nvu : 0.0f;
+  const uint32_t h = (uint32_t)q.at(0) * kDitherPlace + c.dither, hstep = q.wide ? kDitherPlace : 32u * kDitherPlace;
+  F2 km[kStepItems / 2], kv[kStepItems / 2];
+  float rare = 0;
+#pragma unroll
+  for (int i = 0; i < kStepItems / 2; ++i) {
+    const uint32_t d0 = dither_of(h + 2 * i * hstep), d1 = dither_of(h + (2 * i + 1) * hstep);
+    const F2 xm = pair(fabsf(lo_of(m[i])) * mi, fabsf(hi_of(m[i])) * mi), xv = mul2(v[i], both(vi), c.minus_zero);
+    km[i] = codes_near<false>(xm, pair(root_near(lo_of(xm)), root_near(hi_of(xm))),
+                              add2(pair(half_magic(d0, 1), half_magic(d1, 1)), both(-128.0f)), rare, c);
+    kv[i] = codes_near<true>(xv, pair(root_near(root_near(lo_of(xv))), root_near(root_near(hi_of(xv)))),
+                             add2(pair(half_magic(d0, 0), half_magic(d1, 0)), both(-128.0f)), rare, c);
+  }
+  if (rare > 0) {
+#pragma unroll
+    for (int i = 0; i < kStepItems / 2; ++i) {
+      float a[2], b[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t d = dither_of(h + (2 * i + k) * hstep);
+        const float xm = fabsf(k ? hi_of(m[i]) : lo_of(m[i])) * mi, xv = (k ? hi_of(v[i]) : lo_of(v[i])) * vi;
+        a[k] = code_exact<127, false>(xm, root_near(xm), (float)(d >> 16));
+        b[k] = code_exact<255, true>(xv, root_near(root_near(xv)), (float)(d & 0xffffu));
+      }
+      km[i] = pair(a[0], a[1]);
+      kv[i] = pair(b[0], b[1]);
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    uint32_t bm[4], bv[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int j = 2 * w + i;
+      const F2 sm = add2(pair(copysignf(lo_of(km[j]), lo_of(m[j])), copysignf(hi_of(km[j]), hi_of(m[j]))), both(kByteMagic));
+      // at least 1 where v is above zero: v 2^200, cut at 1, is 0 or 1
+      const F2 big = mul2(v[j], both(0x1p100f), c.minus_zero);
+      const F2 sv = add2(pair(fmaxf(lo_of(kv[j]), __saturatef(lo_of(big) * 0x1p100f)), fmaxf(hi_of(kv[j]), __saturatef(hi_of(big) * 0x1p100f))), both(kByteMagic));
+      bm[2 * i] = (uint32_t)sm;
+      bm[2 * i + 1] = (uint32_t)(sm >> 32);
+      bv[2 * i] = (uint32_t)sv;
+      bv[2 * i + 1] = (uint32_t)(sv >> 32);
+    }
+    cm[w] = __byte_perm(__byte_perm(bm[0], bm[1], 0x0040), __byte_perm(bm[2], bm[3], 0x0040), 0x5410);
+    cv[w] = __byte_perm(__byte_perm(bv[0], bv[1], 0x0040), __byte_perm(bv[2], bv[3], 0x0040), 0x5410);
+  }
+  store_codes((int8_t *)e.m, cm, q);
+  store_codes((uint8_t *)e.v, cv, q);
   if ((threadIdx.x & 31) == 0) {
     e.m_unit[block] = nmu;
     e.v_unit[block] = nvu;
@@ -282,22 +455,26 @@ adamw8_kernel(const __grid_constant__ StepTable<N> table, const StepScalars<floa
 // What the codes stand for: param and master of the entry are the float results for the first and second moment.
 template <int N>
 __global__ void __launch_bounds__(kStepThreads)
-adamw_values_kernel(const __grid_constant__ StepTable<N> table) {
+adamw_values_kernel(const __grid_constant__ StepTable<N> table, const __grid_constant__ StepPairs c) {
   pdl_prologue();
   const StepEntry &e = entry_of(table, blockIdx.x);
   const Place q = place_of(e, blockIdx.x);
   const int64_t block = (int64_t)(blockIdx.x - e.first_tile) * (kStepThreads / 32) + (threadIdx.x >> 5);
   if (block * kUnitItems >= e.n) return;
-  Eight<int8_t> cm;
-  Eight<uint8_t> cv;
+  uint32_t cm[2], cv[2];
   Eight<float> m, v;
-  load_eight(cm, (const int8_t *)e.m, q);
-  load_eight(cv, (const uint8_t *)e.v, q);
-  const float mu = e.m_unit[block], vu = e.v_unit[block];
+  load_codes(cm, (const int8_t *)e.m, q);
+  load_codes(cv, (const uint8_t *)e.v, q);
+  const F2 mu = both(e.m_unit[block]), vu = both(e.v_unit[block]);
+  cm[0] ^= 0x80808080u;
+  cm[1] ^= 0x80808080u;
 #pragma unroll
-  for (int j = 0; j < kStepItems; ++j) {
-    m.e[j] = first_value(cm.e[j]) * mu;
-    v.e[j] = second_value(cv.e[j]) * vu;
+  for (int j = 0; j < kStepItems; j += 2) {
+    const F2 a = first_pair(cm, j, mu, c), b = second_pair(cv, j, vu, c);
+    m.e[j] = lo_of(a);
+    m.e[j + 1] = hi_of(a);
+    v.e[j] = lo_of(b);
+    v.e[j + 1] = hi_of(b);
   }
   store_eight((float *)e.param, m, q);
   store_eight((float *)e.master, v, q);
@@ -358,6 +535,22 @@ int launch_table(const thcb200_adamw_tensor *t, int count, size_t esz, StepKind 
   return 0;
 }
 
+StepPairs step_pairs(const StepScalars<float> &s) {
+  StepPairs c;
+  c.grad_scale = both(s.grad_scale);
+  c.beta1 = both(s.beta1);
+  c.one_minus_beta1 = both(s.one_minus_beta1);
+  c.beta2 = both(s.beta2);
+  c.one_minus_beta2 = both(s.one_minus_beta2);
+  c.keep = both(s.keep);
+  c.minus_size = both(-s.size);
+  c.root = both(s.root);
+  c.eps = both(s.eps);
+  c.minus_zero = both(-0.0f);
+  c.dither = s.dither;
+  return c;
+}
+
 template <typename T, bool MASTER, int N>
 int run_step(const thcb200_adamw_tensor *t, int count, int bits, const thcb200_adamw_args &a, cudaStream_t st) {
   using A = typename State<T>::type;
@@ -377,8 +570,8 @@ int run_step(const thcb200_adamw_tensor *t, int count, int bits, const thcb200_a
       launch_pdl(adamw_kernel<T, MASTER, N>, tiles, kStepThreads, 0, st, table, s);
     });
   if constexpr (sizeof(T) < 8)
-    return launch_table<N>(t, count, sizeof(T), kStep8, [&](const StepTable<N> &table, unsigned tiles) {
-      launch_pdl(adamw8_kernel<T, MASTER, N>, tiles, kStepThreads, 0, st, table, s);
+    return launch_table<N>(t, count, sizeof(T), kStep8, [&, pairs = step_pairs(s)](const StepTable<N> &table, unsigned tiles) {
+      launch_pdl(adamw8_kernel<T, MASTER, N>, tiles, kStepThreads, 0, st, table, pairs);
     });
   return THCB200_ERR_UNSUPPORTED;
 }
@@ -478,12 +671,13 @@ int thcb200_adamw_values(thcb200_ctx *ctx, const thcb200_adamw_tensor *tensors, 
   }
   cudaStream_t st = (cudaStream_t)stream;
   set_plan_name("adamw_values");
+  const StepPairs pairs = step_pairs(StepScalars<float>());
   if (n <= kFewTensors)
     return launch_table<kFewTensors>(tensors, n, 4, kStepValues, [&](const StepTable<kFewTensors> &table, unsigned tiles) {
-      launch_pdl(adamw_values_kernel<kFewTensors>, tiles, kStepThreads, 0, st, table);
+      launch_pdl(adamw_values_kernel<kFewTensors>, tiles, kStepThreads, 0, st, table, pairs);
     });
   return launch_table<kManyTensors>(tensors, n, 4, kStepValues, [&](const StepTable<kManyTensors> &table, unsigned tiles) {
-    launch_pdl(adamw_values_kernel<kManyTensors>, tiles, kStepThreads, 0, st, table);
+    launch_pdl(adamw_values_kernel<kManyTensors>, tiles, kStepThreads, 0, st, table, pairs);
   });
 }
 

@@ -29,11 +29,12 @@ def inputs(r, kind, n, master=False):
     return p, g, m, v, (p.astype(acc) + (r.standard_normal(n) * 1e-5).astype(acc)) if master else None
 
 
-def check_param(got, start, g, m0, v0, step, kind, master=None):
+def check_param(got, start, g, m0, v0, step, kind, master=None, quotient=12):
     """The new parameter against the formula.  With u half a step of the arithmetic: the moments' sums have terms with at most
     four roundings (first) and six (second), the root halves its argument's relative error; with the scalars' own
     roundings the denominator is within 8 u, its quotient and product within 3 u more, and the two terms of the
-    parameter are rounded twice and once more."""
+    parameter are rounded twice and once more: 12 u for the quotient.  The 8-bit step takes the GPU's approximate root (2 u in
+    place of 1) and quotient (2 units in the last place, 4 u, in place of 1): 16 u."""
     u = 2.0 ** -53 if kind == "Double" else 2.0 ** -24
     h = HYPER
     p, m, v, den = ro.adamw(start, g, m0, v0, step, **h)
@@ -41,7 +42,7 @@ def check_param(got, start, g, m0, v0, step, kind, master=None):
     m_size = np.abs(m0.astype(np.float64)) * h["beta1"] + (1 - h["beta1"]) * gs
     size = h["lr"] / (1 - h["beta1"] ** step)
     with np.errstate(invalid="ignore", divide="ignore"):
-        tol = u * np.abs(p) + 2 * u * np.abs(start.astype(np.float64)) + size * (4 * u * m_size + 12 * u * np.abs(m)) / den
+        tol = u * np.abs(p) + 2 * u * np.abs(start.astype(np.float64)) + size * (4 * u * m_size + quotient * u * np.abs(m)) / den
     tol = 1.01 * tol * (2 if kind == "Double" else 1)          # the formula's own roundings where it has as many bits
     if kind == "Half" and master is None:
         tol = tol + 2.0 ** -11 * (np.abs(p) + tol) + 2.0 ** -25
@@ -132,7 +133,7 @@ def test_eight_bit_step(state, kind, master, step, start):
     mv.adamwValues(vv, cm, cv, um, uv)
     for (p0, g0, cm0, cv0, um0, uv0, w0), p1, cm1, cv1, um1, uv1, w1, mval, vval in zip(data, *outs, numpys(mv), numpys(vv)):
         m0, v0, m, v, km, kv, mu, vu = ro.adamw8(p0, g0, cm0, cv0, um0, uv0, step, **HYPER)
-        check_param(w1 if master else p1, w0 if master else p0, g0, m0, v0, step, kind, w0)
+        check_param(w1 if master else p1, w0 if master else p0, g0, m0, v0, step, kind, w0, quotient=16)
         if master:
             assert_bit_equal(p1, w1.astype(np.float16))
         for got, want, what in ((um1, mu, "first unit"), (uv1, vu, "second unit"), (cm1, km, "first code"), (cv1, kv, "second code"),
