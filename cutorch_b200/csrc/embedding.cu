@@ -74,32 +74,33 @@ template <typename T> struct GradArgs {
   const T *grad;
   const uint32_t *key, *pos;
   typename TypeTraits<T>::Acc *partial;      // [chunk][head, tail][width]
+  uint32_t *start_count;                     // rows that lie across more than two chunks
+  uint4 *starts;                             // for each: the chunk it begins in, the chunks behind that, its key
   int64_t tokens, width, rows;
   int64_t grad_stride, grad_col, table_stride;
   uint32_t chunk, chunks;
-  int accumulate;
   typename TypeTraits<T>::Acc scale;
 };
 
-template <typename T, int V>
-__device__ __forceinline__ void write_row(const GradArgs<T> &a, uint32_t key, int64_t col, const typename TypeTraits<T>::Acc (&acc)[V]) {
+// A row's sum, rounded once: over what is there or, `old` holding it, added to it.
+template <typename T, int V, bool ADD>
+__device__ __forceinline__ void write_row(const GradArgs<T> &a, uint32_t key, int64_t col, const typename TypeTraits<T>::Acc (&acc)[V], const Pack<T, V> &old) {
   using Acc = typename TypeTraits<T>::Acc;
-  T *p = a.table + (int64_t)key * a.table_stride + col;
   Pack<T, V> out;
-  if (a.accumulate) {
-    out = load_pack<T, V>(p);
 #pragma unroll
-    for (int e = 0; e < V; ++e) out.e[e] = round_from<T>((Acc)to_math(out.e[e]) + acc[e] * a.scale);
-  } else {
+  for (int e = 0; e < V; ++e) out.e[e] = ADD ? round_from<T>((Acc)to_math(old.e[e]) + acc[e] * a.scale) : round_from<T>(acc[e] * a.scale);
+  store_pack<T, V>(a.table + (int64_t)key * a.table_stride + col, out);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void add_partial(typename TypeTraits<T>::Acc (&acc)[V], const typename TypeTraits<T>::Acc *p) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) out.e[e] = round_from<T>(acc[e] * a.scale);
-  }
-  store_pack<T, V>(p, out);
+  for (int e = 0; e < V; ++e) acc[e] += p[e];
 }
 
 // CTAs 0 .. chunks-1 sum the rows named in their chunk of the sorted tokens; the ones behind clear the rows no token
 // names (accumulate = 0).
-template <typename T, int V>
+template <typename T, int V, bool ADD>
 __global__ void __launch_bounds__(kGradThreads)
 embedding_grad_kernel(GradArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
@@ -127,45 +128,70 @@ embedding_grad_kernel(GradArgs<T> a) {
       if (!used[r]) store_pack<T, V>(a.table + (row0 + r) * a.table_stride + col, zero);
     return;
   }
-  __shared__ uint32_t skey[kGradMaxChunk + 2], spos[kGradMaxChunk];
+  __shared__ uint32_t skey[2 * kGradMaxChunk + 2], spos[2 * kGradMaxChunk];
   const int64_t begin = (int64_t)blockIdx.x * a.chunk;
-  const uint32_t count = (uint32_t)min((int64_t)a.chunk, a.tokens - begin);
-  // skey[0]: the key in front of the chunk; skey[count + 1]: the one behind it (a sentinel stands behind the last)
-  for (uint32_t i = threadIdx.x; i < count + 2; i += kGradThreads) {
+  const uint32_t own = (uint32_t)min((int64_t)a.chunk, a.tokens - begin), seen = (uint32_t)min((int64_t)2 * a.chunk, a.tokens - begin);
+  // skey[0]: the key in front of the chunk; then the chunk's, the next chunk's, and the one behind (a sentinel ends the list)
+  for (uint32_t i = threadIdx.x; i < seen + 2; i += kGradThreads) {
     const int64_t p = begin + (int64_t)i - 1;
     skey[i] = p < 0 ? 0xfffffffeu : a.key[p];
-    if (i >= 1 && i <= count) spos[i - 1] = a.pos[p];
+    if (i >= 1 && i <= seen) spos[i - 1] = a.pos[p];
   }
+  const uint32_t none = (uint32_t)a.rows;
+  // the row that is under way at the chunk's start, and the one at its end
+  const bool wide_open = begin > a.chunk && a.key[begin - a.chunk - 1] == a.key[begin];   // began before the last chunk
   __syncthreads();
   if (col >= a.width) return;
-  const uint32_t none = (uint32_t)a.rows;
+  const uint32_t first = skey[1], last = skey[own];
+  const bool head = skey[0] == first;
+  const bool goes_on = skey[own + 1] == last, far = seen == 2 * a.chunk && skey[2 * a.chunk + 1] == last;
+  // A row that began in the last chunk and ends in this one was that chunk's; one that lies across more chunks leaves its
+  // sum over this one for the join.
+  const bool head_long = head && (wide_open || (goes_on && first == last));
+  const bool tail_long = goes_on && far;               // a row that began here: it does not end in the next chunk either
+  uint32_t from = 0, to = own;
+  if (head && !head_long)
+    while (from < own && skey[from + 1] == first) ++from;
+  if (goes_on && !tail_long && !(head && first == last))
+    while (to < seen && skey[to + 1] == last) ++to;
+  if (blockIdx.y == 0 && threadIdx.x == 0 && tail_long && last != none && !(head && first == last)) {
+    // chunks whose first token is the row's: the next two at least
+    int64_t lo = (int64_t)blockIdx.x + 3, hi = a.chunks, reach = 2;
+    while (lo + reach < hi && a.key[(lo + reach) * a.chunk] == last) { lo += reach + 1; reach *= 2; }
+    hi = min(hi, lo + reach);
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (a.key[mid * a.chunk] == last) lo = mid + 1; else hi = mid;
+    }
+    a.starts[atomicAdd(a.start_count, 1u)] = make_uint4(blockIdx.x, (uint32_t)(lo - 1 - (int64_t)blockIdx.x), last, 0);
+  }
   Acc acc[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0;
-  const uint32_t first = skey[1];
-  const bool head_open = skey[0] == first;                      // the first row began in an earlier chunk
-  const bool tail_open = skey[count] == skey[count + 1];        // the last row goes on in the next
-  for (uint32_t i = 0; i < count; i += kGradBatch) {
-    Pack<T, V> x[kGradBatch];
-#pragma unroll
-    for (int u = 0; u < kGradBatch; ++u)
-      if (i + u < count && skey[i + u + 1] != none)
-        x[u] = load_pack<T, V>(a.grad + (int64_t)spos[i + u] * a.grad_stride + col * a.grad_col);
+  for (uint32_t i = from; i < to; i += kGradBatch) {
+    Pack<T, V> x[kGradBatch], old[ADD ? kGradBatch : 1];
 #pragma unroll
     for (int u = 0; u < kGradBatch; ++u) {
-      if (i + u >= count) break;
+      if (i + u >= to || skey[i + u + 1] == none) continue;
+      x[u] = load_pack<T, V>(a.grad + (int64_t)spos[i + u] * a.grad_stride + col * a.grad_col);
+      // what the sum of a row that ends here is added to comes with the same batch
+      if (ADD && (i + u + 1 >= to || skey[i + u + 2] != skey[i + u + 1])) old[u] = load_pack<T, V>(a.table + (int64_t)skey[i + u + 1] * a.table_stride + col);
+    }
+#pragma unroll
+    for (int u = 0; u < kGradBatch; ++u) {
+      if (i + u >= to) break;
       const uint32_t key = skey[i + u + 1];
       if (key == none) return;                                  // items without a row come last
 #pragma unroll
       for (int e = 0; e < V; ++e) acc[e] += (Acc)to_math(x[u].e[e]);
-      if (i + u + 1 < count ? skey[i + u + 2] == key : false) continue;
-      const bool head = key == first && head_open, tail = i + u + 1 == count && tail_open;
-      if (head || tail) {
-        Acc *p = a.partial + ((int64_t)blockIdx.x * 2 + (head ? 0 : 1)) * a.width + col;
+      if (i + u + 1 < to && skey[i + u + 2] == key) continue;
+      const bool in_head = head_long && key == first, in_tail = tail_long && key == last;
+      if (in_head || in_tail) {
+        Acc *p = a.partial + ((int64_t)blockIdx.x * 2 + (in_head ? 0 : 1)) * a.width + col;
 #pragma unroll
         for (int e = 0; e < V; ++e) p[e] = acc[e];
       } else {
-        write_row<T, V>(a, key, col, acc);
+        write_row<T, V, ADD>(a, key, col, acc, old[ADD ? u : 0]);
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) acc[e] = 0;
@@ -173,30 +199,46 @@ embedding_grad_kernel(GradArgs<T> a) {
   }
 }
 
-// Joins the rows whose tokens cross chunks: the CTA of the chunk a row begins in adds the partial sums of the chunks
-// behind it, in order.
-template <typename T, int V>
+// Joins the rows whose tokens cross chunks.  `starts` lists the chunks in which such a row begins (in the order their CTAs came
+// by, which no result depends on); a CTA takes a row and a piece of its columns, its warps take runs of the row's chunks, and
+// the warps' sums are added in chunk order.
+constexpr int kJoinWarps = kGradThreads / 32;
+
+template <typename T, int V, bool ADD>
 __global__ void __launch_bounds__(kGradThreads)
 embedding_grad_join_kernel(GradArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
   pdl_prologue();
-  const int64_t begin = (int64_t)blockIdx.x * a.chunk, end = begin + a.chunk;
-  if (end >= a.tokens) return;
-  const uint32_t key = a.key[end - 1];
-  if (key != a.key[end] || key == (uint32_t)a.rows) return;
-  if (begin > 0 && a.key[begin - 1] == key) return;             // began earlier (and fills this chunk)
-  const int64_t col = ((int64_t)blockIdx.y * kGradThreads + threadIdx.x) * V;
-  if (col >= a.width) return;
-  Acc acc[V];
-  const Acc *p = a.partial + ((int64_t)blockIdx.x * 2 + 1) * a.width + col;
+  __shared__ Acc part[kJoinWarps][32 * V];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t rows = *a.start_count, pieces = (uint32_t)((a.width + 32 * V - 1) / (32 * V));
+  for (uint64_t job = blockIdx.x; job < (uint64_t)rows * pieces; job += gridDim.x) {
+    const uint4 row = a.starts[job / pieces];
+    const int64_t chunk = row.x, count = row.y, col = ((int64_t)(job % pieces) * 32 + lane) * V;
+    const int64_t per = (count + kJoinWarps - 1) / kJoinWarps;
+    const int64_t from = chunk + 1 + min(warp * per, count), to = chunk + 1 + min((warp + 1) * per, count);
+    Pack<T, V> old;
+    Acc acc[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) acc[e] = p[e];
-  for (int64_t c = (int64_t)blockIdx.x + 1; c < a.chunks && a.key[c * a.chunk] == key; ++c) {
-    p = a.partial + c * 2 * a.width + col;
+    for (int e = 0; e < V; ++e) acc[e] = 0;
+    if (col < a.width) {
+      if (ADD && warp == 0) old = load_pack<T, V>(a.table + (int64_t)row.z * a.table_stride + col);
+      if (warp == 0) add_partial<T, V>(acc, a.partial + (chunk * 2 + 1) * a.width + col);
+#pragma unroll 8
+      for (int64_t c = from; c < to; ++c) add_partial<T, V>(acc, a.partial + c * 2 * a.width + col);
+    }
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] += p[e];
+    for (int e = 0; e < V; ++e) part[warp][lane * V + e] = acc[e];
+    __syncthreads();
+    if (warp == 0 && col < a.width) {
+#pragma unroll
+      for (int w = 1; w < kJoinWarps; ++w)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] += part[w][lane * V + e];
+      write_row<T, V, ADD>(a, row.z, col, acc, old);
+    }
+    __syncthreads();
   }
-  write_row<T, V>(a, key, col, acc);
 }
 
 // ---- host --------------------------------------------------------------------------------------
@@ -242,14 +284,16 @@ int run_embedding_grad(thcb200_ctx *ctx, const MatView &table, const MatView &gr
   const int64_t slabs = ((vec ? table.cols / VB : table.cols) + kGradThreads - 1) / kGradThreads;
   if (chunks + zero >= (1ll << 31) || slabs > 65535) { set_error("embeddingAccGrad: tensor too large"); return THCB200_ERR_LIMIT; }
   const size_t nk = ((size_t)(in.n + 1) * 4 + 255) & ~(size_t)255, np = ((size_t)in.n * 4 + 255) & ~(size_t)255;
-  const size_t pb = (size_t)chunks * 2 * (size_t)table.cols * sizeof(Acc);
-  Workspace ws(ctx, nk + np + ((pb + 255) & ~(size_t)255) + sort_by_key_bytes(in.n, in.limit), st);
+  const size_t pb = ((size_t)chunks * 2 * (size_t)table.cols * sizeof(Acc) + 255) & ~(size_t)255, sb = ((size_t)(chunks + 1) * sizeof(uint4) + 255) & ~(size_t)255;
+  Workspace ws(ctx, nk + np + pb + sb + sort_by_key_bytes(in.n, in.limit), st);
   if (!ws.ok) return THCB200_ERR_NOMEM;
   GradArgs<T> a;
   a.key = (uint32_t *)ws.data;
   a.pos = (uint32_t *)(ws.data + nk);
   a.partial = (Acc *)(ws.data + nk + np);
-  int rc = sort_by_key(in, (uint32_t *)a.key, (uint32_t *)a.pos, ws.data + nk + np + ((pb + 255) & ~(size_t)255), st);
+  a.start_count = (uint32_t *)(ws.data + nk + np + pb);
+  a.starts = (uint4 *)a.start_count + 1;
+  int rc = sort_by_key(in, (uint32_t *)a.key, (uint32_t *)a.pos, a.start_count, ws.data + nk + np + pb + sb, st);
   if (rc) return rc;
   a.table = (T *)table.data;
   a.grad = (const T *)grad.data;
@@ -261,16 +305,20 @@ int run_embedding_grad(thcb200_ctx *ctx, const MatView &table, const MatView &gr
   a.table_stride = table.row_stride;
   a.chunk = chunk;
   a.chunks = (uint32_t)chunks;
-  a.accumulate = accumulate;
   a.scale = (Acc)scale;
-  const dim3 grid((unsigned)(chunks + zero), (unsigned)slabs), join((unsigned)chunks, (unsigned)slabs);
-  if (vec) {
-    launch_pdl(embedding_grad_kernel<T, VB>, grid, kGradThreads, 0, st, a);
-    if (chunks > 1) launch_pdl(embedding_grad_join_kernel<T, VB>, join, kGradThreads, 0, st, a);
-  } else {
-    launch_pdl(embedding_grad_kernel<T, 1>, grid, kGradThreads, 0, st, a);
-    if (chunks > 1) launch_pdl(embedding_grad_join_kernel<T, 1>, join, kGradThreads, 0, st, a);
-  }
+  const dim3 grid((unsigned)(chunks + zero), (unsigned)slabs);
+  const int64_t piece = vec ? 32 * VB : 32, pieces = (table.cols + piece - 1) / piece;
+  const unsigned join = (unsigned)(chunks * pieces < 8 * kNumSM_B200 ? chunks * pieces : 8 * kNumSM_B200);
+#define THCB_GRAD(V, ADD) \
+  do { \
+    launch_pdl(embedding_grad_kernel<T, V, ADD>, grid, kGradThreads, 0, st, a); \
+    if (chunks > 1) launch_pdl(embedding_grad_join_kernel<T, V, ADD>, join, kGradThreads, 0, st, a); \
+  } while (0)
+  if (vec && accumulate) THCB_GRAD(VB, true);
+  else if (vec) THCB_GRAD(VB, false);
+  else if (accumulate) THCB_GRAD(1, true);
+  else THCB_GRAD(1, false);
+#undef THCB_GRAD
   count_launch(chunks > 1 ? 2 : 1);
   THCB_CUDA_TRY(cudaGetLastError());
   return 0;

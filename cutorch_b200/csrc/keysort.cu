@@ -6,11 +6,32 @@
 // kernels: digit counts of every tile, a scan of those counts over the tiles, and the scatter.
 #include "keysort.h"
 
+#include <cooperative_groups.h>
+
 #include "core.cuh"
 #include "plan.h"
 
 namespace thcb {
 namespace {
+
+// launch_pdl for clusters of `cluster` CTAs.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl_cluster(void (*kernel)(KArgs...), unsigned cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
 
 constexpr int kTileThreads = 256;
 constexpr int kTileItems = 2048;      // per CTA of the tiled passes: 8 rounds of a warp
@@ -26,13 +47,30 @@ struct KeySource {
   const uint32_t *key, *pos;          // later passes
 };
 
-__device__ __forceinline__ uint32_t source_key(const KeySource &s, int64_t i) {
-  if (s.key) return s.key[i];
-  const int64_t raw = s.index[i * s.stride];
+__device__ __forceinline__ uint32_t key_of(const KeySource &s, int64_t raw) {
   const int64_t k = raw - 1;          // positions are 1-based (TH_INDEX_BASE)
   const bool row = (uint64_t)k < (uint64_t)s.limit;
   if (!row && s.errors && !(raw == 0 && s.zero_is_none) && !(raw == s.skip && s.skip != 0)) atomicAdd(s.errors, 1u);
   return (row && !(raw == s.skip && s.skip != 0)) ? (uint32_t)k : (uint32_t)s.limit;
+}
+__device__ __forceinline__ uint32_t source_key(const KeySource &s, int64_t i) { return s.key ? s.key[i] : key_of(s, s.index[i * s.stride]); }
+// A thread's items first, first + step, ... below n, all loads in flight together; 0 for the others.
+template <int ROUNDS>
+__device__ __forceinline__ void source_keys(uint32_t (&key)[ROUNDS], const KeySource &s, int64_t first, int64_t step, int64_t n) {
+  if (s.key) {
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) key[r] = first + r * step < n ? __ldcg(s.key + first + r * step) : 0;
+    return;
+  }
+  constexpr int B = ROUNDS < 8 ? ROUNDS : 8;
+#pragma unroll
+  for (int r0 = 0; r0 < ROUNDS; r0 += B) {
+    int64_t raw[B];
+#pragma unroll
+    for (int u = 0; u < B; ++u) raw[u] = first + (r0 + u) * step < n ? s.index[(first + (r0 + u) * step) * s.stride] : 0;
+#pragma unroll
+    for (int u = 0; u < B; ++u) key[r0 + u] = first + (r0 + u) * step < n ? key_of(s, raw[u]) : 0;
+  }
 }
 
 // Counts of every digit in a tile: hist[tile][bin].
@@ -43,11 +81,11 @@ tile_hist_kernel(KeySource src, uint32_t *hist, int64_t n, int shift, uint32_t b
   for (uint32_t b = threadIdx.x; b < bins; b += kTileThreads) sm[b] = 0;
   __syncthreads();
   const int64_t base = (int64_t)blockIdx.x * kTileItems;
+  uint32_t key[kTileItems / kTileThreads];
+  source_keys<kTileItems / kTileThreads>(key, src, base + threadIdx.x, kTileThreads, n);
 #pragma unroll
-  for (int r = 0; r < kTileItems / kTileThreads; ++r) {
-    const int64_t i = base + r * kTileThreads + threadIdx.x;
-    if (i < n) atomicAdd(&sm[(source_key(src, i) >> shift) & (bins - 1)], 1u);
-  }
+  for (int r = 0; r < kTileItems / kTileThreads; ++r)
+    if (base + r * kTileThreads + threadIdx.x < n) atomicAdd(&sm[(key[r] >> shift) & (bins - 1)], 1u);
   __syncthreads();
   for (uint32_t b = threadIdx.x; b < bins; b += kTileThreads) hist[(size_t)blockIdx.x * bins + b] = sm[b];
 }
@@ -110,22 +148,47 @@ __device__ __forceinline__ void cta_exclusive_scan(uint32_t *v, uint32_t count, 
   __syncthreads();
 }
 
-// A warp's stable ranks: item r of lane l (item number base + r * 32 + l) gets the count of equal digits in front of it
-// among the warp's items.  `count` holds the warp's counters, zero at the start.
-template <int ROUNDS>
-__device__ __forceinline__ void warp_ranks(const uint32_t (&digit)[ROUNDS], const bool (&live)[ROUNDS], uint32_t (&rank)[ROUNDS], uint32_t *count) {
+// Lanes of the warp with the same digit, among the live ones.  One vote per bit: the match instruction serves one distinct
+// value after the other and took 160 cycles a warp here, 8 bits of votes take about 35 issue slots.
+template <int BITS>
+__device__ __forceinline__ uint32_t lanes_with(uint32_t digit, bool live) {
+  uint32_t peers = __ballot_sync(~0u, live);
+#pragma unroll
+  for (int b = 0; b < BITS; ++b) {
+    const uint32_t mine = (uint32_t)((int32_t)(digit << (31 - b)) >> 31);   // all ones or none
+    peers &= ~(__ballot_sync(~0u, mine != 0) ^ mine);
+  }
+  return peers;
+}
+
+// A warp's stable ranks: item r of lane l (item number first + r * 32 + l) gets the count of equal digits in front of it
+// among the warp's items.  `count` holds the warp's counters, `stride` apart and zero at the start.
+template <int BITS, int ROUNDS, typename C>
+__device__ __forceinline__ void warp_ranks_of(const uint32_t (&key)[ROUNDS], int shift, int64_t first, int64_t n, uint32_t (&rank)[ROUNDS], C *count,
+                                              uint32_t stride) {
   const uint32_t lane = threadIdx.x & 31, below = (1u << lane) - 1;
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
-    const uint32_t peers = __match_any_sync(~0u, live[r] ? digit[r] : 0xffffffffu);
+    const bool live = first + r * 32 < n;
+    const uint32_t d = (key[r] >> shift) & ((1u << BITS) - 1);
+    const uint32_t peers = lanes_with<BITS>(d, live);
     uint32_t seen = 0;
-    if (live[r]) seen = count[digit[r]];
+    if (live) seen = count[d * stride];
     __syncwarp();
-    if (live[r]) {
-      rank[r] = seen + __popc(peers & below);
-      if ((peers & below) == 0) count[digit[r]] = seen + __popc(peers);
-    }
+    rank[r] = seen + __popc(peers & below);
+    if (live && (peers & below) == 0) count[d * stride] = (C)(seen + __popc(peers));
     __syncwarp();
+  }
+}
+// One unrolled form for each width of a digit (2^11 = kSortMaxBins).
+template <int ROUNDS, typename C>
+__device__ __forceinline__ void warp_ranks(const uint32_t (&key)[ROUNDS], int shift, int bits, int64_t first, int64_t n, uint32_t (&rank)[ROUNDS], C *count,
+                                           uint32_t stride) {
+  switch (bits) {
+#define THCB_RANKS(B) case B: warp_ranks_of<B, ROUNDS, C>(key, shift, first, n, rank, count, stride); break;
+    THCB_RANKS(1) THCB_RANKS(2) THCB_RANKS(3) THCB_RANKS(4) THCB_RANKS(5) THCB_RANKS(6) THCB_RANKS(7) THCB_RANKS(8) THCB_RANKS(9) THCB_RANKS(10)
+    THCB_RANKS(11)
+#undef THCB_RANKS
   }
 }
 
@@ -133,7 +196,7 @@ __device__ __forceinline__ void warp_ranks(const uint32_t (&digit)[ROUNDS], cons
 template <bool SLOTS>
 __global__ void __launch_bounds__(kTileThreads)
 tile_scatter_kernel(KeySource src, const uint32_t *hist, const uint32_t *totals, uint32_t *out_key, uint32_t *out_pos,
-                    int64_t *slot, int64_t *order, int64_t *offsets, int64_t n, int shift, uint32_t bins, int last) {
+                    uint32_t *zero, int64_t *slot, int64_t *order, int64_t *offsets, int64_t n, int shift, uint32_t bins, int last) {
   pdl_prologue();
   extern __shared__ uint32_t sm[];
   __shared__ uint32_t warp_sums[32];
@@ -151,17 +214,9 @@ tile_scatter_kernel(KeySource src, const uint32_t *hist, const uint32_t *totals,
   const uint32_t none = SLOTS ? start[src.limit] : 0;   // items with a key
   constexpr int R = kWarpItems / 32;
   const int64_t base = (int64_t)blockIdx.x * kTileItems + warp * kWarpItems + lane;
-  uint32_t key[R], pos[R], digit[R], rank[R];
-  bool live[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int64_t i = base + r * 32;
-    live[r] = i < n;
-    key[r] = live[r] ? source_key(src, i) : 0;
-    pos[r] = live[r] && src.pos ? src.pos[i] : (uint32_t)i;
-    digit[r] = (key[r] >> shift) & (bins - 1);
-  }
-  warp_ranks<R>(digit, live, rank, count + warp * bins);
+  uint32_t key[R], rank[R];
+  source_keys<R>(key, src, base, 32, n);
+  warp_ranks<R>(key, shift, 31 - __clz(bins), base, n, rank, count + warp * bins, 1);
   __syncthreads();
   for (uint32_t b = threadIdx.x; b < bins; b += kTileThreads) {
     uint32_t run = start[b] + hist[(size_t)blockIdx.x * bins + b];
@@ -175,18 +230,22 @@ tile_scatter_kernel(KeySource src, const uint32_t *hist, const uint32_t *totals,
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    if (!live[r]) continue;
-    const uint32_t p = count[warp * bins + digit[r]] + rank[r];
+    const int64_t i = base + r * 32;
+    if (i >= n) continue;
+    const uint32_t p = count[warp * bins + ((key[r] >> shift) & (bins - 1))] + rank[r];
     if constexpr (SLOTS) {
       const bool routed = p < none;
-      slot[base + r * 32] = routed ? (int64_t)p + 1 : 0;
-      order[p] = routed ? base + r * 32 + 1 : 0;
+      slot[i] = routed ? (int64_t)p + 1 : 0;
+      order[p] = routed ? i + 1 : 0;
     } else {
       out_key[p] = key[r];
-      out_pos[p] = pos[r];
+      out_pos[p] = src.pos ? src.pos[i] : (uint32_t)i;
     }
   }
-  if (!SLOTS && last && blockIdx.x == 0 && threadIdx.x == 0) out_key[n] = 0xffffffffu;
+  if (!SLOTS && last && blockIdx.x == 0 && threadIdx.x == 0) {
+    out_key[n] = 0xffffffffu;
+    *zero = 0;
+  }
 }
 
 // ---- one CTA -----------------------------------------------------------------------------------
@@ -199,7 +258,7 @@ constexpr int kSmallRounds = kSmallItems / kSmallThreads;
 // Up to kPairItems items: each thread counts the pairs its item comes after.
 template <bool SLOTS>
 __global__ void __launch_bounds__(kPairItems)
-pair_sort_kernel(KeySource src, uint32_t *out_key, uint32_t *out_pos, int64_t *slot, int64_t *order, int64_t *offsets, uint32_t n) {
+pair_sort_kernel(KeySource src, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, int64_t *slot, int64_t *order, int64_t *offsets, uint32_t n) {
   pdl_prologue();
   __shared__ uint32_t keys[kPairItems];
   const uint32_t i = threadIdx.x;
@@ -228,14 +287,17 @@ pair_sort_kernel(KeySource src, uint32_t *out_key, uint32_t *out_pos, int64_t *s
       offsets[e] = (int64_t)c;
     }
   } else {
-    if (threadIdx.x == 0) out_key[n] = 0xffffffffu;
+    if (threadIdx.x == 0) {
+      out_key[n] = 0xffffffffu;
+      *zero = 0;
+    }
   }
 }
 
 // Up to kSmallItems items: radix passes inside one CTA, items in shared memory between the passes.
 template <bool SLOTS>
 __global__ void __launch_bounds__(kSmallThreads)
-small_sort_kernel(KeySource src, uint32_t *out_key, uint32_t *out_pos, int64_t *slot, int64_t *order, int64_t *offsets, uint32_t n,
+small_sort_kernel(KeySource src, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, int64_t *slot, int64_t *order, int64_t *offsets, uint32_t n,
                   int passes, int digit_bits) {
   pdl_prologue();
   extern __shared__ uint32_t sm[];
@@ -243,35 +305,19 @@ small_sort_kernel(KeySource src, uint32_t *out_key, uint32_t *out_pos, int64_t *
   const uint32_t bins = 1u << digit_bits;
   uint32_t *skey = sm, *spos = sm + kSmallItems;
   uint32_t *count = spos + kSmallItems;      // [bins][warps]: in this order the scan runs over the bins, then the warps
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, below = (1u << lane) - 1;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr uint32_t W = kSmallThreads / 32;
   uint32_t key[kSmallRounds], pos[kSmallRounds], rank[kSmallRounds];
   // a warp's items are consecutive
   const uint32_t base = warp * (kSmallRounds * 32) + lane;
+  source_keys<kSmallRounds>(key, src, base, 32, n);
 #pragma unroll
-  for (int r = 0; r < kSmallRounds; ++r) {
-    const uint32_t i = base + r * 32;
-    pos[r] = i;
-    key[r] = i < n ? source_key(src, i) : 0;
-  }
+  for (int r = 0; r < kSmallRounds; ++r) pos[r] = base + r * 32;
   for (int p = 0; p < passes; ++p) {
     const int shift = p * digit_bits;
     for (uint32_t i = threadIdx.x; i < bins * W; i += kSmallThreads) count[i] = 0;
     __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kSmallRounds; ++r) {
-      const bool live = base + r * 32 < n;
-      const uint32_t d = (key[r] >> shift) & (bins - 1);
-      const uint32_t peers = __match_any_sync(~0u, live ? d : 0xffffffffu);
-      uint32_t seen = 0;
-      if (live) seen = count[d * W + warp];
-      __syncwarp();
-      if (live) {
-        rank[r] = seen + __popc(peers & below);
-        if ((peers & below) == 0) count[d * W + warp] = seen + __popc(peers);
-      }
-      __syncwarp();
-    }
+    warp_ranks<kSmallRounds>(key, shift, digit_bits, base, n, rank, count + warp, W);
     __syncthreads();
     cta_exclusive_scan(count, bins * W, kSmallThreads, warp_sums);
     const bool last = p == passes - 1;
@@ -301,7 +347,132 @@ small_sort_kernel(KeySource src, uint32_t *out_key, uint32_t *out_pos, int64_t *
       if (i < n) { key[r] = skey[i]; pos[r] = spos[i]; }
     }
   }
-  if (!SLOTS && threadIdx.x == 0) out_key[n] = 0xffffffffu;
+  if (!SLOTS && threadIdx.x == 0) {
+    out_key[n] = 0xffffffffu;
+    *zero = 0;
+  }
+}
+
+// ---- one cluster -------------------------------------------------------------------------------
+// Up to kClusterItems items: eight or sixteen CTAs that wait for one another in hardware, so that all passes fit one launch.
+// Sixteen (more than every GPU grants a cluster, hence the function attribute) where eight would take a second round: a pass is
+// bound by its instructions, about 100 per warp and round.  Items
+// go through global memory between the passes (they stay in the L2), digit counts through distributed shared memory.
+// A CTA first puts its items in order in its own shared memory and then writes each digit's run side by side: with eight
+// SMs the rate of scattered stores is what a pass would wait for (131072 places of one pass: 37 us scattered).
+constexpr int kClusterFew = 8, kClusterMany = 16;
+constexpr int kClusterThreads = 1024;
+constexpr int kClusterWarps = kClusterThreads / 32;
+constexpr int kClusterMaxRounds = 16;
+constexpr int64_t kClusterItems = (int64_t)kClusterMany * kClusterThreads * kClusterMaxRounds;
+constexpr int kClusterBins = 1 << kMaxDigitBits;
+
+template <bool SLOTS, int ROUNDS>
+__global__ void __launch_bounds__(kClusterThreads)
+cluster_sort_kernel(KeySource src, uint32_t *tkey, uint32_t *tpos, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, int64_t *slot, int64_t *order,
+                    int64_t *offsets, uint32_t n, int passes, int digit_bits) {
+  pdl_prologue();
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  extern __shared__ uint4 cluster_smem[];
+  uint32_t *skey = reinterpret_cast<uint32_t *>(cluster_smem), *spos = skey + ROUNDS * kClusterThreads;
+  __shared__ __align__(16) uint16_t count[kClusterWarps * kClusterBins];   // at most 512 equal digits in a warp, 16384 in a CTA
+  __shared__ uint32_t total[kClusterBins], base[kClusterBins], local[kClusterBins], warp_sums[2][32];
+  const uint32_t cta = cluster.block_rank(), ctas = cluster.num_blocks(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t bins = 1u << digit_bits;
+  const uint32_t first = (cta * kClusterWarps + warp) * (ROUNDS * 32) + lane;   // a warp's items are consecutive
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * digit_bits;
+    const bool last = p == passes - 1, from_out = ((passes - 1 - p) & 1) != 0;
+    const uint32_t *in_key = from_out ? out_key : tkey, *in_pos = from_out ? out_pos : tpos;
+    uint32_t key[ROUNDS], rank[ROUNDS];
+    if (p > 0) src.key = in_key;
+    source_keys<ROUNDS>(key, src, first, 32, n);
+    for (uint32_t i = threadIdx.x; i < kClusterWarps * bins / 8; i += kClusterThreads) reinterpret_cast<uint4 *>(count)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    uint16_t *mine = count + warp * bins;
+    warp_ranks<ROUNDS>(key, shift, digit_bits, first, n, rank, mine, 1);
+    __syncthreads();
+    const uint32_t b = threadIdx.x;
+    if (b < bins) {
+      uint32_t run = 0;
+#pragma unroll 8
+      for (int w = 0; w < kClusterWarps; ++w) {
+        const uint32_t c = count[w * bins + b];
+        count[w * bins + b] = (uint16_t)run;
+        run += c;
+      }
+      total[b] = run;
+    }
+    cluster.sync();
+    uint32_t before = 0, all = 0, here = 0;
+    if (b < bins) {
+      here = total[b];
+      for (uint32_t c0 = 0; c0 < ctas; c0 += kClusterFew) {
+        uint32_t t[kClusterFew];
+#pragma unroll
+        for (int u = 0; u < kClusterFew; ++u) t[u] = cluster.map_shared_rank(total, c0 + u)[b];
+#pragma unroll
+        for (int u = 0; u < kClusterFew; ++u) {
+          if (c0 + u < cta) before += t[u];
+          all += t[u];
+        }
+      }
+    }
+    // exclusive scans of the bins' totals, of the cluster and of this CTA: one bin a thread
+    uint32_t incl = all, incl_here = here;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t o = __shfl_up_sync(~0u, incl, d), h = __shfl_up_sync(~0u, incl_here, d);
+      if (lane >= (uint32_t)d) {
+        incl += o;
+        incl_here += h;
+      }
+    }
+    if (lane == 31) {
+      warp_sums[0][warp] = incl;
+      warp_sums[1][warp] = incl_here;
+    }
+    __syncthreads();
+    uint32_t front = 0, front_here = 0;
+#pragma unroll
+    for (int w = 0; w < kClusterBins / 32; ++w) {
+      front += w < (int)warp ? warp_sums[0][w] : 0;
+      front_here += w < (int)warp ? warp_sums[1][w] : 0;
+    }
+    if (b < bins) {
+      const uint32_t start = front + incl - all;
+      local[b] = front_here + incl_here - here;
+      base[b] = start + before - local[b];            // place of the CTA's item at local place x of this bin: base + x
+      if (SLOTS && last && cta == 0 && b <= (uint32_t)src.limit) offsets[b] = (int64_t)start;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+      const uint32_t i = first + r * 32;
+      if (i >= n) continue;
+      const uint32_t d = (key[r] >> shift) & (bins - 1), x = local[d] + mine[d] + rank[r];
+      skey[x] = key[r];
+      spos[x] = p == 0 ? i : __ldcg(in_pos + i);
+      if constexpr (SLOTS) slot[i] = key[r] < (uint32_t)src.limit ? (int64_t)(base[d] + x) + 1 : 0;   // a single pass: item i is choice i
+    }
+    __syncthreads();
+    const uint32_t start_item = cta * (ROUNDS * kClusterThreads), items = start_item < n ? min(n - start_item, (uint32_t)(ROUNDS * kClusterThreads)) : 0;
+    for (uint32_t x = threadIdx.x; x < items; x += kClusterThreads) {
+      const uint32_t k = skey[x], q = base[(k >> shift) & (bins - 1)] + x;
+      if constexpr (SLOTS) {
+        order[q] = k < (uint32_t)src.limit ? (int64_t)spos[x] + 1 : 0;
+      } else {
+        (from_out ? tkey : out_key)[q] = k;
+        (from_out ? tpos : out_pos)[q] = spos[x];
+      }
+    }
+    // the items are in place for the next pass, and nobody reads this CTA's totals any more
+    cluster.sync();
+  }
+  if (!SLOTS && cta == 0 && threadIdx.x == 0) {
+    out_key[n] = 0xffffffffu;
+    *zero = 0;
+  }
 }
 
 int bits_of(int64_t max_key) {
@@ -332,12 +503,38 @@ size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 int64_t tiles_of(int64_t n) { return (n + kTileItems - 1) / kTileItems; }
 
 template <bool SLOTS>
-int launch_small(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, int64_t *slot, int64_t *order, int64_t *offsets, int passes,
+int launch_small(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, int64_t *slot, int64_t *order, int64_t *offsets, int passes,
                  int digit_bits, cudaStream_t st) {
   const size_t smem = (size_t)(2 * kSmallItems + (kSmallThreads / 32) * (1 << digit_bits)) * sizeof(uint32_t);
   if (smem + 256 > 48 * 1024) THCB_CUDA_TRY(cudaFuncSetAttribute(small_sort_kernel<SLOTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  launch_pdl(small_sort_kernel<SLOTS>, 1, kSmallThreads, smem, st, first_source(in, true), out_key, out_pos, slot, order, offsets,
+  launch_pdl(small_sort_kernel<SLOTS>, 1, kSmallThreads, smem, st, first_source(in, true), out_key, out_pos, zero, slot, order, offsets,
              (uint32_t)in.n, passes, digit_bits);
+  count_launch();
+  THCB_CUDA_TRY(cudaGetLastError());
+  return 0;
+}
+
+template <bool SLOTS>
+int launch_cluster(const SortInput &in, uint32_t *tkey, uint32_t *tpos, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, int64_t *slot, int64_t *order,
+                   int64_t *offsets, int passes, int digit_bits, cudaStream_t st) {
+  const KeySource src = first_source(in, true);
+  const unsigned ctas = in.n <= kClusterFew * kClusterThreads ? kClusterFew : kClusterMany;
+  const int64_t rounds = (in.n + ctas * kClusterThreads - 1) / (ctas * kClusterThreads);
+#define THCB_CLUSTER(R) \
+  do { \
+    auto kernel = cluster_sort_kernel<SLOTS, R>; \
+    const size_t smem = (size_t)(R) * kClusterThreads * 8; \
+    if (smem + 40960 > 48 * 1024) THCB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
+    if (ctas > kClusterFew) THCB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)); \
+    THCB_CUDA_TRY(launch_pdl_cluster(kernel, ctas, ctas, kClusterThreads, smem, st, src, tkey, tpos, out_key, out_pos, zero, slot, order, offsets, \
+                                     (uint32_t)in.n, passes, digit_bits)); \
+  } while (0)
+  if (rounds <= 1) { THCB_CLUSTER(1); }
+  else if (rounds <= 2) { THCB_CLUSTER(2); }
+  else if (rounds <= 4) { THCB_CLUSTER(4); }
+  else if (rounds <= 8) { THCB_CLUSTER(8); }
+  else { THCB_CLUSTER(16); }
+#undef THCB_CLUSTER
   count_launch();
   THCB_CUDA_TRY(cudaGetLastError());
   return 0;
@@ -352,10 +549,10 @@ size_t sort_by_key_bytes(int64_t n, int64_t limit) {
   return align256((size_t)tiles_of(n) * bins * 4) + align256(bins * 4) + 2 * align256(((size_t)n + 1) * 4);
 }
 
-int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, void *ws, cudaStream_t st) {
+int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, void *ws, cudaStream_t st) {
   const int bits = bits_of(in.limit);   // keys 0 .. limit
   if (in.n <= kPairItems) {
-    launch_pdl(pair_sort_kernel<false>, 1, kPairItems, 0, st, first_source(in, true), out_key, out_pos, (int64_t *)nullptr, (int64_t *)nullptr,
+    launch_pdl(pair_sort_kernel<false>, 1, kPairItems, 0, st, first_source(in, true), out_key, out_pos, zero, (int64_t *)nullptr, (int64_t *)nullptr,
                (int64_t *)nullptr, (uint32_t)in.n);
     count_launch();
     THCB_CUDA_TRY(cudaGetLastError());
@@ -363,12 +560,16 @@ int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, void 
   }
   if (in.n <= kSmallItems) {
     const int passes = (bits + 7) / 8;
-    return launch_small<false>(in, out_key, out_pos, nullptr, nullptr, nullptr, passes, (bits + passes - 1) / passes, st);
+    return launch_small<false>(in, out_key, out_pos, zero, nullptr, nullptr, nullptr, passes, (bits + passes - 1) / passes, st);
   }
   const int passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits, digit_bits = (bits + passes - 1) / passes;
   const uint32_t bins = 1u << digit_bits;
   const int64_t tiles = tiles_of(in.n);
   char *w = (char *)ws;
+  if (in.n <= kClusterItems) {
+    uint32_t *tkey = (uint32_t *)w, *tpos = (uint32_t *)(w + align256(((size_t)in.n + 1) * 4));
+    return launch_cluster<false>(in, tkey, tpos, out_key, out_pos, zero, nullptr, nullptr, nullptr, passes, digit_bits, st);
+  }
   uint32_t *hist = (uint32_t *)w;
   w += align256((size_t)tiles * (1u << kMaxDigitBits) * 4);
   uint32_t *totals = (uint32_t *)w;
@@ -386,7 +587,7 @@ int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, void 
     launch_pdl(tile_scan_kernel, (bins + 31) / 32, 1024, 0, st, hist, totals, (int)tiles, bins);
     src.errors = nullptr;
     launch_pdl(tile_scatter_kernel<false>, (unsigned)tiles, kTileThreads, (1 + kTileWarps) * bins * 4, st, src, (const uint32_t *)hist,
-               (const uint32_t *)totals, dk, dp, (int64_t *)nullptr, (int64_t *)nullptr, (int64_t *)nullptr, in.n, shift, bins, p == passes - 1 ? 1 : 0);
+               (const uint32_t *)totals, dk, dp, zero, (int64_t *)nullptr, (int64_t *)nullptr, (int64_t *)nullptr, in.n, shift, bins, p == passes - 1 ? 1 : 0);
     count_launch(3);
     THCB_CUDA_TRY(cudaGetLastError());
     src.key = dk;
@@ -396,21 +597,23 @@ int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, void 
 }
 
 size_t sort_to_slots_bytes(int64_t n, int64_t limit) {
-  if (n <= kPairItems || (n <= kSmallItems && limit < kSmallBins)) return 0;
+  if (n <= kPairItems || (n <= kSmallItems && limit < kSmallBins) || (n <= kClusterItems && limit < kClusterBins)) return 0;
   const size_t bins = pow2_at_least((uint32_t)limit + 1);
   return align256((size_t)tiles_of(n) * bins * 4) + align256(bins * 4);
 }
 
 int sort_to_slots(const SortInput &in, int64_t *slot, int64_t *order, int64_t *offsets, void *ws, cudaStream_t st) {
   if (in.n <= kPairItems) {
-    launch_pdl(pair_sort_kernel<true>, 1, kPairItems, 0, st, first_source(in, true), (uint32_t *)nullptr, (uint32_t *)nullptr, slot, order, offsets,
+    launch_pdl(pair_sort_kernel<true>, 1, kPairItems, 0, st, first_source(in, true), (uint32_t *)nullptr, (uint32_t *)nullptr, (uint32_t *)nullptr, slot, order, offsets,
                (uint32_t)in.n);
     count_launch();
     THCB_CUDA_TRY(cudaGetLastError());
     return 0;
   }
   const int bits = bits_of(in.limit);
-  if (in.n <= kSmallItems && in.limit < kSmallBins) return launch_small<true>(in, nullptr, nullptr, slot, order, offsets, 1, bits, st);
+  if (in.n <= kSmallItems && in.limit < kSmallBins) return launch_small<true>(in, nullptr, nullptr, nullptr, slot, order, offsets, 1, bits, st);
+  if (in.n <= kClusterItems && in.limit < kClusterBins)
+    return launch_cluster<true>(in, nullptr, nullptr, nullptr, nullptr, nullptr, slot, order, offsets, 1, bits, st);
   const uint32_t bins = pow2_at_least((uint32_t)in.limit + 1);
   const int64_t tiles = tiles_of(in.n);
   uint32_t *hist = (uint32_t *)ws, *totals = (uint32_t *)((char *)ws + align256((size_t)tiles * bins * 4));
@@ -421,7 +624,7 @@ int sort_to_slots(const SortInput &in, int64_t *slot, int64_t *order, int64_t *o
   const size_t smem = (size_t)(1 + kTileWarps) * bins * 4;
   if (smem + 256 > 48 * 1024) THCB_CUDA_TRY(cudaFuncSetAttribute(tile_scatter_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   launch_pdl(tile_scatter_kernel<true>, (unsigned)tiles, kTileThreads, smem, st, src, (const uint32_t *)hist, (const uint32_t *)totals,
-             (uint32_t *)nullptr, (uint32_t *)nullptr, slot, order, offsets, in.n, 0, bins, 1);
+             (uint32_t *)nullptr, (uint32_t *)nullptr, (uint32_t *)nullptr, slot, order, offsets, in.n, 0, bins, 1);
   count_launch(3);
   THCB_CUDA_TRY(cudaGetLastError());
   return 0;

@@ -29,8 +29,8 @@ struct SortInput {
 // Workspace of sort_by_key for this many items.
 size_t sort_by_key_bytes(int64_t n, int64_t limit);
 // out_key[p], out_pos[p]: key and item number of the p-th item in (key, item number) order; both hold n entries
-// followed by one sentinel key (0xffffffff) in out_key.
-int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, void *ws, cudaStream_t st);
+// followed by one sentinel key (0xffffffff) in out_key.  *zero becomes 0 on the way.
+int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, void *ws, cudaStream_t st);
 
 // One counting pass over at most kSortMaxBins - 1 keys: slot[i] = 1-based place of item i (0 for an item without a
 // key), order[p] = 1-based item at place p (0 behind the last), offsets[e] = items with a key below e, e = 0 .. limit.
