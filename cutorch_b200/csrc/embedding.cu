@@ -247,19 +247,19 @@ int run_embedding(thcb200_ctx *ctx, const MatView &out, const MatView &w, const 
                   cudaStream_t st) {
   using Math = typename TypeTraits<T>::Math;
   unsigned int *errors = index_errors(ctx);
-  constexpr int VB = 16 / sizeof(T);
-  const bool vec = mat_vec(out, sizeof(T), 16) && mat_vec(w, sizeof(T), 16);
-  const uint64_t vecs = vec ? (uint64_t)out.cols / VB : (uint64_t)out.cols;
+  const int bytes = mat_vec(out, sizeof(T), 32) && mat_vec(w, sizeof(T), 32) ? 32 : mat_vec(out, sizeof(T), 16) && mat_vec(w, sizeof(T), 16) ? 16 : sizeof(T);
+  const uint64_t vecs = (uint64_t)out.cols * sizeof(T) / bytes;
   const uint64_t items = vecs * (uint64_t)out.rows;
   const uint64_t blocks = (items + kLookThreads * kLookUnroll - 1) / (kLookThreads * kLookUnroll);
   if (blocks >= (1ull << 31) || vecs >= (1ull << 31)) { set_error("embedding: tensor too large"); return THCB200_ERR_LIMIT; }
   const FastDiv32 div((uint32_t)vecs);
-  if (vec)
-    launch_pdl(embedding_kernel<T, VB>, (unsigned)blocks, kLookThreads, 0, st, (T *)out.data, (const T *)w.data, index, div, vecs,
-               items, index_stride, w.rows, w.row_stride, (int64_t)1, out.row_stride, (Math)scale, errors);
-  else
-    launch_pdl(embedding_kernel<T, 1>, (unsigned)blocks, kLookThreads, 0, st, (T *)out.data, (const T *)w.data, index, div, vecs,
-               items, index_stride, w.rows, w.row_stride, w.col_stride, out.row_stride, (Math)scale, errors);
+  auto launch = [&](auto kernel) {
+    launch_pdl(kernel, (unsigned)blocks, kLookThreads, 0, st, (T *)out.data, (const T *)w.data, index, div, vecs, items, index_stride, w.rows,
+               w.row_stride, bytes == (int)sizeof(T) ? w.col_stride : (int64_t)1, out.row_stride, (Math)scale, errors);
+  };
+  if (bytes == 32) launch(embedding_kernel<T, 32 / sizeof(T)>);
+  else if (bytes == 16) launch(embedding_kernel<T, 16 / sizeof(T)>);
+  else launch(embedding_kernel<T, 1>);
   count_launch();
   THCB_CUDA_TRY(cudaGetLastError());
   return 0;

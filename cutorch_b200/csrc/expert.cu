@@ -30,8 +30,9 @@ template <typename T> struct RouteArgs {
   const T *src;            // token rows (dispatch) or sorted rows (combine)
   const int64_t *slot;     // [tokens][chosen]
   const typename Weight<T>::type *weight;
-  uint64_t vecs, items;    // vectors per row; tokens * vecs
-  FastDiv32 vecs32;
+  int64_t vecs;            // vectors per row
+  uint64_t per, items;     // items per token (dispatch: vectors; combine: stretches of a row); tokens * per
+  FastDiv32 per32;
   int chosen;
   int64_t places;          // rows on the sorted side
   int64_t dst_stride, src_stride, src_col;
@@ -39,15 +40,15 @@ template <typename T> struct RouteArgs {
 };
 
 template <typename T>
-__device__ __forceinline__ void split_item(const RouteArgs<T> &a, uint64_t i, int64_t *token, int64_t *vec) {
+__device__ __forceinline__ void split_item(const RouteArgs<T> &a, uint64_t i, int64_t *token, int64_t *part) {
   if (a.items <= 0xffffffffull) {
     uint32_t q, r;
-    a.vecs32.divmod((uint32_t)i, q, r);
+    a.per32.divmod((uint32_t)i, q, r);
     *token = q;
-    *vec = r;
+    *part = r;
   } else {
-    *token = (int64_t)(i / a.vecs);
-    *vec = (int64_t)(i - (uint64_t)*token * a.vecs);
+    *token = (int64_t)(i / a.per);
+    *part = (int64_t)(i - (uint64_t)*token * a.per);
   }
 }
 
@@ -85,43 +86,168 @@ dispatch_kernel(RouteArgs<T> a) {
   }
 }
 
-constexpr int kCombineBatch = 4;
+// Rows made of 16-byte vectors.  A warp takes stretches of tokens' rows, one after the other; its lanes read a token's slots
+// and weights, one each, and hand them round.  The rows' vectors come by asynchronous copies into slots of shared memory
+// that belong to the lane that asked for them (no barrier), the copies of one stretch on their way while the one before
+// is summed and the slots of the one after are read: 64 to 128 KiB per SM in flight without a register for them.  Held in registers
+// instead, 8 rows in flight took 100 registers and 112 us where this takes @K8 (16384 tokens x 8 rows of 2048 halves).
+// BATCH rows of G vectors, 32 apart, in a stretch: 8 vectors per lane.
+constexpr int kRingSlots = 8, kRingStages = 2;
+constexpr size_t kRingBytes = (size_t)kRingStages * kRingSlots * kRowThreads * 16;
 
-template <typename T, int V>
+template <typename T, int BATCH>
+__global__ void __launch_bounds__(kRowThreads)
+combine_ring_kernel(RouteArgs<T> a) {
+  using Acc = typename TypeTraits<T>::Acc;
+  using W = typename Weight<T>::type;
+  constexpr int V = 16 / sizeof(T), G = kRingSlots / BATCH;
+  extern __shared__ Bytes16 ring[];        // [stage][slot][thread]
+  pdl_prologue();
+  const uint32_t lane = threadIdx.x & 31;
+  const uint64_t stride = (uint64_t)gridDim.x * (kRowThreads / 32);
+  struct Item {                            // a batch of choices of a stretch
+    uint64_t unit;
+    int64_t token, stretch;
+    int k0;
+    uint32_t valid;                        // choices of the batch that have a place
+    int64_t slot;                          // the lane's choice
+    W weight;
+  };
+  auto read = [&](Item &x) {               // the item's slots and weights; nothing behind the last item
+    x.slot = 0;
+    x.weight = 1;
+    if (x.unit >= a.items) return;
+    split_item(a, x.unit, &x.token, &x.stretch);
+    const int k = x.k0 + (int)lane;
+    if (lane < BATCH && k < a.chosen) {
+      x.slot = a.slot[x.token * a.chosen + k];
+      if (a.weight) x.weight = a.weight[x.token * a.chosen + k];
+    }
+  };
+  auto after = [&](const Item &x) {
+    Item y;
+    y.unit = x.unit;
+    y.k0 = x.k0 + BATCH;
+    if (y.k0 >= a.chosen) {
+      y.unit += stride;
+      y.k0 = 0;
+    }
+    read(y);
+    return y;
+  };
+  auto copy = [&](Item &x, int stage) {
+    if (x.unit < a.items) {
+      const int place = (int)place_of(x.slot, a.places, x.stretch == 0, a.errors);
+      x.valid = __ballot_sync(~0u, place >= 0);
+      const int64_t vec0 = x.stretch * (32 * G) + lane;
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const int p = __shfl_sync(~0u, place, u);
+        if (p < 0) continue;
+        const T *row = a.src + p * a.src_stride + vec0 * V;
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+          if (vec0 + 32 * g < a.vecs)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                         :: "r"((uint32_t)__cvta_generic_to_shared(&ring[(stage * kRingSlots + u * G + g) * kRowThreads + threadIdx.x])), "l"(row + 32 * g * V) : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  Acc acc[G][V];
+  auto sum = [&](const Item &x, int stage) {
+    if (x.k0 == 0) {
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[g][e] = 0;
+    }
+    const int64_t vec0 = x.stretch * (32 * G) + lane;
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const Acc w = (Acc)__shfl_sync(~0u, x.weight, u);
+      if (!(x.valid >> u & 1)) continue;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        if (vec0 + 32 * g >= a.vecs) continue;
+        const Bytes16 b = ring[(stage * kRingSlots + u * G + g) * kRowThreads + threadIdx.x];
+        Pack<T, V> v;
+        memcpy(&v, &b, 16);
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[g][e] += (Acc)to_math(v.e[e]) * w;
+      }
+    }
+    if (x.k0 + BATCH < a.chosen) return;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      if (vec0 + 32 * g >= a.vecs) continue;
+      Pack<T, V> y;
+#pragma unroll
+      for (int e = 0; e < V; ++e) y.e[e] = round_from<T>(acc[g][e]);
+      store_pack<T, V>(a.dst + x.token * a.dst_stride + (vec0 + 32 * g) * V, y);
+    }
+  };
+  Item now, next;
+  now.unit = (uint64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+  now.k0 = 0;
+  read(now);
+  copy(now, 0);
+  next = after(now);
+  for (int stage = 0; now.unit < a.items; stage ^= 1) {
+    copy(next, stage ^ 1);
+    const Item third = after(next);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    sum(now, stage);
+    now = next;
+    next = third;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// Other rows: single elements, G per lane and row, 32 apart.
+template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
 combine_kernel(RouteArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
+  constexpr int G = 4, BATCH = 8;
   pdl_prologue();
-  const uint64_t i = (uint64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  if (i >= a.items) return;
-  int64_t token, vec;
-  split_item(a, i, &token, &vec);
-  Acc acc[V];
+  const uint32_t lane = threadIdx.x & 31;
+  const uint64_t unit = (uint64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+  if (unit >= a.items) return;
+  int64_t token, stretch;
+  split_item(a, unit, &token, &stretch);
+  const int64_t col0 = stretch * (32 * G) + lane;
+  Acc acc[G];
 #pragma unroll
-  for (int e = 0; e < V; ++e) acc[e] = 0;
-  for (int k0 = 0; k0 < a.chosen; k0 += kCombineBatch) {
-    Pack<T, V> x[kCombineBatch];
-    int64_t p[kCombineBatch];
-    Acc w[kCombineBatch];
+  for (int g = 0; g < G; ++g) acc[g] = 0;
+  for (int k0 = 0; k0 < a.chosen; k0 += BATCH) {
+    const int k = k0 + (int)lane;
+    const bool mine = lane < BATCH && k < a.chosen;
+    const int64_t slot = mine ? a.slot[token * a.chosen + k] : 0;
+    const typename Weight<T>::type weight = mine && a.weight ? a.weight[token * a.chosen + k] : 1;
+    const int place = (int)place_of(slot, a.places, stretch == 0, a.errors);
+    T x[BATCH][G];
+    int p[BATCH];
 #pragma unroll
-    for (int u = 0; u < kCombineBatch; ++u) {
-      p[u] = k0 + u < a.chosen ? place_of(a.slot[token * a.chosen + k0 + u], a.places, vec == 0, a.errors) : -1;
-      w[u] = p[u] >= 0 && a.weight ? (Acc)a.weight[token * a.chosen + k0 + u] : (Acc)1;
+    for (int u = 0; u < BATCH; ++u) {
+      p[u] = __shfl_sync(~0u, place, u);
+      if (p[u] < 0) continue;
+      const T *row = a.src + p[u] * a.src_stride;
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+        if (col0 + 32 * g < a.vecs) x[u][g] = row[(col0 + 32 * g) * a.src_col];
     }
 #pragma unroll
-    for (int u = 0; u < kCombineBatch; ++u)
-      if (p[u] >= 0) x[u] = load_pack<T, V>(a.src + p[u] * a.src_stride + vec * V * a.src_col);
-#pragma unroll
-    for (int u = 0; u < kCombineBatch; ++u) {
+    for (int u = 0; u < BATCH; ++u) {
+      const Acc w = (Acc)__shfl_sync(~0u, weight, u);
       if (p[u] < 0) continue;
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] += (Acc)to_math(x[u].e[e]) * w[u];
+      for (int g = 0; g < G; ++g) acc[g] += (Acc)to_math(x[u][g]) * w;
     }
   }
-  Pack<T, V> y;
 #pragma unroll
-  for (int e = 0; e < V; ++e) y.e[e] = round_from<T>(acc[e]);
-  store_pack<T, V>(a.dst + token * a.dst_stride + vec * V, y);
+  for (int g = 0; g < G; ++g)
+    if (col0 + 32 * g < a.vecs) a.dst[token * a.dst_stride + col0 + 32 * g] = round_from<T>(acc[g]);
 }
 
 template <typename T> struct CombineGradArgs {
@@ -140,11 +266,12 @@ template <typename T> struct CombineGradArgs {
 
 // A warp per (token, choice): the token's gradient row is read by the warps of its choices, which sit side by side in the
 // CTA, so all but the first find it in the L1.
-template <typename T, int V>
+template <typename T, int V, bool ROWS, bool DOT>
 __global__ void __launch_bounds__(kRowThreads)
 combine_grad_kernel(CombineGradArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
   using Math = typename TypeTraits<T>::Math;
+  constexpr int B = 4;      // vectors of each row in flight per lane
   pdl_prologue();
   const uint32_t lane = threadIdx.x & 31;
   const uint64_t pair = (uint64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
@@ -155,24 +282,34 @@ combine_grad_kernel(CombineGradArgs<T> a) {
   if (p >= 0) {
     const Math w = a.weight ? (Math)a.weight[pair] : (Math)1;
     const T *g = a.grad + token * a.grad_stride, *r = a.rows + p * a.rows_stride;
-    T *o = a.grad_rows ? a.grad_rows + p * a.out_stride : nullptr;
-#pragma unroll 4
-    for (int64_t v = lane; v < a.vecs; v += 32) {
-      const Pack<T, V> x = *reinterpret_cast<const Pack<T, V> *>(g + v * V * a.grad_col);
-      if (a.grad_weight) {
-        const Pack<T, V> y = load_pack<T, V>(r + v * V * a.rows_col);
+    T *o = ROWS ? a.grad_rows + p * a.out_stride : nullptr;
+    for (int64_t v0 = lane; v0 < a.vecs; v0 += 32 * B) {
+      Pack<T, V> x[B], y[DOT ? B : 1];
 #pragma unroll
-        for (int e = 0; e < V; ++e) dot += (Acc)to_math(x.e[e]) * (Acc)to_math(y.e[e]);
+      for (int u = 0; u < B; ++u) {
+        const int64_t v = v0 + 32 * u;
+        if (v >= a.vecs) continue;
+        x[u] = *reinterpret_cast<const Pack<T, V> *>(g + v * V * a.grad_col);
+        if (DOT) y[u] = load_pack<T, V>(r + v * V * a.rows_col);
       }
-      if (o) {
-        Pack<T, V> y;
 #pragma unroll
-        for (int e = 0; e < V; ++e) y.e[e] = from_math<T>(to_math(x.e[e]) * w);
-        store_pack<T, V>(o + v * V, y);
+      for (int u = 0; u < B; ++u) {
+        const int64_t v = v0 + 32 * u;
+        if (v >= a.vecs) continue;
+        if (DOT) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) dot += (Acc)to_math(x[u].e[e]) * (Acc)to_math(y[u].e[e]);
+        }
+        if (ROWS) {
+          Pack<T, V> z;
+#pragma unroll
+          for (int e = 0; e < V; ++e) z.e[e] = from_math<T>(to_math(x[u].e[e]) * w);
+          store_pack<T, V>(o + v * V, z);
+        }
       }
     }
   }
-  if (!a.grad_weight) return;
+  if (!DOT) return;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(~0u, dot, d);
   if (lane == 0) a.grad_weight[pair] = (typename Weight<T>::type)dot;
@@ -228,11 +365,14 @@ int run_route(thcb200_ctx *ctx, bool dispatch, const MatView &dst, const MatView
   a.src = (const T *)src.data;
   a.slot = s.data;
   a.weight = (const typename Weight<T>::type *)weight;
-  a.vecs = (uint64_t)(vec ? dst.cols / VB : dst.cols);
-  a.items = a.vecs * (uint64_t)s.tokens;
-  const uint64_t blocks = (a.items + kRowThreads - 1) / kRowThreads;
-  if (blocks >= (1ull << 31) || a.vecs >= (1ull << 31)) { set_error("expert rows: tensor too large"); return THCB200_ERR_LIMIT; }
-  a.vecs32 = FastDiv32((uint32_t)a.vecs);
+  a.vecs = vec ? dst.cols / VB : dst.cols;
+  const int batch = s.chosen <= 1 ? 1 : s.chosen <= 2 ? 2 : s.chosen <= 4 ? 4 : 8;
+  const int64_t lane_vecs = vec ? kRingSlots / batch : 4;        // G of the combine kernels
+  a.per = dispatch ? (uint64_t)a.vecs : (uint64_t)((a.vecs + 32 * lane_vecs - 1) / (32 * lane_vecs));
+  a.items = a.per * (uint64_t)s.tokens;
+  const uint64_t per_cta = dispatch ? kRowThreads : kRowThreads / 32, blocks = (a.items + per_cta - 1) / per_cta;
+  if (blocks >= (1ull << 31) || a.vecs >= (1ll << 31) || src.rows >= (1ll << 31)) { set_error("expert rows: tensor too large"); return THCB200_ERR_LIMIT; }
+  a.per32 = FastDiv32((uint32_t)a.per);
   a.chosen = (int)s.chosen;
   a.places = dispatch ? dst.rows : src.rows;
   a.dst_stride = dst.row_stride;
@@ -243,8 +383,19 @@ int run_route(thcb200_ctx *ctx, bool dispatch, const MatView &dst, const MatView
     if (vec) launch_pdl(dispatch_kernel<T, VB>, (unsigned)blocks, kRowThreads, 0, st, a);
     else launch_pdl(dispatch_kernel<T, 1>, (unsigned)blocks, kRowThreads, 0, st, a);
   } else {
-    if (vec) launch_pdl(combine_kernel<T, VB>, (unsigned)blocks, kRowThreads, 0, st, a);
-    else launch_pdl(combine_kernel<T, 1>, (unsigned)blocks, kRowThreads, 0, st, a);
+    if (vec) {
+      const unsigned grid = (unsigned)(blocks < 3 * kNumSM_B200 ? blocks : 3 * kNumSM_B200);
+      auto launch = [&](auto kernel) -> int {
+        THCB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes));
+        launch_pdl(kernel, grid, kRowThreads, kRingBytes, st, a);
+        return 0;
+      };
+      const int rc = batch == 1 ? launch(combine_ring_kernel<T, 1>) : batch == 2 ? launch(combine_ring_kernel<T, 2>)
+                   : batch == 4 ? launch(combine_ring_kernel<T, 4>) : launch(combine_ring_kernel<T, 8>);
+      if (rc) return rc;
+    } else {
+      launch_pdl(combine_kernel<T>, (unsigned)blocks, kRowThreads, 0, st, a);
+    }
   }
   count_launch();
   THCB_CUDA_TRY(cudaGetLastError());
@@ -274,8 +425,12 @@ int run_combine_grad(thcb200_ctx *ctx, const MatView *out, void *grad_weight, co
   a.rows_col = vec ? 1 : rows.col_stride;
   a.errors = index_errors(ctx);
   const unsigned blocks = (unsigned)((a.pairs + kRowThreads / 32 - 1) / (kRowThreads / 32));
-  if (vec) launch_pdl(combine_grad_kernel<T, VB>, blocks, kRowThreads, 0, st, a);
-  else launch_pdl(combine_grad_kernel<T, 1>, blocks, kRowThreads, 0, st, a);
+#define THCB_GRAD(V) \
+  if (out && grad_weight) launch_pdl(combine_grad_kernel<T, V, true, true>, blocks, kRowThreads, 0, st, a); \
+  else if (out) launch_pdl(combine_grad_kernel<T, V, true, false>, blocks, kRowThreads, 0, st, a); \
+  else launch_pdl(combine_grad_kernel<T, V, false, true>, blocks, kRowThreads, 0, st, a)
+  if (vec) { THCB_GRAD(VB); } else { THCB_GRAD(1); }
+#undef THCB_GRAD
   count_launch();
   THCB_CUDA_TRY(cudaGetLastError());
   return 0;

@@ -135,6 +135,7 @@ class State:
     def __init__(self):
         self.lib = _lib.load_library()
         lib = self.lib
+        self._failed = lib.THCB200_errorOccurred
         lib.THCState_alloc.restype = C.c_void_p
         lib.THCudaInit.argtypes = [C.c_void_p]
         lib.THCudaShutdown.argtypes = [C.c_void_p]
@@ -155,7 +156,7 @@ class State:
         self._fn_cache = {}
 
     def check(self):
-        if self.lib.THCB200_errorOccurred():
+        if self._failed():
             msg = self.lib.THCB200_errorMessage().decode()
             self.lib.THCB200_clearError()
             raise THCError(msg)
@@ -424,53 +425,61 @@ class Tensor:
             return creal(float(v))
         return creal(int(v))
 
+    def _prototype(self, f, name: str):
+        """Sets the C prototype of a call's function object once (it belongs to one symbol); per argument, its code and the
+        kind a tensor has to be of."""
+        ret, spec = SIGNATURES[name]
+        creal, cacc = KINDS[self.kind][2], KINDS[self.kind][3]
+        codes = {"r": creal, "l": C.c_long, "f": cacc}
+        f.argtypes = [C.c_void_p] + [codes.get(c, C.c_int if c == "i" else C.c_void_p) for c in spec]
+        f.restype = {"v": None, "a": cacc, "R": creal, "n": C.c_int, "p": C.c_ssize_t}[ret]
+        want = {"L": "Long", "B": "Byte", "A": ACC_KIND.get(self.kind), "T": self.kind, "C": "Long", "M": "Byte"}
+        f.prototype = [(c, want.get(c)) for c in spec]
+        return f.prototype
+
     def call(self, name: str, *args):
         """Calls TH<Kind>Tensor_<name>(state, ...) with `args` exactly in C order."""
-        ret, spec = SIGNATURES[name]
-        if len(args) != len(spec):
+        state = self.state
+        f = state.fn(self.kind, name)
+        try:
+            prototype = f.prototype
+        except AttributeError:
+            prototype = self._prototype(f, name)
+        if len(args) != len(prototype):
+            spec = SIGNATURES[name][1]
             raise TypeError(f"{name} takes {len(spec)} arguments ({spec}), got {len(args)}")
-        f = self.state.fn(self.kind, name)
-        creal, cacc = KINDS[self.kind][2], KINDS[self.kind][3]
-        if not hasattr(f, "prototype"):
-            # a function object belongs to one symbol: its prototype is set once
-            codes = {"r": creal, "l": C.c_long, "f": cacc}
-            f.argtypes = [C.c_void_p] + [codes.get(c, C.c_int if c == "i" else C.c_void_p) for c in spec]
-            f.restype = {"v": None, "a": cacc, "R": creal, "n": C.c_int, "p": C.c_ssize_t}[ret]
-            f.prototype = spec
-        cargs = [self.state.ptr]
-        storages = []
-        for code, a in zip(spec, args):
-            if code == "S":
-                sz = self._long_storage(tuple(a))
-                storages.append(sz)
-                cargs.append(sz)
-                continue
+        cargs = [state.ptr]
+        storages = None
+        for (code, want), a in zip(prototype, args):
             if code in "TLBA":
-                if a is None and code == "A":
+                if isinstance(a, Tensor):
+                    if a.kind != want:
+                        raise TypeError(f"{name}: expected a {want} tensor, got {a.kind}")
+                    cargs.append(a.ptr)
+                elif a is None and code == "A":
                     cargs.append(None)
-                    continue
-                if not isinstance(a, Tensor):
+                else:
                     raise TypeError(f"{name}: expected a tensor")
-                want = {"L": "Long", "B": "Byte", "A": ACC_KIND.get(self.kind)}.get(code, self.kind)
-                if a.kind != want:
-                    raise TypeError(f"{name}: expected a {want} tensor, got {a.kind}")
-                cargs.append(a.ptr)
-            elif code in "CM":
-                want = "Long" if code == "C" else "Byte"
-                if not isinstance(a, CpuTensor) or a.kind != want:
-                    raise TypeError(f"{name}: expected a CPU {want} tensor")
-                cargs.append(a.ptr)
             elif code == "r":
                 cargs.append(self._real(a))
             elif code == "f":
                 cargs.append(float(a))
+            elif code == "S":
+                sz = self._long_storage(tuple(a))
+                storages = (storages or []) + [sz]
+                cargs.append(sz)
+            elif code in "CM":
+                if not isinstance(a, CpuTensor) or a.kind != want:
+                    raise TypeError(f"{name}: expected a CPU {want} tensor")
+                cargs.append(a.ptr)
             else:
                 cargs.append(int(a))
         r = f(*cargs)
-        for sz in storages:
-            self.state.lib.THLongStorage_free(sz)
-        self.state.check()
-        if ret == "R" and self.kind == "Half":
+        if storages:
+            for sz in storages:
+                state.lib.THLongStorage_free(sz)
+        state.check()
+        if self.kind == "Half" and SIGNATURES[name][0] == "R":
             return _half_to_float(r)
         return r
 
@@ -533,11 +542,18 @@ class Tensor:
         f(self.state.ptr, self.ptr, C.c_void_p(result_dev_ptr))
         self.state.check()
 
-    def __getattr__(self, name):
-        # tensor methods in the Lua style: the receiver is the first C argument
-        if name in SIGNATURES:
-            return lambda *args: self.call(name, self, *args)
-        raise AttributeError(name)
+
+def _method(name):
+    # tensor methods in the Lua style: the receiver is the first C argument
+    def method(self, *args):
+        return self.call(name, self, *args)
+    method.__name__ = name
+    return method
+
+
+for _name in SIGNATURES:
+    if not hasattr(Tensor, _name):
+        setattr(Tensor, _name, _method(_name))
 
 
 class TensorList:
