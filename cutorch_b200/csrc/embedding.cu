@@ -9,6 +9,8 @@
 // indexAdd adds in any order and, for half, rounds every addend to 11 bits.
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "context.h"
 #include "core.cuh"
 #include "keysort.h"
@@ -65,9 +67,9 @@ embedding_kernel(T *out, const T *weight, const int64_t *index, FastDiv32 vecs32
 
 // ---- gradient ----------------------------------------------------------------------------------
 constexpr int kGradThreads = 256;
-constexpr int kGradBatch = 8;        // rows in flight per thread
+template <int V, bool ADD> constexpr int kGradBatch = V > 1 && ADD ? 4 : 8;   // rows in flight per thread (and as many of the table's)
 constexpr int kGradMaxChunk = 64;    // sorted tokens per CTA
-constexpr int kZeroRows = 32;        // table rows a CTA checks and clears
+constexpr int kGradKeys = 2048;      // sorted tokens per CTA where rows are narrow and it takes several chunks
 
 template <typename T> struct GradArgs {
   T *table;
@@ -79,6 +81,8 @@ template <typename T> struct GradArgs {
   int64_t tokens, width, rows;
   int64_t grad_stride, grad_col, table_stride;
   uint32_t chunk, chunks;
+  uint32_t group_bits;                       // 2^group_bits threads take a chunk together: 256 for wide rows
+  uint32_t sum_ctas, zero_rows;              // CTAs that sum; table rows that one of the others checks and clears
   typename TypeTraits<T>::Acc scale;
 };
 
@@ -101,15 +105,17 @@ __device__ __forceinline__ void add_partial(typename TypeTraits<T>::Acc (&acc)[V
 // CTAs 0 .. chunks-1 sum the rows named in their chunk of the sorted tokens; the ones behind clear the rows no token
 // names (accumulate = 0).
 template <typename T, int V, bool ADD>
-__global__ void __launch_bounds__(kGradThreads)
+__global__ void __launch_bounds__(kGradThreads, 4)
 embedding_grad_kernel(GradArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
+  constexpr int B = kGradBatch<V, ADD>;
   pdl_prologue();
-  const int64_t col = ((int64_t)blockIdx.y * kGradThreads + threadIdx.x) * V;
-  if (blockIdx.x >= a.chunks) {
-    __shared__ int used[kZeroRows];
-    const int64_t row0 = (int64_t)(blockIdx.x - a.chunks) * kZeroRows;
-    if (threadIdx.x < kZeroRows) {
+  const uint32_t group = 1u << a.group_bits, groups = kGradThreads >> a.group_bits, mine = threadIdx.x >> a.group_bits, member = threadIdx.x & (group - 1);
+  const int64_t col = ((int64_t)blockIdx.y * group + member) * V;
+  extern __shared__ uint32_t grad_smem[];
+  if (blockIdx.x >= a.sum_ctas) {
+    const int64_t row0 = (int64_t)(blockIdx.x - a.sum_ctas) * a.zero_rows;
+    if (threadIdx.x < a.zero_rows) {
       const int64_t row = row0 + threadIdx.x;
       // first sorted key that is not below the row
       int64_t lo = 0, hi = a.tokens;
@@ -117,31 +123,35 @@ embedding_grad_kernel(GradArgs<T> a) {
         const int64_t mid = (lo + hi) >> 1;
         if ((int64_t)a.key[mid] < row) lo = mid + 1; else hi = mid;
       }
-      used[threadIdx.x] = row >= a.rows || (lo < a.tokens && (int64_t)a.key[lo] == row);
+      grad_smem[threadIdx.x] = row >= a.rows || (lo < a.tokens && (int64_t)a.key[lo] == row);
     }
     __syncthreads();
     if (col >= a.width) return;
     Pack<T, V> zero;
 #pragma unroll
     for (int e = 0; e < V; ++e) zero.e[e] = round_from<T>((Acc)0);
-    for (int r = 0; r < kZeroRows; ++r)
-      if (!used[r]) store_pack<T, V>(a.table + (row0 + r) * a.table_stride + col, zero);
+    for (uint32_t r = mine; r < a.zero_rows; r += groups)
+      if (!grad_smem[r]) store_pack<T, V>(a.table + (row0 + r) * a.table_stride + col, zero);
     return;
   }
-  __shared__ uint32_t skey[2 * kGradMaxChunk + 2], spos[2 * kGradMaxChunk];
-  const int64_t begin = (int64_t)blockIdx.x * a.chunk;
-  const uint32_t own = (uint32_t)min((int64_t)a.chunk, a.tokens - begin), seen = (uint32_t)min((int64_t)2 * a.chunk, a.tokens - begin);
+  const uint32_t index = blockIdx.x * groups + mine;            // the group's chunk
+  uint32_t *skey = grad_smem + mine * (2 * a.chunk + 2), *spos = grad_smem + groups * (2 * a.chunk + 2) + mine * 2 * a.chunk;
+  const int64_t begin = (int64_t)index * a.chunk;
+  const uint32_t own = index < a.chunks ? (uint32_t)min((int64_t)a.chunk, a.tokens - begin) : 0;
+  const uint32_t seen = index < a.chunks ? (uint32_t)min((int64_t)2 * a.chunk, a.tokens - begin) : 0;
   // skey[0]: the key in front of the chunk; then the chunk's, the next chunk's, and the one behind (a sentinel ends the list)
-  for (uint32_t i = threadIdx.x; i < seen + 2; i += kGradThreads) {
-    const int64_t p = begin + (int64_t)i - 1;
-    skey[i] = p < 0 ? 0xfffffffeu : a.key[p];
-    if (i >= 1 && i <= seen) spos[i - 1] = a.pos[p];
+  if (own > 0) {
+    for (uint32_t i = member; i < seen + 2; i += group) {
+      const int64_t p = begin + (int64_t)i - 1;
+      skey[i] = p < 0 ? 0xfffffffeu : a.key[p];
+      if (i >= 1 && i <= seen) spos[i - 1] = a.pos[p];
+    }
   }
   const uint32_t none = (uint32_t)a.rows;
   // the row that is under way at the chunk's start, and the one at its end
-  const bool wide_open = begin > a.chunk && a.key[begin - a.chunk - 1] == a.key[begin];   // began before the last chunk
+  const bool wide_open = own > 0 && begin > a.chunk && a.key[begin - a.chunk - 1] == a.key[begin];   // began before the last chunk
   __syncthreads();
-  if (col >= a.width) return;
+  if (col >= a.width || own == 0) return;
   const uint32_t first = skey[1], last = skey[own];
   const bool head = skey[0] == first;
   const bool goes_on = skey[own + 1] == last, far = seen == 2 * a.chunk && skey[2 * a.chunk + 1] == last;
@@ -154,31 +164,31 @@ embedding_grad_kernel(GradArgs<T> a) {
     while (from < own && skey[from + 1] == first) ++from;
   if (goes_on && !tail_long && !(head && first == last))
     while (to < seen && skey[to + 1] == last) ++to;
-  if (blockIdx.y == 0 && threadIdx.x == 0 && tail_long && last != none && !(head && first == last)) {
+  if (blockIdx.y == 0 && member == 0 && tail_long && last != none && !(head && first == last)) {
     // chunks whose first token is the row's: the next two at least
-    int64_t lo = (int64_t)blockIdx.x + 3, hi = a.chunks, reach = 2;
+    int64_t lo = (int64_t)index + 3, hi = a.chunks, reach = 2;
     while (lo + reach < hi && a.key[(lo + reach) * a.chunk] == last) { lo += reach + 1; reach *= 2; }
     hi = min(hi, lo + reach);
     while (lo < hi) {
       const int64_t mid = (lo + hi) >> 1;
       if (a.key[mid * a.chunk] == last) lo = mid + 1; else hi = mid;
     }
-    a.starts[atomicAdd(a.start_count, 1u)] = make_uint4(blockIdx.x, (uint32_t)(lo - 1 - (int64_t)blockIdx.x), last, 0);
+    a.starts[atomicAdd(a.start_count, 1u)] = make_uint4(index, (uint32_t)(lo - 1 - (int64_t)index), last, 0);
   }
   Acc acc[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0;
-  for (uint32_t i = from; i < to; i += kGradBatch) {
-    Pack<T, V> x[kGradBatch], old[ADD ? kGradBatch : 1];
+  for (uint32_t i = from; i < to; i += B) {
+    Pack<T, V> x[B], old[ADD ? B : 1];
 #pragma unroll
-    for (int u = 0; u < kGradBatch; ++u) {
+    for (int u = 0; u < B; ++u) {
       if (i + u >= to || skey[i + u + 1] == none) continue;
       x[u] = load_pack<T, V>(a.grad + (int64_t)spos[i + u] * a.grad_stride + col * a.grad_col);
       // what the sum of a row that ends here is added to comes with the same batch
       if (ADD && (i + u + 1 >= to || skey[i + u + 2] != skey[i + u + 1])) old[u] = load_pack<T, V>(a.table + (int64_t)skey[i + u + 1] * a.table_stride + col);
     }
 #pragma unroll
-    for (int u = 0; u < kGradBatch; ++u) {
+    for (int u = 0; u < B; ++u) {
       if (i + u >= to) break;
       const uint32_t key = skey[i + u + 1];
       if (key == none) return;                                  // items without a row come last
@@ -187,7 +197,7 @@ embedding_grad_kernel(GradArgs<T> a) {
       if (i + u + 1 < to && skey[i + u + 2] == key) continue;
       const bool in_head = head_long && key == first, in_tail = tail_long && key == last;
       if (in_head || in_tail) {
-        Acc *p = a.partial + ((int64_t)blockIdx.x * 2 + (in_head ? 0 : 1)) * a.width + col;
+        Acc *p = a.partial + ((int64_t)index * 2 + (in_head ? 0 : 1)) * a.width + col;
 #pragma unroll
         for (int e = 0; e < V; ++e) p[e] = acc[e];
       } else {
@@ -265,10 +275,10 @@ int run_embedding(thcb200_ctx *ctx, const MatView &out, const MatView &w, const 
   return 0;
 }
 
-uint32_t grad_chunk(int64_t tokens) {
-  // long chunks leave fewer partial sums, short ones give every SM a CTA
+uint32_t grad_chunk(int64_t tokens, uint32_t groups, int64_t slabs) {
+  // long chunks leave fewer partial sums, short ones give every SM several CTAs
   uint32_t c = kGradMaxChunk;
-  while (c > 8 && tokens / c < 8 * kNumSM_B200) c >>= 1;
+  while (c > 8 && (c * groups > kGradKeys || tokens / (c * groups) * slabs < 8 * kNumSM_B200)) c >>= 1;
   return c;
 }
 
@@ -278,10 +288,14 @@ int run_embedding_grad(thcb200_ctx *ctx, const MatView &table, const MatView &gr
   using Acc = typename TypeTraits<T>::Acc;
   constexpr int VB = 16 / sizeof(T);
   const bool vec = mat_vec(table, sizeof(T), 16) && mat_vec(grad, sizeof(T), 16);
-  const uint32_t chunk = grad_chunk(in.n);
-  const int64_t chunks = (in.n + chunk - 1) / chunk;
-  const int64_t zero = accumulate ? 0 : (table.rows + kZeroRows - 1) / kZeroRows;
-  const int64_t slabs = ((vec ? table.cols / VB : table.cols) + kGradThreads - 1) / kGradThreads;
+  const int64_t vecs = vec ? table.cols / VB : table.cols;
+  uint32_t group_bits = 8;
+  while (group_bits > 2 && (1 << (group_bits - 1)) >= vecs) --group_bits;
+  const uint32_t group = 1u << group_bits, groups = kGradThreads >> group_bits, zero_rows = groups >= 8 ? kGradThreads : 32;
+  const int64_t slabs = (vecs + group - 1) / group;
+  const uint32_t chunk = grad_chunk(in.n, groups, slabs);
+  const int64_t chunks = (in.n + chunk - 1) / chunk, sum_ctas = (chunks + groups - 1) / groups;
+  const int64_t zero = accumulate ? 0 : (table.rows + zero_rows - 1) / zero_rows;
   if (chunks + zero >= (1ll << 31) || slabs > 65535) { set_error("embeddingAccGrad: tensor too large"); return THCB200_ERR_LIMIT; }
   const size_t nk = ((size_t)(in.n + 1) * 4 + 255) & ~(size_t)255, np = ((size_t)in.n * 4 + 255) & ~(size_t)255;
   const size_t pb = ((size_t)chunks * 2 * (size_t)table.cols * sizeof(Acc) + 255) & ~(size_t)255, sb = ((size_t)(chunks + 1) * sizeof(uint4) + 255) & ~(size_t)255;
@@ -305,13 +319,17 @@ int run_embedding_grad(thcb200_ctx *ctx, const MatView &table, const MatView &gr
   a.table_stride = table.row_stride;
   a.chunk = chunk;
   a.chunks = (uint32_t)chunks;
+  a.group_bits = group_bits;
+  a.sum_ctas = (uint32_t)sum_ctas;
+  a.zero_rows = zero_rows;
   a.scale = (Acc)scale;
-  const dim3 grid((unsigned)(chunks + zero), (unsigned)slabs);
+  const dim3 grid((unsigned)(sum_ctas + zero), (unsigned)slabs);
+  const size_t smem = std::max((size_t)groups * (4 * chunk + 2), (size_t)zero_rows) * sizeof(uint32_t);   // at most 34 KiB
   const int64_t piece = vec ? 32 * VB : 32, pieces = (table.cols + piece - 1) / piece;
   const unsigned join = (unsigned)(chunks * pieces < 8 * kNumSM_B200 ? chunks * pieces : 8 * kNumSM_B200);
 #define THCB_GRAD(V, ADD) \
   do { \
-    launch_pdl(embedding_grad_kernel<T, V, ADD>, grid, kGradThreads, 0, st, a); \
+    launch_pdl(embedding_grad_kernel<T, V, ADD>, grid, kGradThreads, smem, st, a); \
     if (chunks > 1) launch_pdl(embedding_grad_join_kernel<T, V, ADD>, join, kGradThreads, 0, st, a); \
   } while (0)
   if (vec && accumulate) THCB_GRAD(VB, true);

@@ -1,9 +1,13 @@
 // Stable counting / radix sort of row numbers (see keysort.h).
 //
 // place(i) = #{j : key_j < key_i} + #{j < i : key_j = key_i}: unique, so the result does not depend on how threads are
-// scheduled and everything summed in this order repeats bit for bit.  Up to kSmallItems items one CTA does the whole
-// sort (by counting pairs up to kPairItems, by radix passes in shared memory above); beyond, each pass is three
-// kernels: digit counts of every tile, a scan of those counts over the tiles, and the scatter.
+// scheduled and everything summed in this order repeats bit for bit.  Up to kPairItems items one CTA counts pairs; up to
+// kClusterItems one cluster does all radix passes in one launch; beyond, each pass is three kernels: digit counts of
+// every tile, a scan of those counts over the tiles, and the scatter.  One pass, B200, us back to back in a graph:
+//   items        300   4096   8192  16384  32768  65536  131072  262144
+//   cluster      4.0    4.6    4.6    5.0    7.1    8.8    13.3    22.1    (64 keys; 500 keys: 4.9 .. 26)
+//   tiles                           10.8   10.6   10.9   11.1    11.7    15.7    (500 keys: 12 .. 17)
+// (one CTA's shared memory instead of the cluster: 5.4 at 300 items, 10.8 at 4096.)
 #include "keysort.h"
 
 #include <cooperative_groups.h>
@@ -250,11 +254,6 @@ tile_scatter_kernel(KeySource src, const uint32_t *hist, const uint32_t *totals,
 
 // ---- one CTA -----------------------------------------------------------------------------------
 constexpr int kPairItems = 256;
-constexpr int kSmallThreads = 1024;
-constexpr int kSmallItems = 4096;     // 4 rounds of 32 warps; 32 x 256 counters = 32 KiB of shared memory
-constexpr int kSmallBins = 256;
-constexpr int kSmallRounds = kSmallItems / kSmallThreads;
-
 // Up to kPairItems items: each thread counts the pairs its item comes after.
 template <bool SLOTS>
 __global__ void __launch_bounds__(kPairItems)
@@ -294,76 +293,17 @@ pair_sort_kernel(KeySource src, uint32_t *out_key, uint32_t *out_pos, uint32_t *
   }
 }
 
-// Up to kSmallItems items: radix passes inside one CTA, items in shared memory between the passes.
-template <bool SLOTS>
-__global__ void __launch_bounds__(kSmallThreads)
-small_sort_kernel(KeySource src, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, int64_t *slot, int64_t *order, int64_t *offsets, uint32_t n,
-                  int passes, int digit_bits) {
-  pdl_prologue();
-  extern __shared__ uint32_t sm[];
-  __shared__ uint32_t warp_sums[32];
-  const uint32_t bins = 1u << digit_bits;
-  uint32_t *skey = sm, *spos = sm + kSmallItems;
-  uint32_t *count = spos + kSmallItems;      // [bins][warps]: in this order the scan runs over the bins, then the warps
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr uint32_t W = kSmallThreads / 32;
-  uint32_t key[kSmallRounds], pos[kSmallRounds], rank[kSmallRounds];
-  // a warp's items are consecutive
-  const uint32_t base = warp * (kSmallRounds * 32) + lane;
-  source_keys<kSmallRounds>(key, src, base, 32, n);
-#pragma unroll
-  for (int r = 0; r < kSmallRounds; ++r) pos[r] = base + r * 32;
-  for (int p = 0; p < passes; ++p) {
-    const int shift = p * digit_bits;
-    for (uint32_t i = threadIdx.x; i < bins * W; i += kSmallThreads) count[i] = 0;
-    __syncthreads();
-    warp_ranks<kSmallRounds>(key, shift, digit_bits, base, n, rank, count + warp, W);
-    __syncthreads();
-    cta_exclusive_scan(count, bins * W, kSmallThreads, warp_sums);
-    const bool last = p == passes - 1;
-    if (SLOTS && last)
-      for (uint32_t e = threadIdx.x; e <= (uint32_t)src.limit; e += kSmallThreads) offsets[e] = (int64_t)count[e * W];
-#pragma unroll
-    for (int r = 0; r < kSmallRounds; ++r) {
-      if (base + r * 32 >= n) continue;
-      const uint32_t q = count[((key[r] >> shift) & (bins - 1)) * W + warp] + rank[r];
-      if (!last) {
-        skey[q] = key[r];
-        spos[q] = pos[r];
-      } else if constexpr (SLOTS) {
-        const bool routed = key[r] < (uint32_t)src.limit;
-        slot[pos[r]] = routed ? (int64_t)q + 1 : 0;
-        order[q] = routed ? (int64_t)pos[r] + 1 : 0;
-      } else {
-        out_key[q] = key[r];
-        out_pos[q] = pos[r];
-      }
-    }
-    if (last) break;
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kSmallRounds; ++r) {
-      const uint32_t i = base + r * 32;
-      if (i < n) { key[r] = skey[i]; pos[r] = spos[i]; }
-    }
-  }
-  if (!SLOTS && threadIdx.x == 0) {
-    out_key[n] = 0xffffffffu;
-    *zero = 0;
-  }
-}
-
 // ---- one cluster -------------------------------------------------------------------------------
 // Up to kClusterItems items: eight or sixteen CTAs that wait for one another in hardware, so that all passes fit one launch.
 // Sixteen (more than every GPU grants a cluster, hence the function attribute) where eight would take a second round: a pass is
 // bound by its instructions, about 100 per warp and round.  Items
 // go through global memory between the passes (they stay in the L2), digit counts through distributed shared memory.
 // A CTA first puts its items in order in its own shared memory and then writes each digit's run side by side: with eight
-// SMs the rate of scattered stores is what a pass would wait for (131072 places of one pass: 37 us scattered).
+// or sixteen SMs the rate of scattered stores is part of what a pass waits for.
 constexpr int kClusterFew = 8, kClusterMany = 16;
 constexpr int kClusterThreads = 1024;
 constexpr int kClusterWarps = kClusterThreads / 32;
-constexpr int kClusterMaxRounds = 16;
+constexpr int kClusterMaxRounds = 4;
 constexpr int64_t kClusterItems = (int64_t)kClusterMany * kClusterThreads * kClusterMaxRounds;
 constexpr int kClusterBins = 1 << kMaxDigitBits;
 
@@ -375,7 +315,7 @@ cluster_sort_kernel(KeySource src, uint32_t *tkey, uint32_t *tpos, uint32_t *out
   cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
   extern __shared__ uint4 cluster_smem[];
   uint32_t *skey = reinterpret_cast<uint32_t *>(cluster_smem), *spos = skey + ROUNDS * kClusterThreads;
-  __shared__ __align__(16) uint16_t count[kClusterWarps * kClusterBins];   // at most 512 equal digits in a warp, 16384 in a CTA
+  __shared__ __align__(16) uint16_t count[kClusterWarps * kClusterBins];   // at most 4096 equal digits in a CTA
   __shared__ uint32_t total[kClusterBins], base[kClusterBins], local[kClusterBins], warp_sums[2][32];
   const uint32_t cta = cluster.block_rank(), ctas = cluster.num_blocks(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t bins = 1u << digit_bits;
@@ -503,18 +443,6 @@ size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 int64_t tiles_of(int64_t n) { return (n + kTileItems - 1) / kTileItems; }
 
 template <bool SLOTS>
-int launch_small(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, int64_t *slot, int64_t *order, int64_t *offsets, int passes,
-                 int digit_bits, cudaStream_t st) {
-  const size_t smem = (size_t)(2 * kSmallItems + (kSmallThreads / 32) * (1 << digit_bits)) * sizeof(uint32_t);
-  if (smem + 256 > 48 * 1024) THCB_CUDA_TRY(cudaFuncSetAttribute(small_sort_kernel<SLOTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  launch_pdl(small_sort_kernel<SLOTS>, 1, kSmallThreads, smem, st, first_source(in, true), out_key, out_pos, zero, slot, order, offsets,
-             (uint32_t)in.n, passes, digit_bits);
-  count_launch();
-  THCB_CUDA_TRY(cudaGetLastError());
-  return 0;
-}
-
-template <bool SLOTS>
 int launch_cluster(const SortInput &in, uint32_t *tkey, uint32_t *tpos, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, int64_t *slot, int64_t *order,
                    int64_t *offsets, int passes, int digit_bits, cudaStream_t st) {
   const KeySource src = first_source(in, true);
@@ -531,9 +459,7 @@ int launch_cluster(const SortInput &in, uint32_t *tkey, uint32_t *tpos, uint32_t
   } while (0)
   if (rounds <= 1) { THCB_CLUSTER(1); }
   else if (rounds <= 2) { THCB_CLUSTER(2); }
-  else if (rounds <= 4) { THCB_CLUSTER(4); }
-  else if (rounds <= 8) { THCB_CLUSTER(8); }
-  else { THCB_CLUSTER(16); }
+  else { THCB_CLUSTER(4); }
 #undef THCB_CLUSTER
   count_launch();
   THCB_CUDA_TRY(cudaGetLastError());
@@ -542,11 +468,10 @@ int launch_cluster(const SortInput &in, uint32_t *tkey, uint32_t *tpos, uint32_t
 
 }  // namespace
 
-size_t sort_by_key_bytes(int64_t n, int64_t limit) {
-  if (n <= kSmallItems) return 0;
-  (void)limit;
-  const size_t bins = 1u << kMaxDigitBits;
-  return align256((size_t)tiles_of(n) * bins * 4) + align256(bins * 4) + 2 * align256(((size_t)n + 1) * 4);
+size_t sort_by_key_bytes(int64_t n, int64_t) {
+  if (n <= kPairItems) return 0;
+  const size_t bins = 1u << kMaxDigitBits, items = 2 * align256(((size_t)n + 1) * 4);
+  return n <= kClusterItems ? items : align256((size_t)tiles_of(n) * bins * 4) + align256(bins * 4) + items;
 }
 
 int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, void *ws, cudaStream_t st) {
@@ -557,10 +482,6 @@ int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, uint3
     count_launch();
     THCB_CUDA_TRY(cudaGetLastError());
     return 0;
-  }
-  if (in.n <= kSmallItems) {
-    const int passes = (bits + 7) / 8;
-    return launch_small<false>(in, out_key, out_pos, zero, nullptr, nullptr, nullptr, passes, (bits + passes - 1) / passes, st);
   }
   const int passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits, digit_bits = (bits + passes - 1) / passes;
   const uint32_t bins = 1u << digit_bits;
@@ -597,7 +518,7 @@ int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, uint3
 }
 
 size_t sort_to_slots_bytes(int64_t n, int64_t limit) {
-  if (n <= kPairItems || (n <= kSmallItems && limit < kSmallBins) || (n <= kClusterItems && limit < kClusterBins)) return 0;
+  if (n <= kPairItems || (n <= kClusterItems && limit < kClusterBins)) return 0;
   const size_t bins = pow2_at_least((uint32_t)limit + 1);
   return align256((size_t)tiles_of(n) * bins * 4) + align256(bins * 4);
 }
@@ -611,7 +532,6 @@ int sort_to_slots(const SortInput &in, int64_t *slot, int64_t *order, int64_t *o
     return 0;
   }
   const int bits = bits_of(in.limit);
-  if (in.n <= kSmallItems && in.limit < kSmallBins) return launch_small<true>(in, nullptr, nullptr, nullptr, slot, order, offsets, 1, bits, st);
   if (in.n <= kClusterItems && in.limit < kClusterBins)
     return launch_cluster<true>(in, nullptr, nullptr, nullptr, nullptr, nullptr, slot, order, offsets, 1, bits, st);
   const uint32_t bins = pow2_at_least((uint32_t)in.limit + 1);
