@@ -60,7 +60,7 @@ template <int N> struct StepTable {
   int count;
   StepEntry e[N];
 };
-constexpr int kFewTensors = 16, kManyTensors = 320;           // 1 KiB / 22.5 KiB of arguments
+constexpr int kFewTensors = 16, kManyTensors = 320;           // 1 KiB / 22.5 KiB of arguments: a launch takes 2 us longer with the latter
 
 template <typename A> struct StepScalars { A beta1, one_minus_beta1, beta2, one_minus_beta2, keep, size, root, eps, grad_scale; uint32_t dither; };
 
@@ -486,16 +486,53 @@ bool on_grid(const void *p, size_t esz) {
   return (uintptr_t)p % bytes == 0;
 }
 
-// Two arrays that share memory, one of them written, would make the step depend on the order of threads.  Lists of
-// pieces of one buffer come in address order; anything else is sorted.
+// Two arrays that share memory, one of them written, would make the step depend on the order of threads.  The arrays of one
+// kind mostly are pieces of one buffer in address order: each kind's are sorted if need be, and the kinds then merged,
+// which is only walked through where their spans meet.
 struct Range { uintptr_t lo, hi; };
-bool overlap(std::vector<Range> &r) {
-  if (!std::is_sorted(r.begin(), r.end(), [](const Range &a, const Range &b) { return a.lo < b.lo; }))
-    std::sort(r.begin(), r.end(), [](const Range &a, const Range &b) { return a.lo < b.lo; });
-  for (size_t i = 1; i < r.size(); ++i)
-    if (r[i].lo < r[i - 1].hi) return true;
-  return false;
-}
+struct Ranges {
+  static constexpr int kKinds = 7;
+  std::vector<Range> r;
+  size_t first[kKinds + 1] = {};
+  bool written[kKinds] = {};
+  int kinds = 0;
+  void add(const void *p, size_t bytes) { r.push_back(Range{(uintptr_t)p, (uintptr_t)p + bytes}); }
+  void close_kind(bool is_written) {
+    if (r.size() == first[kinds]) return;
+    written[kinds] = is_written;
+    first[++kinds] = r.size();
+  }
+  bool overlap() {
+    const auto before = [](const Range &a, const Range &b) { return a.lo < b.lo; };
+    Range span[kKinds];
+    for (int k = 0; k < kinds; ++k) {
+      const auto b = r.begin() + (ptrdiff_t)first[k], e = r.begin() + (ptrdiff_t)first[k + 1];
+      if (!std::is_sorted(b, e, before)) std::sort(b, e, before);
+      span[k] = *b;
+      for (auto i = b + 1; i < e; ++i) {
+        if (written[k] && i->lo < (i - 1)->hi) return true;
+        span[k].hi = std::max(span[k].hi, i->hi);
+      }
+    }
+    std::sort(span, span + kinds, before);
+    bool apart = true;
+    for (int k = 1; k < kinds; ++k) apart = apart && span[k].lo >= span[k - 1].hi;
+    if (apart) return false;
+    size_t at[kKinds];
+    for (int k = 0; k < kinds; ++k) at[k] = first[k];
+    uintptr_t reach = 0, reach_written = 0;   // ends of the arrays met so far
+    for (size_t n = 0; n < r.size(); ++n) {
+      int least = -1;
+      for (int k = 0; k < kinds; ++k)
+        if (at[k] < first[k + 1] && (least < 0 || r[at[k]].lo < r[at[least]].lo)) least = k;
+      const Range &x = r[at[least]++];
+      if (x.lo < (written[least] ? reach : reach_written)) return true;
+      reach = std::max(reach, x.hi);
+      if (written[least]) reach_written = std::max(reach_written, x.hi);
+    }
+    return false;
+  }
+};
 
 enum StepKind { kStep32, kStep8, kStepValues };
 
@@ -587,24 +624,27 @@ int run_step_typed(const thcb200_adamw_tensor *t, int count, int bits, bool mast
 
 int check_list(const thcb200_adamw_tensor *t, int n, size_t esz, StepKind kind, bool master, const char *name) {
   const size_t wsz = esz == 8 ? 8 : 4, msz = kind == kStep32 ? wsz : 1;
-  std::vector<Range> ranges;
-  ranges.reserve((size_t)n * (master ? 6 : 5) + 1);
-  auto add = [&](const void *p, size_t bytes) { ranges.push_back(Range{(uintptr_t)p, (uintptr_t)p + bytes}); };
-  for (int pass = 0; pass < 6; ++pass) {
-    for (int i = 0; i < n; ++i) {
+  Ranges ranges;
+  ranges.r.reserve((size_t)n * Ranges::kKinds + 1);
+  const bool values = kind == kStepValues;
+  for (int what = 0; what < Ranges::kKinds; ++what) {
+    const bool there = what < 3 || (what == 3 && !values) || (what == 4 && (master || values)) || (what > 4 && kind != kStep32);
+    for (int i = 0; there && i < n; ++i) {
       const size_t k = (size_t)t[i].numel, blocks = (k + kUnitItems - 1) / kUnitItems;
       if (k == 0) continue;
-      switch (pass) {
-        case 0: add(t[i].param, k * (kind == kStepValues ? 4 : esz)); break;
-        case 1: add(t[i].m, k * msz); break;
-        case 2: add(t[i].v, k * msz); break;
-        case 3: if (master || kind == kStepValues) add(t[i].master, k * (kind == kStepValues ? 4 : wsz)); break;
-        case 4: if (kind != kStep32) add(t[i].m_unit, blocks * 4); break;
-        default: if (kind != kStep32) add(t[i].v_unit, blocks * 4); break;
+      switch (what) {
+        case 0: ranges.add(t[i].param, k * (values ? 4 : esz)); break;
+        case 1: ranges.add(t[i].m, k * msz); break;
+        case 2: ranges.add(t[i].v, k * msz); break;
+        case 3: ranges.add(t[i].grad, k * esz); break;
+        case 4: ranges.add(t[i].master, k * (values ? 4 : wsz)); break;
+        case 5: ranges.add(t[i].m_unit, blocks * 4); break;
+        default: ranges.add(t[i].v_unit, blocks * 4); break;
       }
     }
+    ranges.close_kind(values ? what == 0 || what == 4 : what != 3);
   }
-  if (overlap(ranges)) { set_error("%s: two of the tensors share memory (a tensor may be listed once)", name); return THCB200_ERR_ARG; }
+  if (ranges.overlap()) { set_error("%s: a tensor that is written shares memory with another (each may be listed once)", name); return THCB200_ERR_ARG; }
   return 0;
 }
 

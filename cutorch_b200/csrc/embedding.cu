@@ -23,6 +23,14 @@ namespace {
 constexpr int kLookThreads = 256;
 constexpr int kLookUnroll = 4;
 
+// Row of token i, or the row count where it has none.
+__device__ __forceinline__ uint32_t row_key(const SortInput &in, int64_t i, bool count) {
+  const int64_t raw = in.index[i * in.stride], k = raw - 1;   // positions are 1-based (TH_INDEX_BASE)
+  const bool row = (uint64_t)k < (uint64_t)in.limit, skip = in.skip != 0 && raw == in.skip;
+  if (!row && !skip && count) atomicAdd(in.errors, 1u);
+  return row && !skip ? (uint32_t)k : (uint32_t)in.limit;
+}
+
 // One vector of V elements per item, kLookUnroll items per thread: the positions come first, then all row loads are in
 // flight together.
 template <typename T, int V>
@@ -75,6 +83,7 @@ template <typename T> struct GradArgs {
   T *table;
   const T *grad;
   const uint32_t *key, *pos;
+  SortInput index;                           // the positions themselves, for few tokens
   typename TypeTraits<T>::Acc *partial;      // [chunk][head, tail][width]
   uint32_t *start_count;                     // rows that lie across more than two chunks
   uint4 *starts;                             // for each: the chunk it begins in, the chunks behind that, its key
@@ -104,7 +113,11 @@ __device__ __forceinline__ void add_partial(typename TypeTraits<T>::Acc (&acc)[V
 
 // CTAs 0 .. chunks-1 sum the rows named in their chunk of the sorted tokens; the ones behind clear the rows no token
 // names (accumulate = 0).
-template <typename T, int V, bool ADD>
+// FEW: every CTA puts all tokens (at most kFewTokens) in order itself, and a row is summed by the chunk it begins in however
+// long it is: no sort before and no join behind.
+constexpr int kFewTokens = 128;
+
+template <typename T, int V, bool ADD, bool FEW>
 __global__ void __launch_bounds__(kGradThreads, 4)
 embedding_grad_kernel(GradArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
@@ -113,6 +126,25 @@ embedding_grad_kernel(GradArgs<T> a) {
   const uint32_t group = 1u << a.group_bits, groups = kGradThreads >> a.group_bits, mine = threadIdx.x >> a.group_bits, member = threadIdx.x & (group - 1);
   const int64_t col = ((int64_t)blockIdx.y * group + member) * V;
   extern __shared__ uint32_t grad_smem[];
+  __shared__ uint32_t few_raw[FEW ? kFewTokens : 1], few_key[FEW ? kFewTokens + 2 : 1], few_pos[FEW ? kFewTokens : 1];
+  if constexpr (FEW) {
+    const uint32_t i = threadIdx.x, n = (uint32_t)a.tokens;
+    if (i < n) few_raw[i] = row_key(a.index, i, blockIdx.x == 0 && blockIdx.y == 0);
+    __syncthreads();
+    if (i < n) {
+      const uint32_t k = few_raw[i];
+      uint32_t place = 0;
+      for (uint32_t j = 0; j < n; ++j) place += few_raw[j] < k || (few_raw[j] == k && j < i) ? 1u : 0u;
+      few_key[place + 1] = k;
+      few_pos[place] = i;
+    }
+    if (i == 0) {
+      few_key[0] = 0xfffffffeu;
+      few_key[n + 1] = 0xffffffffu;
+    }
+    __syncthreads();
+  }
+  const uint32_t *sorted = FEW ? few_key + 1 : a.key;
   if (blockIdx.x >= a.sum_ctas) {
     const int64_t row0 = (int64_t)(blockIdx.x - a.sum_ctas) * a.zero_rows;
     if (threadIdx.x < a.zero_rows) {
@@ -121,9 +153,9 @@ embedding_grad_kernel(GradArgs<T> a) {
       int64_t lo = 0, hi = a.tokens;
       while (lo < hi) {
         const int64_t mid = (lo + hi) >> 1;
-        if ((int64_t)a.key[mid] < row) lo = mid + 1; else hi = mid;
+        if ((int64_t)sorted[mid] < row) lo = mid + 1; else hi = mid;
       }
-      grad_smem[threadIdx.x] = row >= a.rows || (lo < a.tokens && (int64_t)a.key[lo] == row);
+      grad_smem[threadIdx.x] = row >= a.rows || (lo < a.tokens && (int64_t)sorted[lo] == row);
     }
     __syncthreads();
     if (col >= a.width) return;
@@ -135,12 +167,13 @@ embedding_grad_kernel(GradArgs<T> a) {
     return;
   }
   const uint32_t index = blockIdx.x * groups + mine;            // the group's chunk
-  uint32_t *skey = grad_smem + mine * (2 * a.chunk + 2), *spos = grad_smem + groups * (2 * a.chunk + 2) + mine * 2 * a.chunk;
   const int64_t begin = (int64_t)index * a.chunk;
+  uint32_t *skey = FEW ? few_key + min(begin, a.tokens) : grad_smem + mine * (2 * a.chunk + 2);
+  uint32_t *spos = FEW ? few_pos + min(begin, a.tokens) : grad_smem + groups * (2 * a.chunk + 2) + mine * 2 * a.chunk;
   const uint32_t own = index < a.chunks ? (uint32_t)min((int64_t)a.chunk, a.tokens - begin) : 0;
-  const uint32_t seen = index < a.chunks ? (uint32_t)min((int64_t)2 * a.chunk, a.tokens - begin) : 0;
+  const uint32_t seen = index < a.chunks ? (uint32_t)min(FEW ? a.tokens : (int64_t)2 * a.chunk, a.tokens - begin) : 0;
   // skey[0]: the key in front of the chunk; then the chunk's, the next chunk's, and the one behind (a sentinel ends the list)
-  if (own > 0) {
+  if (!FEW && own > 0) {
     for (uint32_t i = member; i < seen + 2; i += group) {
       const int64_t p = begin + (int64_t)i - 1;
       skey[i] = p < 0 ? 0xfffffffeu : a.key[p];
@@ -149,22 +182,22 @@ embedding_grad_kernel(GradArgs<T> a) {
   }
   const uint32_t none = (uint32_t)a.rows;
   // the row that is under way at the chunk's start, and the one at its end
-  const bool wide_open = own > 0 && begin > a.chunk && a.key[begin - a.chunk - 1] == a.key[begin];   // began before the last chunk
+  const bool wide_open = !FEW && own > 0 && begin > a.chunk && a.key[begin - a.chunk - 1] == a.key[begin];   // began before the last chunk
   __syncthreads();
   if (col >= a.width || own == 0) return;
   const uint32_t first = skey[1], last = skey[own];
   const bool head = skey[0] == first;
-  const bool goes_on = skey[own + 1] == last, far = seen == 2 * a.chunk && skey[2 * a.chunk + 1] == last;
+  const bool goes_on = skey[own + 1] == last, far = !FEW && seen == 2 * a.chunk && skey[2 * a.chunk + 1] == last;
   // A row that began in the last chunk and ends in this one was that chunk's; one that lies across more chunks leaves its
   // sum over this one for the join.
-  const bool head_long = head && (wide_open || (goes_on && first == last));
+  const bool head_long = !FEW && head && (wide_open || (goes_on && first == last));
   const bool tail_long = goes_on && far;               // a row that began here: it does not end in the next chunk either
   uint32_t from = 0, to = own;
   if (head && !head_long)
     while (from < own && skey[from + 1] == first) ++from;
   if (goes_on && !tail_long && !(head && first == last))
     while (to < seen && skey[to + 1] == last) ++to;
-  if (blockIdx.y == 0 && member == 0 && tail_long && last != none && !(head && first == last)) {
+  if (!FEW && blockIdx.y == 0 && member == 0 && tail_long && last != none && !(head && first == last)) {
     // chunks whose first token is the row's: the next two at least
     int64_t lo = (int64_t)index + 3, hi = a.chunks, reach = 2;
     while (lo + reach < hi && a.key[(lo + reach) * a.chunk] == last) { lo += reach + 1; reach *= 2; }
@@ -299,16 +332,20 @@ int run_embedding_grad(thcb200_ctx *ctx, const MatView &table, const MatView &gr
   if (chunks + zero >= (1ll << 31) || slabs > 65535) { set_error("embeddingAccGrad: tensor too large"); return THCB200_ERR_LIMIT; }
   const size_t nk = ((size_t)(in.n + 1) * 4 + 255) & ~(size_t)255, np = ((size_t)in.n * 4 + 255) & ~(size_t)255;
   const size_t pb = ((size_t)chunks * 2 * (size_t)table.cols * sizeof(Acc) + 255) & ~(size_t)255, sb = ((size_t)(chunks + 1) * sizeof(uint4) + 255) & ~(size_t)255;
-  Workspace ws(ctx, nk + np + pb + sb + sort_by_key_bytes(in.n, in.limit), st);
+  const bool few = in.n <= kFewTokens;
+  Workspace ws(ctx, few ? 0 : nk + np + pb + sb + sort_by_key_bytes(in.n, in.limit), st);
   if (!ws.ok) return THCB200_ERR_NOMEM;
   GradArgs<T> a;
+  a.index = in;
   a.key = (uint32_t *)ws.data;
   a.pos = (uint32_t *)(ws.data + nk);
   a.partial = (Acc *)(ws.data + nk + np);
   a.start_count = (uint32_t *)(ws.data + nk + np + pb);
   a.starts = (uint4 *)a.start_count + 1;
-  int rc = sort_by_key(in, (uint32_t *)a.key, (uint32_t *)a.pos, a.start_count, ws.data + nk + np + pb + sb, st);
-  if (rc) return rc;
+  if (!few) {
+    const int rc = sort_by_key(in, (uint32_t *)a.key, (uint32_t *)a.pos, a.start_count, ws.data + nk + np + pb + sb, st);
+    if (rc) return rc;
+  }
   a.table = (T *)table.data;
   a.grad = (const T *)grad.data;
   a.tokens = in.n;
@@ -327,17 +364,22 @@ int run_embedding_grad(thcb200_ctx *ctx, const MatView &table, const MatView &gr
   const size_t smem = std::max((size_t)groups * (4 * chunk + 2), (size_t)zero_rows) * sizeof(uint32_t);   // at most 34 KiB
   const int64_t piece = vec ? 32 * VB : 32, pieces = (table.cols + piece - 1) / piece;
   const unsigned join = (unsigned)(chunks * pieces < 8 * kNumSM_B200 ? chunks * pieces : 8 * kNumSM_B200);
+  const bool joined = !few && chunks > 2;      // a row across more than two chunks needs three
 #define THCB_GRAD(V, ADD) \
   do { \
-    launch_pdl(embedding_grad_kernel<T, V, ADD>, grid, kGradThreads, smem, st, a); \
-    if (chunks > 1) launch_pdl(embedding_grad_join_kernel<T, V, ADD>, join, kGradThreads, 0, st, a); \
+    if (few) { \
+      launch_pdl(embedding_grad_kernel<T, V, ADD, true>, grid, kGradThreads, smem, st, a); \
+    } else { \
+      launch_pdl(embedding_grad_kernel<T, V, ADD, false>, grid, kGradThreads, smem, st, a); \
+      if (joined) launch_pdl(embedding_grad_join_kernel<T, V, ADD>, join, kGradThreads, 0, st, a); \
+    } \
   } while (0)
   if (vec && accumulate) THCB_GRAD(VB, true);
   else if (vec) THCB_GRAD(VB, false);
   else if (accumulate) THCB_GRAD(1, true);
   else THCB_GRAD(1, false);
 #undef THCB_GRAD
-  count_launch(chunks > 1 ? 2 : 1);
+  count_launch(joined ? 2 : 1);
   THCB_CUDA_TRY(cudaGetLastError());
   return 0;
 }

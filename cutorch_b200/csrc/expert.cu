@@ -32,6 +32,7 @@ template <typename T> struct RouteArgs {
   const typename Weight<T>::type *weight;
   int64_t vecs;            // vectors per row
   uint64_t per, items;     // items per token (dispatch: vectors; combine: stretches of a row); tokens * per
+  uint32_t team;           // lanes that take a stretch together: 32, or 8 or 16 where a row has no more vectors
   FastDiv32 per32;
   int chosen;
   int64_t places;          // rows on the sorted side
@@ -86,7 +87,7 @@ dispatch_kernel(RouteArgs<T> a) {
   }
 }
 
-// Rows made of 16-byte vectors.  A warp takes stretches of tokens' rows, one after the other; its lanes read a token's slots
+// Rows made of 16-byte vectors.  A warp (for narrow rows, a team of 8 or 16 lanes) takes stretches of tokens' rows, one after the other; its lanes read a token's slots
 // and weights, one each, and hand them round.  The rows' vectors come by asynchronous copies into slots of shared memory
 // that belong to the lane that asked for them (no barrier), the copies of one stretch on their way while the one before
 // is summed and the slots of the one after are read: 64 to 128 KiB per SM in flight without a register for them.  Held in registers
@@ -103,8 +104,8 @@ combine_ring_kernel(RouteArgs<T> a) {
   constexpr int V = 16 / sizeof(T), G = kRingSlots / BATCH;
   extern __shared__ Bytes16 ring[];        // [stage][slot][thread]
   pdl_prologue();
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t stride = (uint64_t)gridDim.x * (kRowThreads / 32);
+  const uint32_t team = a.team, lane = threadIdx.x & (team - 1), teams = 32 / team;
+  const uint64_t stride = (uint64_t)gridDim.x * (kRowThreads / 32) * teams;
   struct Item {                            // a batch of choices of a stretch
     uint64_t unit;
     int64_t token, stretch;
@@ -116,6 +117,7 @@ combine_ring_kernel(RouteArgs<T> a) {
   auto read = [&](Item &x) {               // the item's slots and weights; nothing behind the last item
     x.slot = 0;
     x.weight = 1;
+    x.token = x.stretch = 0;
     if (x.unit >= a.items) return;
     split_item(a, x.unit, &x.token, &x.stretch);
     const int k = x.k0 + (int)lane;
@@ -136,21 +138,19 @@ combine_ring_kernel(RouteArgs<T> a) {
     return y;
   };
   auto copy = [&](Item &x, int stage) {
-    if (x.unit < a.items) {
-      const int place = (int)place_of(x.slot, a.places, x.stretch == 0, a.errors);
-      x.valid = __ballot_sync(~0u, place >= 0);
-      const int64_t vec0 = x.stretch * (32 * G) + lane;
+    const int place = (int)place_of(x.slot, a.places, x.stretch == 0, a.errors);      // no slot behind the last item
+    x.valid = __ballot_sync(~0u, place >= 0) >> (threadIdx.x & 31 & ~(team - 1));
+    const int64_t vec0 = x.stretch * (team * G) + lane;
 #pragma unroll
-      for (int u = 0; u < BATCH; ++u) {
-        const int p = __shfl_sync(~0u, place, u);
-        if (p < 0) continue;
-        const T *row = a.src + p * a.src_stride + vec0 * V;
+    for (int u = 0; u < BATCH; ++u) {
+      const int p = __shfl_sync(~0u, place, u, team);
+      if (p < 0) continue;
+      const T *row = a.src + p * a.src_stride + vec0 * V;
 #pragma unroll
-        for (int g = 0; g < G; ++g)
-          if (vec0 + 32 * g < a.vecs)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                         :: "r"((uint32_t)__cvta_generic_to_shared(&ring[(stage * kRingSlots + u * G + g) * kRowThreads + threadIdx.x])), "l"(row + 32 * g * V) : "memory");
-      }
+      for (int g = 0; g < G; ++g)
+        if (vec0 + team * g < a.vecs)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                       :: "r"((uint32_t)__cvta_generic_to_shared(&ring[(stage * kRingSlots + u * G + g) * kRowThreads + threadIdx.x])), "l"(row + team * g * V) : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -162,14 +162,14 @@ combine_ring_kernel(RouteArgs<T> a) {
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[g][e] = 0;
     }
-    const int64_t vec0 = x.stretch * (32 * G) + lane;
+    const int64_t vec0 = x.stretch * (team * G) + lane;
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
-      const Acc w = (Acc)__shfl_sync(~0u, x.weight, u);
+      const Acc w = (Acc)__shfl_sync(~0u, x.weight, u, team);
       if (!(x.valid >> u & 1)) continue;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        if (vec0 + 32 * g >= a.vecs) continue;
+        if (vec0 + team * g >= a.vecs) continue;
         const Bytes16 b = ring[(stage * kRingSlots + u * G + g) * kRowThreads + threadIdx.x];
         Pack<T, V> v;
         memcpy(&v, &b, 16);
@@ -177,23 +177,24 @@ combine_ring_kernel(RouteArgs<T> a) {
         for (int e = 0; e < V; ++e) acc[g][e] += (Acc)to_math(v.e[e]) * w;
       }
     }
-    if (x.k0 + BATCH < a.chosen) return;
+    if (x.k0 + BATCH < a.chosen || x.unit >= a.items) return;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      if (vec0 + 32 * g >= a.vecs) continue;
+      if (vec0 + team * g >= a.vecs) continue;
       Pack<T, V> y;
 #pragma unroll
       for (int e = 0; e < V; ++e) y.e[e] = round_from<T>(acc[g][e]);
-      store_pack<T, V>(a.dst + x.token * a.dst_stride + (vec0 + 32 * g) * V, y);
+      store_pack<T, V>(a.dst + x.token * a.dst_stride + (vec0 + team * g) * V, y);
     }
   };
   Item now, next;
-  now.unit = (uint64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+  now.unit = ((uint64_t)blockIdx.x * kRowThreads + threadIdx.x) / team;
   now.k0 = 0;
   read(now);
   copy(now, 0);
   next = after(now);
-  for (int stage = 0; now.unit < a.items; stage ^= 1) {
+  // all teams of a warp go as far as its first, which never has fewer items than they
+  for (int stage = 0; __shfl_sync(~0u, now.unit, 0) < a.items; stage ^= 1) {
     copy(next, stage ^ 1);
     const Item third = after(next);
     asm volatile("cp.async.wait_group 1;" ::: "memory");
@@ -259,42 +260,44 @@ template <typename T> struct CombineGradArgs {
   uint64_t pairs;
   int64_t vecs;
   FastDiv32 chosen;
+  uint32_t team_bits;                          // 2^team_bits lanes take a pair together
   int64_t places;
   int64_t out_stride, grad_stride, grad_col, rows_stride, rows_col;
   unsigned int *errors;
 };
 
-// A warp per (token, choice): the token's gradient row is read by the warps of its choices, which sit side by side in the
+// A warp (for narrow rows, a team of 4, 8 or 16 lanes) per (token, choice): the token's gradient row is read by the warps of its choices, which sit side by side in the
 // CTA, so all but the first find it in the L1.
-template <typename T, int V, bool ROWS, bool DOT>
+template <typename T, int V, bool ROWS, bool DOT, bool TEAMS>
 __global__ void __launch_bounds__(kRowThreads)
 combine_grad_kernel(CombineGradArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
   using Math = typename TypeTraits<T>::Math;
-  constexpr int B = 4;      // vectors of each row in flight per lane
+  constexpr int B = sizeof(T) == 8 ? 4 : 2;      // vectors of each row in flight per lane (measured best of 2 and 4)
   pdl_prologue();
-  const uint32_t lane = threadIdx.x & 31;
-  const uint64_t pair = (uint64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
-  if (pair >= a.pairs) return;
-  const int64_t token = a.chosen.div((uint32_t)pair);
-  const int64_t p = place_of(a.slot[pair], a.places, lane == 0, a.errors);
+  const uint32_t team_bits = TEAMS ? a.team_bits : 5, team = 1u << team_bits, lane = threadIdx.x & (team - 1);
+  const uint64_t pair = ((uint64_t)blockIdx.x * kRowThreads + threadIdx.x) >> team_bits;
+  if (((uint64_t)blockIdx.x * kRowThreads + (threadIdx.x & ~31u)) >> team_bits >= a.pairs) return;   // whole warps
+  const bool there = pair < a.pairs;
+  const int64_t token = there ? a.chosen.div((uint32_t)pair) : 0;
+  const int64_t p = there ? place_of(a.slot[pair], a.places, lane == 0, a.errors) : -1;
   Acc dot = 0;
   if (p >= 0) {
     const Math w = a.weight ? (Math)a.weight[pair] : (Math)1;
     const T *g = a.grad + token * a.grad_stride, *r = a.rows + p * a.rows_stride;
     T *o = ROWS ? a.grad_rows + p * a.out_stride : nullptr;
-    for (int64_t v0 = lane; v0 < a.vecs; v0 += 32 * B) {
+    for (int64_t v0 = lane; v0 < a.vecs; v0 += team * B) {
       Pack<T, V> x[B], y[DOT ? B : 1];
 #pragma unroll
       for (int u = 0; u < B; ++u) {
-        const int64_t v = v0 + 32 * u;
+        const int64_t v = v0 + team * u;
         if (v >= a.vecs) continue;
-        x[u] = *reinterpret_cast<const Pack<T, V> *>(g + v * V * a.grad_col);
+        x[u] = load_kept<T, V>(g + v * V * a.grad_col);
         if (DOT) y[u] = load_pack<T, V>(r + v * V * a.rows_col);
       }
 #pragma unroll
       for (int u = 0; u < B; ++u) {
-        const int64_t v = v0 + 32 * u;
+        const int64_t v = v0 + team * u;
         if (v >= a.vecs) continue;
         if (DOT) {
 #pragma unroll
@@ -311,8 +314,9 @@ combine_grad_kernel(CombineGradArgs<T> a) {
   }
   if (!DOT) return;
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(~0u, dot, d);
-  if (lane == 0) a.grad_weight[pair] = (typename Weight<T>::type)dot;
+  for (uint32_t d = 16; d > 0; d >>= 1)
+    if (d < team) dot += __shfl_xor_sync(~0u, dot, d);
+  if (lane == 0 && there) a.grad_weight[pair] = (typename Weight<T>::type)dot;
 }
 
 // ---- host --------------------------------------------------------------------------------------
@@ -367,10 +371,11 @@ int run_route(thcb200_ctx *ctx, bool dispatch, const MatView &dst, const MatView
   a.weight = (const typename Weight<T>::type *)weight;
   a.vecs = vec ? dst.cols / VB : dst.cols;
   const int batch = s.chosen <= 1 ? 1 : s.chosen <= 2 ? 2 : s.chosen <= 4 ? 4 : 8;
+  a.team = vec && a.vecs <= 8 ? 8 : vec && a.vecs <= 16 ? 16 : 32;
   const int64_t lane_vecs = vec ? kRingSlots / batch : 4;        // G of the combine kernels
-  a.per = dispatch ? (uint64_t)a.vecs : (uint64_t)((a.vecs + 32 * lane_vecs - 1) / (32 * lane_vecs));
+  a.per = dispatch ? (uint64_t)a.vecs : (uint64_t)((a.vecs + a.team * lane_vecs - 1) / (a.team * lane_vecs));
   a.items = a.per * (uint64_t)s.tokens;
-  const uint64_t per_cta = dispatch ? kRowThreads : kRowThreads / 32, blocks = (a.items + per_cta - 1) / per_cta;
+  const uint64_t per_cta = dispatch ? kRowThreads : kRowThreads / a.team, blocks = (a.items + per_cta - 1) / per_cta;
   if (blocks >= (1ull << 31) || a.vecs >= (1ll << 31) || src.rows >= (1ll << 31)) { set_error("expert rows: tensor too large"); return THCB200_ERR_LIMIT; }
   a.per32 = FastDiv32((uint32_t)a.per);
   a.chosen = (int)s.chosen;
@@ -405,8 +410,9 @@ int run_route(thcb200_ctx *ctx, bool dispatch, const MatView &dst, const MatView
 template <typename T>
 int run_combine_grad(thcb200_ctx *ctx, const MatView *out, void *grad_weight, const MatView &grad, const MatView &rows, const SlotView &s,
                      const void *weight, cudaStream_t st) {
-  constexpr int VB = 16 / sizeof(T);
-  const bool vec = (!out || mat_vec(*out, sizeof(T), 16)) && mat_vec(grad, sizeof(T), 16) && mat_vec(rows, sizeof(T), 16);
+  auto made_of = [&](size_t bytes) { return (!out || mat_vec(*out, sizeof(T), bytes)) && mat_vec(grad, sizeof(T), bytes) && mat_vec(rows, sizeof(T), bytes); };
+  const int bytes = made_of(32) && grad.cols * (int64_t)sizeof(T) >= 32 * 32 ? 32 : made_of(16) ? 16 : (int)sizeof(T);
+  const bool vec = bytes > (int)sizeof(T);
   CombineGradArgs<T> a;
   a.grad_rows = out ? (T *)out->data : nullptr;
   a.grad_weight = (typename Weight<T>::type *)grad_weight;
@@ -415,7 +421,7 @@ int run_combine_grad(thcb200_ctx *ctx, const MatView *out, void *grad_weight, co
   a.slot = s.data;
   a.weight = (const typename Weight<T>::type *)weight;
   a.pairs = (uint64_t)(s.tokens * s.chosen);
-  a.vecs = vec ? grad.cols / VB : grad.cols;
+  a.vecs = grad.cols * (int64_t)sizeof(T) / bytes;
   a.chosen = FastDiv32((uint32_t)s.chosen);
   a.places = rows.rows;
   a.out_stride = out ? out->row_stride : 0;
@@ -424,12 +430,20 @@ int run_combine_grad(thcb200_ctx *ctx, const MatView *out, void *grad_weight, co
   a.rows_stride = rows.row_stride;
   a.rows_col = vec ? 1 : rows.col_stride;
   a.errors = index_errors(ctx);
-  const unsigned blocks = (unsigned)((a.pairs + kRowThreads / 32 - 1) / (kRowThreads / 32));
-#define THCB_GRAD(V) \
-  if (out && grad_weight) launch_pdl(combine_grad_kernel<T, V, true, true>, blocks, kRowThreads, 0, st, a); \
-  else if (out) launch_pdl(combine_grad_kernel<T, V, true, false>, blocks, kRowThreads, 0, st, a); \
-  else launch_pdl(combine_grad_kernel<T, V, false, true>, blocks, kRowThreads, 0, st, a)
-  if (vec) { THCB_GRAD(VB); } else { THCB_GRAD(1); }
+  a.team_bits = 5;
+  while (a.team_bits > 2 && (1 << (a.team_bits - 1)) >= a.vecs) --a.team_bits;
+  const uint64_t per_cta = kRowThreads >> a.team_bits;
+  const unsigned blocks = (unsigned)((a.pairs + per_cta - 1) / per_cta);
+  auto launch = [&](auto kernel) { launch_pdl(kernel, blocks, kRowThreads, 0, st, a); };
+#define THCB_GRAD(V, TEAMS) \
+  do { \
+    if (out && grad_weight) launch(combine_grad_kernel<T, V, true, true, TEAMS>); \
+    else if (out) launch(combine_grad_kernel<T, V, true, false, TEAMS>); \
+    else launch(combine_grad_kernel<T, V, false, true, TEAMS>); \
+  } while (0)
+  if (bytes == 32) THCB_GRAD(32 / sizeof(T), false);
+  else if (bytes == 16) THCB_GRAD(16 / sizeof(T), true);
+  else THCB_GRAD(1, true);
 #undef THCB_GRAD
   count_launch();
   THCB_CUDA_TRY(cudaGetLastError());

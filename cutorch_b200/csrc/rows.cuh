@@ -26,6 +26,19 @@ template <typename T, int V> __device__ __forceinline__ Pack<T, V> load_pack(con
   }
   return x;
 }
+// The same for rows that other warps of the CTA read as well: through the L1.
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> load_kept(const T *p) {
+  Pack<T, V> x;
+  if constexpr (sizeof(T) * V == 32) {
+    Bytes32 b;
+    asm volatile("ld.global.v8.u32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(b.w[0]), "=r"(b.w[1]), "=r"(b.w[2]), "=r"(b.w[3]), "=r"(b.w[4]), "=r"(b.w[5]), "=r"(b.w[6]), "=r"(b.w[7]) : "l"(p));
+    memcpy(&x, &b, 32);
+  } else {
+    x = *reinterpret_cast<const Pack<T, V> *>(p);
+  }
+  return x;
+}
 template <typename T, int V> __device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &x) {
   if constexpr (sizeof(T) * V == 16) {
     Bytes16 b;

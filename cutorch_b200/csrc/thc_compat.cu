@@ -1911,21 +1911,33 @@ void expert_combine_grad(THCState *state, TensorT<R> *grad_rows, TensorT<A> *gra
   if (gwd) gwd->finish();
 }
 
-// A list's tensors, contiguous for the call.
+// A list's tensors, contiguous for the call.  Lists have hundreds of tensors and small ones make steps of a few
+// microseconds, so a contiguous tensor costs a walk over its sizes and a compare here.
 template <typename R> struct HeldList {
   std::vector<Held<R>> v;
+  int device;
+  explicit HeldList(int current) : device(current) {}
   R *add(THCState *state, TensorT<R> *t, ptrdiff_t n, bool written, int arg, int i) {
     if (!t) th_arg_error(arg, "tensor %d is missing", i + 1);
-    check_gpu<R>(state, {t});
-    if (tensor_nelement<R>(t) != n) th_arg_error(arg, "tensor %d has %ld elements, expected %ld", i + 1, (long)tensor_nelement<R>(t), (long)n);
+    ptrdiff_t have = t->nDimension > 0 ? 1 : 0;
+    long run = 1;
+    bool dense = true;
+    for (int d = t->nDimension - 1; d >= 0; --d) {
+      have *= t->size[d];
+      if (t->size[d] == 1) continue;
+      dense = dense && t->stride[d] == run;
+      run *= t->size[d];
+    }
+    if (have != n) th_arg_error(arg, "tensor %d has %ld elements, expected %ld", i + 1, (long)have, (long)n);
     if (n == 0) return nullptr;
-    const bool dense = tensor_is_contiguous<R>(t);
+    check_gpu1<R>(state, t, device);
     if (!dense) {
       v.emplace_back(state);
       if (written) v.back().inout(t, false, arg); else v.back().in(t, false);
       t = v.back().t;
     }
-    return (R *)describe<R>(t).data;
+    if (!t->storage || t->storageOffset < 0 || t->storageOffset + n > t->storage->size) describe<R>(t);   // reports what it reaches
+    return t->storage ? t->storage->data + t->storageOffset : nullptr;
   }
   void finish() { for (Held<R> &h : v) h.finish(); }
 };
@@ -1936,13 +1948,13 @@ template <typename R, typename A>
 void adamw(THCState *state, TensorT<R> **param, TensorT<R> **grad, TensorT<A> **m, TensorT<A> **v, TensorT<A> **master, int n, thcb200_adamw_args args) {
   THArgCheck(n >= 0 && (n == 0 || (param && grad && m && v)), 2, "expecting lists of tensors");
   std::vector<thcb200_adamw_tensor> list((size_t)n);
-  HeldList<R> hp;
-  HeldList<A> ha;
+  const int current = current_device();
+  HeldList<R> hp(current);
+  HeldList<A> ha(current);
   for (int i = 0; i < n; ++i) {
     THArgCheck(param[i] != nullptr, 2, "tensor %d is missing", i + 1);
     const ptrdiff_t k = tensor_nelement<R>(param[i]);
     thcb200_adamw_tensor &t = list[(size_t)i];
-    t = thcb200_adamw_tensor{};
     t.numel = k;
     t.param = hp.add(state, param[i], k, true, 2, i);
     t.grad = hp.add(state, grad[i], k, false, 3, i);
@@ -1960,16 +1972,16 @@ void adamw8bit(THCState *state, TensorT<R> **param, TensorT<R> **grad, TensorT<c
                TensorT<float> **v_unit, TensorT<A> **master, int n, thcb200_adamw_args args) {
   THArgCheck(n >= 0 && (n == 0 || (param && grad && m && v && m_unit && v_unit)), 2, "expecting lists of tensors");
   std::vector<thcb200_adamw_tensor> list((size_t)n);
-  HeldList<R> hp;
-  HeldList<A> ha;
-  HeldList<char> hm;
-  HeldList<unsigned char> hv;
-  HeldList<float> hu;
+  const int current = current_device();
+  HeldList<R> hp(current);
+  HeldList<A> ha(current);
+  HeldList<char> hm(current);
+  HeldList<unsigned char> hv(current);
+  HeldList<float> hu(current);
   for (int i = 0; i < n; ++i) {
     THArgCheck(param[i] != nullptr, 2, "tensor %d is missing", i + 1);
     const ptrdiff_t k = tensor_nelement<R>(param[i]);
     thcb200_adamw_tensor &t = list[(size_t)i];
-    t = thcb200_adamw_tensor{};
     t.numel = k;
     t.param = hp.add(state, param[i], k, true, 2, i);
     t.grad = hp.add(state, grad[i], k, false, 3, i);
@@ -1991,9 +2003,10 @@ void adamw_values(THCState *state, TensorT<float> **m_value, TensorT<float> **v_
                   TensorT<float> **m_unit, TensorT<float> **v_unit, int n) {
   THArgCheck(n >= 0 && (n == 0 || (m_value && v_value && m && v && m_unit && v_unit)), 2, "expecting lists of tensors");
   std::vector<thcb200_adamw_tensor> list((size_t)n);
-  HeldList<float> hf;
-  HeldList<char> hm;
-  HeldList<unsigned char> hv;
+  const int current = current_device();
+  HeldList<float> hf(current);
+  HeldList<char> hm(current);
+  HeldList<unsigned char> hv(current);
   for (int i = 0; i < n; ++i) {
     THArgCheck(m[i] != nullptr && v[i] != nullptr && m_value[i] != nullptr && v_value[i] != nullptr, 2, "tensor %d is missing", i + 1);
     const ptrdiff_t k = tensor_nelement<char>(m[i]);

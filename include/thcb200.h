@@ -457,7 +457,7 @@ THCB200_API int thcb200_expert_combine_grad(thcb200_ctx *ctx, const thcb200_tens
  * A code c of m stands for c|c| * unit, one of v for c^4 * unit; values between two codes are rounded up or down by a hash of
  * the element's place and the step, so that averages keep their expectation.  A NaN or infinite gradient makes its
  * block's moments NaN.  master (F16; all tensors or none): float copies the step is computed from.
- * No element may be written twice: a list whose written arrays share memory is refused.  The arguments, step among them, are
+ * A list in which an array that is written shares memory with another is refused.  The arguments, step among them, are
  * fixed when a call is captured into a graph. */
 #define THCB200_ADAMW_BLOCK 256
 typedef struct thcb200_adamw_tensor {

@@ -124,12 +124,26 @@ def test_adamw(lib):
     refused(lib, f(dtype=F16, n=2, tensors=[Tensor(at, at + 1024, at + 256, at + 512, None, None, at + 700, 4),
                                             Tensor(at + 2000, at + 1024, at + 2256, at + 2512, None, None, None, 4)]), ARG, "has no master")
     # the second moment ends inside the first; a tensor listed twice; in either order
-    refused(lib, f(tensors=[Tensor(at, at + 1024, at + 256, at + 268, None, None, None, 4)]), ARG, "share memory")
+    refused(lib, f(tensors=[Tensor(at, at + 1024, at + 256, at + 268, None, None, None, 4)]), ARG, "shares memory")
     one = Tensor(at, at + 1024, at + 256, at + 512, None, None, None, 4)
     for pair in ([one, Tensor(at, at + 1024, at + 2256, at + 2512, None, None, None, 4)],
                  [one, Tensor(at + 3000, at + 1024, at + 252, at + 2512, None, None, None, 4)]):
-        refused(lib, f(tensors=pair, n=2), ARG, "share memory")
-        refused(lib, f(tensors=pair[::-1], n=2), ARG, "share memory")
+        refused(lib, f(tensors=pair, n=2), ARG, "shares memory")
+        refused(lib, f(tensors=pair[::-1], n=2), ARG, "shares memory")
+
+
+def test_adamw_gradients_apart_from_what_is_written(lib):
+    """A gradient inside a written array is refused wherever the lists lie; gradients may share memory with one another."""
+    at = HERE.ctypes.data
+
+    def f(*tensors):
+        args = Args(1e-3, 0.9, 0.99, 1e-8, 0, 1, 1)
+        return lib.thcb200_adamw(CONTEXT, F32, 32, (Tensor * len(tensors))(*tensors), len(tensors), C.byref(args), None)
+
+    for grad in (0, 8, 256, 264, 512, 524):
+        refused(lib, f(Tensor(at, at + grad, at + 256, at + 512, None, None, None, 4)), ARG, "shares memory")
+        refused(lib, f(Tensor(at, at + 1024, at + 256, at + 512, None, None, None, 4),
+                       Tensor(at + 2048, at + grad, at + 2304, at + 2560, None, None, None, 4)), ARG, "shares memory")
 
 
 def test_large_kernel_arguments_fit():
