@@ -129,6 +129,16 @@ def _half_to_float(h: _Half) -> float:
     return float(np.array(h.x, dtype=np.uint16).view(np.float16))
 
 
+def _real_of(kind: str):
+    """The conversion of a number to a tensor kind's C `real`."""
+    creal = KINDS[kind][2]
+    if kind == "Half":
+        return lambda v: _half_from_float(float(v))
+    if kind in FLOATING:
+        return lambda v: creal(float(v))
+    return lambda v: creal(int(v))
+
+
 class State:
     """THCState: owns the per-device contexts; `stream` selects the current stream."""
 
@@ -154,6 +164,7 @@ class State:
         lib.THCudaInit(self.ptr)
         self.check()
         self._fn_cache = {}
+        self._calls = {}
 
     def check(self):
         if self._failed():
@@ -276,8 +287,9 @@ class Tensor:
         free(state.ptr, storage)
         return t
 
-    def _long_storage(self, values):
-        lib = self.state.lib
+    @staticmethod
+    def _long_storage(state, values):
+        lib = state.lib
         lib.THLongStorage_newWithSize.restype = C.c_void_p
         lib.THLongStorage_newWithSize.argtypes = [C.c_ssize_t]
         lib.THLongStorage_set.argtypes = [C.c_void_p, C.c_ssize_t, C.c_long]
@@ -290,7 +302,7 @@ class Tensor:
     def _set_storage(self, storage, offset, sizes, strides):
         f = self.state.fn(self.kind, "setStorage")
         f.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_ssize_t, C.c_void_p, C.c_void_p]
-        sz, st = self._long_storage(sizes), self._long_storage(strides)
+        sz, st = self._long_storage(self.state, sizes), self._long_storage(self.state, strides)
         f(self.state.ptr, self.ptr, storage, offset, sz, st)
         self.state.lib.THLongStorage_free(sz)
         self.state.lib.THLongStorage_free(st)
@@ -299,7 +311,7 @@ class Tensor:
     def resize(self, *sizes):
         f = self.state.fn(self.kind, "resize")
         f.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
-        sz = self._long_storage(sizes)
+        sz = self._long_storage(self.state, sizes)
         f(self.state.ptr, self.ptr, sz, None)
         self.state.lib.THLongStorage_free(sz)
         self.state.check()
@@ -326,7 +338,7 @@ class Tensor:
         f = self.state.fn(self.kind, "newExpand")
         f.restype = C.c_void_p
         f.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
-        sz = self._long_storage(sizes)
+        sz = self._long_storage(self.state, sizes)
         p = f(self.state.ptr, self.ptr, sz)
         self.state.lib.THLongStorage_free(sz)
         self.state.check()
@@ -417,71 +429,60 @@ class Tensor:
         return np.array(view, copy=True)
 
     # ---- THC calls ---------------------------------------------------------------------
-    def _real(self, v):
-        creal = KINDS[self.kind][2]
-        if self.kind == "Half":
-            return _half_from_float(float(v))
-        if self.kind in FLOATING:
-            return creal(float(v))
-        return creal(int(v))
-
-    def _prototype(self, f, name: str):
-        """Sets the C prototype of a call's function object once (it belongs to one symbol); per argument, its code and the
-        kind a tensor has to be of."""
+    def _prepare(self, name: str):
+        """A call's function object with its C prototype, and per argument the kind a tensor has to be of, whether it may be
+        missing, and the conversion of anything that is not a GPU tensor."""
+        f = self.state.fn(self.kind, name)
         ret, spec = SIGNATURES[name]
         creal, cacc = KINDS[self.kind][2], KINDS[self.kind][3]
         codes = {"r": creal, "l": C.c_long, "f": cacc}
         f.argtypes = [C.c_void_p] + [codes.get(c, C.c_int if c == "i" else C.c_void_p) for c in spec]
         f.restype = {"v": None, "a": cacc, "R": creal, "n": C.c_int, "p": C.c_ssize_t}[ret]
-        want = {"L": "Long", "B": "Byte", "A": ACC_KIND.get(self.kind), "T": self.kind, "C": "Long", "M": "Byte"}
-        f.prototype = [(c, want.get(c)) for c in spec]
-        return f.prototype
+        kinds = {"T": self.kind, "L": "Long", "B": "Byte", "A": ACC_KIND.get(self.kind)}
+
+        def cpu(want):
+            def convert(a):
+                if not isinstance(a, CpuTensor) or a.kind != want:
+                    raise TypeError(f"{name}: expected a CPU {want} tensor")
+                return a.ptr
+            return convert
+
+        state = self.state
+        converts = {"r": _real_of(self.kind), "l": int, "i": int, "f": float, "C": cpu("Long"), "M": cpu("Byte"),
+                    "S": lambda a: Tensor._long_storage(state, tuple(a))}
+        arguments = [(kinds.get(c), c == "A", converts.get(c)) for c in spec]
+        storages = [k + 1 for k, c in enumerate(spec) if c == "S"]
+        call = f, arguments, storages, ret == "R" and self.kind == "Half"
+        state._calls[self.kind, name] = call
+        return call
 
     def call(self, name: str, *args):
         """Calls TH<Kind>Tensor_<name>(state, ...) with `args` exactly in C order."""
         state = self.state
-        f = state.fn(self.kind, name)
         try:
-            prototype = f.prototype
-        except AttributeError:
-            prototype = self._prototype(f, name)
-        if len(args) != len(prototype):
+            f, arguments, storages, half = state._calls[self.kind, name]
+        except KeyError:
+            f, arguments, storages, half = self._prepare(name)
+        if len(args) != len(arguments):
             spec = SIGNATURES[name][1]
             raise TypeError(f"{name} takes {len(spec)} arguments ({spec}), got {len(args)}")
         cargs = [state.ptr]
-        storages = None
-        for (code, want), a in zip(prototype, args):
-            if code in "TLBA":
-                if isinstance(a, Tensor):
-                    if a.kind != want:
-                        raise TypeError(f"{name}: expected a {want} tensor, got {a.kind}")
-                    cargs.append(a.ptr)
-                elif a is None and code == "A":
-                    cargs.append(None)
-                else:
-                    raise TypeError(f"{name}: expected a tensor")
-            elif code == "r":
-                cargs.append(self._real(a))
-            elif code == "f":
-                cargs.append(float(a))
-            elif code == "S":
-                sz = self._long_storage(tuple(a))
-                storages = (storages or []) + [sz]
-                cargs.append(sz)
-            elif code in "CM":
-                if not isinstance(a, CpuTensor) or a.kind != want:
-                    raise TypeError(f"{name}: expected a CPU {want} tensor")
+        for (kind, optional, convert), a in zip(arguments, args):
+            if convert is not None:
+                cargs.append(convert(a))
+            elif isinstance(a, Tensor):
+                if a.kind != kind:
+                    raise TypeError(f"{name}: expected a {kind} tensor, got {a.kind}")
                 cargs.append(a.ptr)
+            elif optional and a is None:
+                cargs.append(None)
             else:
-                cargs.append(int(a))
+                raise TypeError(f"{name}: expected a tensor")
         r = f(*cargs)
-        if storages:
-            for sz in storages:
-                state.lib.THLongStorage_free(sz)
+        for k in storages:
+            state.lib.THLongStorage_free(cargs[k])
         state.check()
-        if self.kind == "Half" and SIGNATURES[name][0] == "R":
-            return _half_to_float(r)
-        return r
+        return _half_to_float(r) if half else r
 
     def copy_from(self, src: "Tensor"):
         """self:copy(src) with type conversion (THCTensor_(copyCuda<Type>))."""
