@@ -18,10 +18,10 @@
 // Moments and codes take one IEEE operation after the other (the library is compiled without contraction), so they do not
 // depend on the compiler's choice of fused operations; the 8-bit form's parameter takes the approximate root and reciprocal.
 //
-// Both are bound by HBM in principle.  200 M float elements in 290 tensors, B200: 32-bit moments 804 us, 5.6 GB, 6970 GB/s (the
-// box's copy: 6558).  8-bit moments, 3.2 GB: 860 us, 3.7 TB/s, bound by instruction issue (105 per element, 75 % of the issue
-// slots; 1310 us with scalar instructions, IEEE roots and byte conversions, 925 us packed, 890 us with the spills of 64 registers
-// taken for a fourth CTA, 860 us with the next tile prefetched into the L2).
+// Both are bound by HBM in principle.  200 M float elements in 290 tensors, B200: 32-bit moments 800 us, 5.6 GB, 7000 GB/s (the
+// box's copy: 6558).  8-bit moments, 3.2 GB: 840 us, 3.8 TB/s, bound by instruction issue (90 per element): 1310 us with scalar
+// instructions, IEEE roots and byte conversions, 925 us packed, 890 us with four CTAs per SM, 860 us with the next tile
+// prefetched into the L2, 840 us with the rare exact codes apart.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -343,6 +343,13 @@ __device__ __forceinline__ void prefetch_ahead(const void *base, size_t esz, con
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p), "r"((uint32_t)(kStepTile * esz)) : "memory");
 }
 
+__device__ __forceinline__ float pick(const F2 (&x)[kStepItems / 2], int j) {      // element j, without an indexed register
+  float r = 0;
+#pragma unroll
+  for (int i = 0; i < kStepItems; ++i) r = i == j ? (i & 1 ? hi_of(x[i / 2]) : lo_of(x[i / 2])) : r;
+  return r;
+}
+
 template <typename T, bool MASTER, int N>
 __global__ void __launch_bounds__(kStepThreads, 4)
 adamw8_kernel(const __grid_constant__ StepTable<N> table, const __grid_constant__ StepPairs c) {
@@ -411,21 +418,6 @@ adamw8_kernel(const __grid_constant__ StepTable<N> table, const __grid_constant_
     kv[i] = codes_near<true>(xv, pair(root_near(root_near(lo_of(xv))), root_near(root_near(hi_of(xv)))),
                              add2(pair(half_magic(d0, 0), half_magic(d1, 0)), both(-128.0f)), rare, c);
   }
-  if (rare > 0) {
-#pragma unroll
-    for (int i = 0; i < kStepItems / 2; ++i) {
-      float a[2], b[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t d = dither_of(h + (2 * i + k) * hstep);
-        const float xm = fabsf(k ? hi_of(m[i]) : lo_of(m[i])) * mi, xv = (k ? hi_of(v[i]) : lo_of(v[i])) * vi;
-        a[k] = code_exact<127, false>(xm, root_near(xm), (float)(d >> 16));
-        b[k] = code_exact<255, true>(xv, root_near(root_near(xv)), (float)(d & 0xffffu));
-      }
-      km[i] = pair(a[0], a[1]);
-      kv[i] = pair(b[0], b[1]);
-    }
-  }
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     uint32_t bm[4], bv[4];
@@ -434,8 +426,8 @@ adamw8_kernel(const __grid_constant__ StepTable<N> table, const __grid_constant_
       const int j = 2 * w + i;
       const F2 sm = add2(pair(copysignf(lo_of(km[j]), lo_of(m[j])), copysignf(hi_of(km[j]), hi_of(m[j]))), both(kByteMagic));
       // at least 1 where v is above zero: v 2^200, cut at 1, is 0 or 1
-      const F2 big = mul2(v[j], both(0x1p100f), c.minus_zero);
-      const F2 sv = add2(pair(fmaxf(lo_of(kv[j]), __saturatef(lo_of(big) * 0x1p100f)), fmaxf(hi_of(kv[j]), __saturatef(hi_of(big) * 0x1p100f))), both(kByteMagic));
+      const F2 sv = add2(pair(fmaxf(lo_of(kv[j]), __saturatef(lo_of(v[j]) * 0x1p100f * 0x1p100f)),
+                              fmaxf(hi_of(kv[j]), __saturatef(hi_of(v[j]) * 0x1p100f * 0x1p100f))), both(kByteMagic));
       bm[2 * i] = (uint32_t)sm;
       bm[2 * i + 1] = (uint32_t)(sm >> 32);
       bv[2 * i] = (uint32_t)sv;
@@ -446,6 +438,18 @@ adamw8_kernel(const __grid_constant__ StepTable<N> table, const __grid_constant_
   }
   store_codes((int8_t *)e.m, cm, q);
   store_codes((uint8_t *)e.v, cv, q);
+  if (rare > 0) {      // apart from the codes above, so that nothing of it costs the others a register
+#pragma unroll 1
+    for (int j = 0; j < kStepItems; ++j) {
+      const float mj = pick(m, j), vj = pick(v, j);
+      const uint32_t d = dither_of(h + j * hstep);
+      const float xm = fabsf(mj) * mi, xv = vj * vi;
+      const float a = code_exact<127, false>(xm, root_near(xm), (float)(d >> 16)), b = code_exact<255, true>(xv, root_near(root_near(xv)), (float)(d & 0xffffu));
+      if (q.at(j) >= q.n) break;
+      ((int8_t *)e.m)[q.at(j)] = (int8_t)(int)copysignf(a, mj);
+      ((uint8_t *)e.v)[q.at(j)] = (uint8_t)(int)(vj > 0 ? fmaxf(b, 1.0f) : b);
+    }
+  }
   if ((threadIdx.x & 31) == 0) {
     e.m_unit[block] = nmu;
     e.v_unit[block] = nvu;
