@@ -75,9 +75,11 @@ embedding_kernel(T *out, const T *weight, const int64_t *index, FastDiv32 vecs32
 
 // ---- gradient ----------------------------------------------------------------------------------
 constexpr int kGradThreads = 256;
-template <int V, bool ADD> constexpr int kGradBatch = V > 1 && ADD ? 4 : 8;   // rows in flight per thread (and as many of the table's)
+constexpr int kGradBatch = 4;        // tokens that are added up between two looks at the copies
+constexpr int kGradStages = 3;       // batches of rows of 16-byte vectors in shared memory: two on their way, one being added
+constexpr size_t kGradRing = (size_t)kGradStages * kGradBatch * kGradThreads * 16;
 constexpr int kGradMaxChunk = 64;    // sorted tokens per CTA
-constexpr int kGradKeys = 2048;      // sorted tokens per CTA where rows are narrow and it takes several chunks
+constexpr int kGradKeys = 1024;      // sorted tokens per CTA where rows are narrow and it takes several chunks
 
 template <typename T> struct GradArgs {
   T *table;
@@ -105,10 +107,29 @@ __device__ __forceinline__ void write_row(const GradArgs<T> &a, uint32_t key, in
   store_pack<T, V>(a.table + (int64_t)key * a.table_stride + col, out);
 }
 
+// Partial sums lie in rows of `width` accumulators, on 16-byte boundaries where the rows' elements are taken in vectors.
 template <typename T, int V>
 __device__ __forceinline__ void add_partial(typename TypeTraits<T>::Acc (&acc)[V], const typename TypeTraits<T>::Acc *p) {
+  using Acc = typename TypeTraits<T>::Acc;
+  constexpr int W = V > 1 ? 16 / sizeof(Acc) : 1;
 #pragma unroll
-  for (int e = 0; e < V; ++e) acc[e] += p[e];
+  for (int e = 0; e < V; e += W) {
+    const Pack<Acc, W> x = *reinterpret_cast<const Pack<Acc, W> *>(p + e);
+#pragma unroll
+    for (int k = 0; k < W; ++k) acc[e + k] += x.e[k];
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_sums(typename TypeTraits<T>::Acc *p, const typename TypeTraits<T>::Acc (&acc)[V]) {
+  using Acc = typename TypeTraits<T>::Acc;
+  constexpr int W = V > 1 ? 16 / sizeof(Acc) : 1;
+#pragma unroll
+  for (int e = 0; e < V; e += W) {
+    Pack<Acc, W> x;
+#pragma unroll
+    for (int k = 0; k < W; ++k) x.e[k] = acc[e + k];
+    *reinterpret_cast<Pack<Acc, W> *>(p + e) = x;
+  }
 }
 
 // CTAs 0 .. chunks-1 sum the rows named in their chunk of the sorted tokens; the ones behind clear the rows no token
@@ -121,11 +142,12 @@ template <typename T, int V, bool ADD, bool FEW>
 __global__ void __launch_bounds__(kGradThreads, 4)
 embedding_grad_kernel(GradArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
-  constexpr int B = kGradBatch<V, ADD>;
+  constexpr int B = V == 1 ? 2 * kGradBatch : kGradBatch;
   pdl_prologue();
   const uint32_t group = 1u << a.group_bits, groups = kGradThreads >> a.group_bits, mine = threadIdx.x >> a.group_bits, member = threadIdx.x & (group - 1);
   const int64_t col = ((int64_t)blockIdx.y * group + member) * V;
-  extern __shared__ uint32_t grad_smem[];
+  extern __shared__ Bytes16 grad_ring[];
+  uint32_t *grad_smem = reinterpret_cast<uint32_t *>(V > 1 ? grad_ring + kGradStages * kGradBatch * kGradThreads : grad_ring);
   __shared__ uint32_t few_raw[FEW ? kFewTokens : 1], few_key[FEW ? kFewTokens + 2 : 1], few_pos[FEW ? kFewTokens : 1];
   if constexpr (FEW) {
     const uint32_t i = threadIdx.x, n = (uint32_t)a.tokens;
@@ -162,8 +184,9 @@ embedding_grad_kernel(GradArgs<T> a) {
     Pack<T, V> zero;
 #pragma unroll
     for (int e = 0; e < V; ++e) zero.e[e] = round_from<T>((Acc)0);
-    for (uint32_t r = mine; r < a.zero_rows; r += groups)
+    for (uint32_t r = mine; r < a.zero_rows; r += groups) {
       if (!grad_smem[r]) store_pack<T, V>(a.table + (row0 + r) * a.table_stride + col, zero);
+    }
     return;
   }
   const uint32_t index = blockIdx.x * groups + mine;            // the group's chunk
@@ -197,8 +220,76 @@ embedding_grad_kernel(GradArgs<T> a) {
     while (from < own && skey[from + 1] == first) ++from;
   if (goes_on && !tail_long && !(head && first == last))
     while (to < seen && skey[to + 1] == last) ++to;
+  if (last == none)                                    // items without a row come last
+    for (to = from; to < own && skey[to + 1] != none;) ++to;
+  Acc acc[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0;
+  const auto row_ends = [&](uint32_t i) { return i + 1 >= to || skey[i + 2] != skey[i + 1]; };
+  // Adds token i; the sum of a row that ends there goes to the table, over `old` or not, or to the partial sums.
+  const auto add = [&](const Pack<T, V> &x, uint32_t i, const Pack<T, V> &old) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] += (Acc)to_math(x.e[e]);
+    if (!row_ends(i)) return;
+    const uint32_t key = skey[i + 1];
+    const bool in_head = head_long && key == first, in_tail = tail_long && key == last;
+    if (in_head || in_tail) store_sums<T, V>(a.partial + ((int64_t)index * 2 + (in_head ? 0 : 1)) * a.width + col, acc);
+    else write_row<T, V, ADD>(a, key, col, acc, old);
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0;
+  };
+  Pack<T, V> x[B], old[ADD ? B : 1];
+  // what the sum of a row that ends at token i is added to comes with the token's batch
+  const auto read_old = [&](Pack<T, V> (&o)[ADD ? B : 1], uint32_t i, int u) {
+    if (ADD && row_ends(i)) o[ADD ? u : 0] = load_pack<T, V>(a.table + (int64_t)skey[i + 1] * a.table_stride + col);
+  };
+  if constexpr (V > 1) {
+    // every thread copies what it will add itself, so that no barrier is needed: two batches on their way while one is added
+    const auto copy = [&](uint32_t i0, int stage) {
+#pragma unroll
+      for (int u = 0; u < B; ++u)
+        if (i0 + u < to)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                       :: "r"((uint32_t)__cvta_generic_to_shared(&grad_ring[(stage * B + u) * kGradThreads + threadIdx.x])),
+                          "l"(a.grad + (int64_t)spos[i0 + u] * a.grad_stride + col) : "memory");
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    copy(from, 0);
+    copy(from + B, 1);
+    int stage = 0;
+    for (uint32_t i = from; i < to; i += B) {
+      copy(i + 2 * B, stage == 0 ? 2 : stage - 1);
+#pragma unroll
+      for (int u = 0; u < B; ++u)
+        if (i + u < to) read_old(old, i + u, u);
+      asm volatile("cp.async.wait_group 2;" ::: "memory");
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        if (i + u >= to) break;
+        const Bytes16 b = grad_ring[(stage * B + u) * kGradThreads + threadIdx.x];
+        memcpy(&x[0], &b, 16);
+        add(x[0], i + u, old[ADD ? u : 0]);
+      }
+      stage = stage == 2 ? 0 : stage + 1;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else {
+    for (uint32_t i = from; i < to; i += B) {
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        if (i + u >= to) continue;
+        x[u] = load_pack<T, V>(a.grad + (int64_t)spos[i + u] * a.grad_stride + col * a.grad_col);
+        read_old(old, i + u, u);
+      }
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        if (i + u >= to) break;
+        add(x[u], i + u, old[ADD ? u : 0]);
+      }
+    }
+  }
+  // A row across more than two chunks is joined later: its chunks whose first token is the row's, the next two at least.
   if (!FEW && blockIdx.y == 0 && member == 0 && tail_long && last != none && !(head && first == last)) {
-    // chunks whose first token is the row's: the next two at least
     int64_t lo = (int64_t)index + 3, hi = a.chunks, reach = 2;
     while (lo + reach < hi && a.key[(lo + reach) * a.chunk] == last) { lo += reach + 1; reach *= 2; }
     hi = min(hi, lo + reach);
@@ -207,38 +298,6 @@ embedding_grad_kernel(GradArgs<T> a) {
       if (a.key[mid * a.chunk] == last) lo = mid + 1; else hi = mid;
     }
     a.starts[atomicAdd(a.start_count, 1u)] = make_uint4(index, (uint32_t)(lo - 1 - (int64_t)index), last, 0);
-  }
-  Acc acc[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) acc[e] = 0;
-  for (uint32_t i = from; i < to; i += B) {
-    Pack<T, V> x[B], old[ADD ? B : 1];
-#pragma unroll
-    for (int u = 0; u < B; ++u) {
-      if (i + u >= to || skey[i + u + 1] == none) continue;
-      x[u] = load_pack<T, V>(a.grad + (int64_t)spos[i + u] * a.grad_stride + col * a.grad_col);
-      // what the sum of a row that ends here is added to comes with the same batch
-      if (ADD && (i + u + 1 >= to || skey[i + u + 2] != skey[i + u + 1])) old[u] = load_pack<T, V>(a.table + (int64_t)skey[i + u + 1] * a.table_stride + col);
-    }
-#pragma unroll
-    for (int u = 0; u < B; ++u) {
-      if (i + u >= to) break;
-      const uint32_t key = skey[i + u + 1];
-      if (key == none) return;                                  // items without a row come last
-#pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] += (Acc)to_math(x[u].e[e]);
-      if (i + u + 1 < to && skey[i + u + 2] == key) continue;
-      const bool in_head = head_long && key == first, in_tail = tail_long && key == last;
-      if (in_head || in_tail) {
-        Acc *p = a.partial + ((int64_t)index * 2 + (in_head ? 0 : 1)) * a.width + col;
-#pragma unroll
-        for (int e = 0; e < V; ++e) p[e] = acc[e];
-      } else {
-        write_row<T, V, ADD>(a, key, col, acc, old[ADD ? u : 0]);
-      }
-#pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] = 0;
-    }
   }
 }
 
@@ -361,24 +420,27 @@ int run_embedding_grad(thcb200_ctx *ctx, const MatView &table, const MatView &gr
   a.zero_rows = zero_rows;
   a.scale = (Acc)scale;
   const dim3 grid((unsigned)(sum_ctas + zero), (unsigned)slabs);
-  const size_t smem = std::max((size_t)groups * (4 * chunk + 2), (size_t)zero_rows) * sizeof(uint32_t);   // at most 34 KiB
+  const size_t smem = (vec ? kGradRing : 0) + std::max((size_t)groups * (4 * chunk + 2), (size_t)zero_rows) * sizeof(uint32_t);   // at most 66 KiB
   const int64_t piece = vec ? 32 * VB : 32, pieces = (table.cols + piece - 1) / piece;
   const unsigned join = (unsigned)(chunks * pieces < 8 * kNumSM_B200 ? chunks * pieces : 8 * kNumSM_B200);
   const bool joined = !few && chunks > 2;      // a row across more than two chunks needs three
+  auto sum = [&](auto kernel) -> int {
+    if (smem + 2048 > 48 * 1024) THCB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    launch_pdl(kernel, grid, kGradThreads, smem, st, a);
+    return 0;
+  };
+  int rc = 0;
 #define THCB_GRAD(V, ADD) \
   do { \
-    if (few) { \
-      launch_pdl(embedding_grad_kernel<T, V, ADD, true>, grid, kGradThreads, smem, st, a); \
-    } else { \
-      launch_pdl(embedding_grad_kernel<T, V, ADD, false>, grid, kGradThreads, smem, st, a); \
-      if (joined) launch_pdl(embedding_grad_join_kernel<T, V, ADD>, join, kGradThreads, 0, st, a); \
-    } \
+    rc = few ? sum(embedding_grad_kernel<T, V, ADD, true>) : sum(embedding_grad_kernel<T, V, ADD, false>); \
+    if (!rc && joined) launch_pdl(embedding_grad_join_kernel<T, V, ADD>, join, kGradThreads, 0, st, a); \
   } while (0)
   if (vec && accumulate) THCB_GRAD(VB, true);
   else if (vec) THCB_GRAD(VB, false);
   else if (accumulate) THCB_GRAD(1, true);
   else THCB_GRAD(1, false);
 #undef THCB_GRAD
+  if (rc) return rc;
   count_launch(joined ? 2 : 1);
   THCB_CUDA_TRY(cudaGetLastError());
   return 0;
