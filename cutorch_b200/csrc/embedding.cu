@@ -75,9 +75,12 @@ embedding_kernel(T *out, const T *weight, const int64_t *index, FastDiv32 vecs32
 
 // ---- gradient ----------------------------------------------------------------------------------
 constexpr int kGradThreads = 256;
-constexpr int kGradBatch = 4;        // tokens that are added up between two looks at the copies
-constexpr int kGradStages = 3;       // batches of rows of 16-byte vectors in shared memory: two on their way, one being added
-constexpr size_t kGradRing = (size_t)kGradStages * kGradBatch * kGradThreads * 16;
+// Rows on their way while others are added: vectors by asynchronous copies into shared
+// memory, kGradStages batches of them; single elements, whose copies cost more instructions than they save, by loads of a batch.
+constexpr int kGradStages = 3;
+template <typename T, int V> constexpr int kGradBatch = V > 1 ? 4 : 8;
+template <typename T, int V> constexpr bool kGradCopies = V > 1;
+template <typename T, int V> constexpr size_t kGradRing = kGradCopies<T, V> ? kGradStages * kGradBatch<T, V> * kGradThreads * sizeof(T) * V : 0;
 constexpr int kGradMaxChunk = 64;    // sorted tokens per CTA
 constexpr int kGradKeys = 1024;      // sorted tokens per CTA where rows are narrow and it takes several chunks
 
@@ -142,12 +145,13 @@ template <typename T, int V, bool ADD, bool FEW>
 __global__ void __launch_bounds__(kGradThreads, 4)
 embedding_grad_kernel(GradArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
-  constexpr int B = V == 1 ? 2 * kGradBatch : kGradBatch;
+  constexpr int B = kGradBatch<T, V>;
   pdl_prologue();
   const uint32_t group = 1u << a.group_bits, groups = kGradThreads >> a.group_bits, mine = threadIdx.x >> a.group_bits, member = threadIdx.x & (group - 1);
   const int64_t col = ((int64_t)blockIdx.y * group + member) * V;
-  extern __shared__ Bytes16 grad_ring[];
-  uint32_t *grad_smem = reinterpret_cast<uint32_t *>(V > 1 ? grad_ring + kGradStages * kGradBatch * kGradThreads : grad_ring);
+  extern __shared__ Bytes16 grad_dynamic[];
+  Pack<T, V> *grad_ring = reinterpret_cast<Pack<T, V> *>(grad_dynamic);
+  uint32_t *grad_smem = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(grad_dynamic) + kGradRing<T, V>);
   __shared__ uint32_t few_raw[FEW ? kFewTokens : 1], few_key[FEW ? kFewTokens + 2 : 1], few_pos[FEW ? kFewTokens : 1];
   if constexpr (FEW) {
     const uint32_t i = threadIdx.x, n = (uint32_t)a.tokens;
@@ -238,20 +242,18 @@ embedding_grad_kernel(GradArgs<T> a) {
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] = 0;
   };
-  Pack<T, V> x[B], old[ADD ? B : 1];
+  Pack<T, V> old[ADD ? B : 1];
   // what the sum of a row that ends at token i is added to comes with the token's batch
   const auto read_old = [&](Pack<T, V> (&o)[ADD ? B : 1], uint32_t i, int u) {
     if (ADD && row_ends(i)) o[ADD ? u : 0] = load_pack<T, V>(a.table + (int64_t)skey[i + 1] * a.table_stride + col);
   };
-  if constexpr (V > 1) {
+  if constexpr (kGradCopies<T, V>) {
     // every thread copies what it will add itself, so that no barrier is needed: two batches on their way while one is added
     const auto copy = [&](uint32_t i0, int stage) {
 #pragma unroll
       for (int u = 0; u < B; ++u)
         if (i0 + u < to)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                       :: "r"((uint32_t)__cvta_generic_to_shared(&grad_ring[(stage * B + u) * kGradThreads + threadIdx.x])),
-                          "l"(a.grad + (int64_t)spos[i0 + u] * a.grad_stride + col) : "memory");
+          copy_async<T, V>(&grad_ring[(stage * B + u) * kGradThreads + threadIdx.x], a.grad + (int64_t)spos[i0 + u] * a.grad_stride + col * a.grad_col);
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
     copy(from, 0);
@@ -266,15 +268,14 @@ embedding_grad_kernel(GradArgs<T> a) {
 #pragma unroll
       for (int u = 0; u < B; ++u) {
         if (i + u >= to) break;
-        const Bytes16 b = grad_ring[(stage * B + u) * kGradThreads + threadIdx.x];
-        memcpy(&x[0], &b, 16);
-        add(x[0], i + u, old[ADD ? u : 0]);
+        add(grad_ring[(stage * B + u) * kGradThreads + threadIdx.x], i + u, old[ADD ? u : 0]);
       }
       stage = stage == 2 ? 0 : stage + 1;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else {
     for (uint32_t i = from; i < to; i += B) {
+      Pack<T, V> x[B];
 #pragma unroll
       for (int u = 0; u < B; ++u) {
         if (i + u >= to) continue;
@@ -420,7 +421,7 @@ int run_embedding_grad(thcb200_ctx *ctx, const MatView &table, const MatView &gr
   a.zero_rows = zero_rows;
   a.scale = (Acc)scale;
   const dim3 grid((unsigned)(sum_ctas + zero), (unsigned)slabs);
-  const size_t smem = (vec ? kGradRing : 0) + std::max((size_t)groups * (4 * chunk + 2), (size_t)zero_rows) * sizeof(uint32_t);   // at most 66 KiB
+  const size_t smem = (vec ? kGradRing<T, VB> : kGradRing<T, 1>) + std::max((size_t)groups * (4 * chunk + 2), (size_t)zero_rows) * sizeof(uint32_t);   // at most 66 KiB
   const int64_t piece = vec ? 32 * VB : 32, pieces = (table.cols + piece - 1) / piece;
   const unsigned join = (unsigned)(chunks * pieces < 8 * kNumSM_B200 ? chunks * pieces : 8 * kNumSM_B200);
   const bool joined = !few && chunks > 2;      // a row across more than two chunks needs three

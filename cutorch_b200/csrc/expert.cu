@@ -149,8 +149,7 @@ combine_ring_kernel(RouteArgs<T> a) {
 #pragma unroll
       for (int g = 0; g < G; ++g)
         if (vec0 + team * g < a.vecs)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                       :: "r"((uint32_t)__cvta_generic_to_shared(&ring[(stage * kRingSlots + u * G + g) * kRowThreads + threadIdx.x])), "l"(row + team * g * V) : "memory");
+          copy_async<T, V>(&ring[(stage * kRingSlots + u * G + g) * kRowThreads + threadIdx.x], row + team * g * V);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -205,19 +204,21 @@ combine_ring_kernel(RouteArgs<T> a) {
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// Other rows: single elements, G per lane and row, 32 apart.
-template <typename T>
+// Other rows: single elements, G per lane and row, 32 apart, of BATCH rows at a time.
+template <typename T, int BATCH>
 __global__ void __launch_bounds__(kRowThreads)
 combine_kernel(RouteArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
-  constexpr int G = 4, BATCH = 8;
+  constexpr int G = 4;
   pdl_prologue();
   const uint32_t lane = threadIdx.x & 31;
   const uint64_t unit = (uint64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
   if (unit >= a.items) return;
   int64_t token, stretch;
   split_item(a, unit, &token, &stretch);
-  const int64_t col0 = stretch * (32 * G) + lane;
+  const int32_t col0 = (int32_t)stretch * (32 * G) + (int32_t)lane, width = (int32_t)a.vecs;
+  const T *src = a.src + col0 * a.src_col;
+  const int64_t step = 32 * a.src_col;
   Acc acc[G];
 #pragma unroll
   for (int g = 0; g < G; ++g) acc[g] = 0;
@@ -233,10 +234,10 @@ combine_kernel(RouteArgs<T> a) {
     for (int u = 0; u < BATCH; ++u) {
       p[u] = __shfl_sync(~0u, place, u);
       if (p[u] < 0) continue;
-      const T *row = a.src + p[u] * a.src_stride;
+      const T *row = src + p[u] * a.src_stride;
 #pragma unroll
       for (int g = 0; g < G; ++g)
-        if (col0 + 32 * g < a.vecs) x[u][g] = row[(col0 + 32 * g) * a.src_col];
+        if (col0 + 32 * g < width) x[u][g] = row[g * step];
     }
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
@@ -246,9 +247,10 @@ combine_kernel(RouteArgs<T> a) {
       for (int g = 0; g < G; ++g) acc[g] += (Acc)to_math(x[u][g]) * w;
     }
   }
+  T *dst = a.dst + token * a.dst_stride + col0;
 #pragma unroll
   for (int g = 0; g < G; ++g)
-    if (col0 + 32 * g < a.vecs) a.dst[token * a.dst_stride + col0 + 32 * g] = round_from<T>(acc[g]);
+    if (col0 + 32 * g < width) dst[32 * g] = round_from<T>(acc[g]);
 }
 
 template <typename T> struct CombineGradArgs {
@@ -273,9 +275,9 @@ __global__ void __launch_bounds__(kRowThreads)
 combine_grad_kernel(CombineGradArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
   using Math = typename TypeTraits<T>::Math;
-  // vectors of each row in flight per lane: 64 to 128 bytes for whole vectors (2 of 32 bytes 140 us, 4 157 us, 16384 x 4 x 2048 half),
-  // as many elements as registers allow for single ones
-  constexpr int B = V == 1 ? 8 : V * sizeof(T) == 32 && sizeof(T) < 8 ? 2 : 4;
+  // vectors of each row in flight per lane (2 of 32 bytes 140 us, 4 157 us, 16384 x 4 x 2048 half; doubles, whose few pairs leave
+  // few warps, 127 us with 4 and 140 us with 2 at 567 x 8 x 5632)
+  constexpr int B = V == 1 || (V * sizeof(T) == 32 && sizeof(T) == 8) ? 4 : 2;
   pdl_prologue();
   const uint32_t team_bits = TEAMS ? a.team_bits : 5, team = 1u << team_bits, lane = threadIdx.x & (team - 1);
   const uint64_t pair = ((uint64_t)blockIdx.x * kRowThreads + threadIdx.x) >> team_bits;
@@ -286,21 +288,20 @@ combine_grad_kernel(CombineGradArgs<T> a) {
   Acc dot = 0;
   if (p >= 0) {
     const Math w = a.weight ? (Math)a.weight[pair] : (Math)1;
-    const T *g = a.grad + token * a.grad_stride, *r = a.rows + p * a.rows_stride;
-    T *o = ROWS ? a.grad_rows + p * a.out_stride : nullptr;
-    for (int64_t v0 = lane; v0 < a.vecs; v0 += team * B) {
+    const T *g = a.grad + token * a.grad_stride + (int64_t)lane * V * a.grad_col, *r = a.rows + p * a.rows_stride + (int64_t)lane * V * a.rows_col;
+    T *o = ROWS ? a.grad_rows + p * a.out_stride + lane * V : nullptr;
+    const int64_t g_step = (int64_t)team * V * a.grad_col, r_step = (int64_t)team * V * a.rows_col;
+    for (int32_t left = (int32_t)a.vecs - (int32_t)lane; left > 0; left -= (int32_t)team * B) {
       Pack<T, V> x[B], y[DOT ? B : 1];
 #pragma unroll
       for (int u = 0; u < B; ++u) {
-        const int64_t v = v0 + team * u;
-        if (v >= a.vecs) continue;
-        x[u] = load_kept<T, V>(g + v * V * a.grad_col);
-        if (DOT) y[u] = load_pack<T, V>(r + v * V * a.rows_col);
+        if (left <= (int32_t)team * u) continue;
+        x[u] = load_kept<T, V>(g + u * g_step);
+        if (DOT) y[u] = load_pack<T, V>(r + u * r_step);
       }
 #pragma unroll
       for (int u = 0; u < B; ++u) {
-        const int64_t v = v0 + team * u;
-        if (v >= a.vecs) continue;
+        if (left <= (int32_t)team * u) continue;
         if (DOT) {
 #pragma unroll
           for (int e = 0; e < V; ++e) dot += (Acc)to_math(x[u].e[e]) * (Acc)to_math(y[u].e[e]);
@@ -309,9 +310,12 @@ combine_grad_kernel(CombineGradArgs<T> a) {
           Pack<T, V> z;
 #pragma unroll
           for (int e = 0; e < V; ++e) z.e[e] = from_math<T>(to_math(x[u].e[e]) * w);
-          store_pack<T, V>(o + v * V, z);
+          store_pack<T, V>(o + u * team * V, z);
         }
       }
+      g += B * g_step;
+      if (DOT) r += B * r_step;
+      if (ROWS) o += (int64_t)B * team * V;
     }
   }
   if (!DOT) return;
@@ -378,7 +382,7 @@ int run_route(thcb200_ctx *ctx, bool dispatch, const MatView &dst, const MatView
   a.per = dispatch ? (uint64_t)a.vecs : (uint64_t)((a.vecs + a.team * lane_vecs - 1) / (a.team * lane_vecs));
   a.items = a.per * (uint64_t)s.tokens;
   const uint64_t per_cta = dispatch ? kRowThreads : kRowThreads / a.team, blocks = (a.items + per_cta - 1) / per_cta;
-  if (blocks >= (1ull << 31) || a.vecs >= (1ll << 31) || src.rows >= (1ll << 31)) { set_error("expert rows: tensor too large"); return THCB200_ERR_LIMIT; }
+  if (blocks >= (1ull << 31) || a.vecs >= (1ll << 31) - 1024 || src.rows >= (1ll << 31)) { set_error("expert rows: tensor too large"); return THCB200_ERR_LIMIT; }
   a.per32 = FastDiv32((uint32_t)a.per);
   a.chosen = (int)s.chosen;
   a.places = dispatch ? dst.rows : src.rows;
@@ -401,7 +405,10 @@ int run_route(thcb200_ctx *ctx, bool dispatch, const MatView &dst, const MatView
                    : batch == 4 ? launch(combine_ring_kernel<T, 4>) : launch(combine_ring_kernel<T, 8>);
       if (rc) return rc;
     } else {
-      launch_pdl(combine_kernel<T>, (unsigned)blocks, kRowThreads, 0, st, a);
+      auto launch = [&](auto kernel) { launch_pdl(kernel, (unsigned)blocks, kRowThreads, 0, st, a); };
+      if (batch <= 2) launch(combine_kernel<T, 2>);
+      else if (batch == 4) launch(combine_kernel<T, 4>);
+      else launch(combine_kernel<T, 8>);
     }
   }
   count_launch();
@@ -424,6 +431,7 @@ int run_combine_grad(thcb200_ctx *ctx, const MatView *out, void *grad_weight, co
   a.weight = (const typename Weight<T>::type *)weight;
   a.pairs = (uint64_t)(s.tokens * s.chosen);
   a.vecs = grad.cols * (int64_t)sizeof(T) / bytes;
+  if (a.vecs >= (1ll << 31) - 1024) { set_error("expert rows: tensor too large"); return THCB200_ERR_LIMIT; }
   a.chosen = FastDiv32((uint32_t)s.chosen);
   a.places = rows.rows;
   a.out_stride = out ? out->row_stride : 0;

@@ -53,6 +53,14 @@ template <typename T, int V> __device__ __forceinline__ void store_pack(T *p, co
   }
 }
 
+// Asynchronous copy of V elements (4, 8 or 16 bytes) into shared memory.
+template <typename T, int V> __device__ __forceinline__ void copy_async(void *shared, const T *p) {
+  const uint32_t s = (uint32_t)__cvta_generic_to_shared(shared);
+  if constexpr (sizeof(T) * V == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(s), "l"(p) : "memory");
+  else if constexpr (sizeof(T) * V == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" :: "r"(s), "l"(p) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(s), "l"(p) : "memory");
+}
+
 // An accumulator rounded once to the element type.
 template <typename T> __device__ __forceinline__ T round_from(typename TypeTraits<T>::Acc v) { return (T)v; }
 template <> __device__ __forceinline__ __half round_from<__half>(float v) { return __float2half_rn(v); }
