@@ -56,11 +56,16 @@ embedding_kernel(T *out, const T *weight, const int64_t *index, FastDiv32 vecs32
       tok[u] = i / vecs;
       col[u] = i - tok[u] * vecs;
     }
-    const int64_t k = index[(int64_t)tok[u] * index_stride] - 1;   // positions are 1-based (TH_INDEX_BASE)
-    if ((uint64_t)k < (uint64_t)rows) row[u] = k;
-    else if (col[u] == 0) atomicAdd(errors, 1u);
+    row[u] = index[(int64_t)tok[u] * index_stride] - 1;            // positions are 1-based (TH_INDEX_BASE)
   }
   Pack<T, V> x[kLookUnroll];
+  unsigned int bad = 0;
+#pragma unroll
+  for (int u = 0; u < kLookUnroll; ++u) {
+    if (base + (uint64_t)u * kLookThreads >= items || (uint64_t)row[u] < (uint64_t)rows) continue;
+    bad += col[u] == 0 ? 1u : 0u;
+    row[u] = -1;
+  }
 #pragma unroll
   for (int u = 0; u < kLookUnroll; ++u)
     if (row[u] >= 0) x[u] = load_pack<T, V>(weight + row[u] * row_stride + (int64_t)(col[u] * V) * col_stride);
@@ -71,6 +76,7 @@ embedding_kernel(T *out, const T *weight, const int64_t *index, FastDiv32 vecs32
     for (int e = 0; e < V; ++e) x[u].e[e] = from_math<T>(to_math(x[u].e[e]) * scale);
     store_pack<T, V>(out + (int64_t)tok[u] * out_stride + (int64_t)(col[u] * V), x[u]);
   }
+  if (bad) atomicAdd(errors, bad);
 }
 
 // ---- gradient ----------------------------------------------------------------------------------
@@ -188,9 +194,8 @@ embedding_grad_kernel(GradArgs<T> a) {
     Pack<T, V> zero;
 #pragma unroll
     for (int e = 0; e < V; ++e) zero.e[e] = round_from<T>((Acc)0);
-    for (uint32_t r = mine; r < a.zero_rows; r += groups) {
+    for (uint32_t r = mine; r < a.zero_rows; r += groups)
       if (!grad_smem[r]) store_pack<T, V>(a.table + (row0 + r) * a.table_stride + col, zero);
-    }
     return;
   }
   const uint32_t index = blockIdx.x * groups + mine;            // the group's chunk

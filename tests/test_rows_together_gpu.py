@@ -313,3 +313,22 @@ def test_tensors_of_another_device_are_refused(state):
     w = torch.zeros(4, 8, device="cuda:1")
     with pytest.raises(thc.THCError, match="different GPUs"):
         thc.Tensor.new(state, "Float").embedding(torch_handle(state, w, "Float"), to_device(state, np.array([1])), 1.0)
+
+
+def test_a_failed_workspace_leaves_the_call_undone_and_the_state_usable():
+    """The library's own allocation fails (injected on the host): the call reports it, its result is as it was, the next call works."""
+    own = thc.State()
+    index = rng("failed workspace").integers(1, 50, 20000)
+    go = np.ones((20000, 40), np.float32)
+    table, dgo, dindex = to_device(own, np.full((50, 40), 7, np.float32)), to_device(own, go), to_device(own, index)
+    slot, order, offsets = (thc.Tensor.new(own, "Long") for _ in range(3))
+    own.lib.thcb200_debug_fail_allocation(1)
+    with pytest.raises(thc.THCError, match="workspace"):
+        table.embeddingAccGrad(dgo, dindex, 1.0, 0, 0)
+    assert_bit_equal(table.numpy(), np.full((50, 40), 7, np.float32))
+    own.lib.thcb200_debug_fail_allocation(0)
+    table.embeddingAccGrad(dgo, dindex, 1.0, 0, 0)
+    assert_bit_equal(table.numpy(), np.repeat(np.bincount(index, minlength=51)[1:, None], 40, 1).astype(np.float32))
+    slot.expertSort(order, offsets, dindex, 50)
+    assert_bit_equal(offsets.numpy(), np.concatenate([[0], np.cumsum(np.bincount(index, minlength=51)[1:])]))
+    own.shutdown()
