@@ -19,9 +19,9 @@
 // depend on the compiler's choice of fused operations; the 8-bit form's parameter takes the approximate root and reciprocal.
 //
 // Both are bound by HBM in principle.  200 M float elements in 290 tensors, B200: 32-bit moments 800 us, 5.6 GB, 7000 GB/s (the
-// box's copy: 6558).  8-bit moments, 3.2 GB: 840 us, 3.8 TB/s, bound by instruction issue (90 per element): 1310 us with scalar
-// instructions, IEEE roots and byte conversions, 925 us packed, 890 us with four CTAs per SM, 860 us with the next tile
-// prefetched into the L2, 840 us with the rare exact codes apart.
+// box's copy: 6558).  8-bit moments, 3.2 GB: 795 us, 4.0 TB/s, bound by instruction issue (89 per element): 1310 us with scalar
+// instructions, IEEE roots and byte conversions, 925 us packed, 890 us with 1024 threads per SM, 860 us with the next tile
+// prefetched into the L2, 840 us with the rare exact codes apart, 795 us with CTAs of 128 threads.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -40,6 +40,7 @@ namespace {
 constexpr int kStepThreads = 256;
 constexpr int kStepItems = 8;                                 // elements per thread
 constexpr int kStepTile = kStepThreads * kStepItems;          // elements per CTA
+constexpr int kCodeThreads = 128, kCodeTile = kCodeThreads * kStepItems;   // the 8-bit step's: smaller CTAs fall into step less (69 -> 67 us, 20 M elements)
 constexpr int kUnitItems = THCB200_ADAMW_BLOCK;               // elements that share a unit: a warp's
 static_assert(kUnitItems == 32 * kStepItems, "a warp holds one block of codes");
 
@@ -140,9 +141,9 @@ template <typename T> __device__ __forceinline__ void store_eight(T *p, const Ei
       if (q.at(j) < q.n) p[q.at(j)] = x.e[j];
   }
 }
-__device__ __forceinline__ Place place_of(const StepEntry &e, uint32_t tile) {
+template <int TILE> __device__ __forceinline__ Place place_of(const StepEntry &e, uint32_t tile) {
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t block = (int64_t)(tile - e.first_tile) * kStepTile + (int64_t)warp * kUnitItems;
+  const int64_t block = (int64_t)(tile - e.first_tile) * TILE + (int64_t)warp * kUnitItems;
   Place q;
   q.n = e.n;
   q.wide = e.wide && block + kUnitItems <= e.n;
@@ -190,7 +191,7 @@ adamw_kernel(const __grid_constant__ StepTable<N> table, const StepScalars<typen
   using A = typename State<T>::type;
   pdl_prologue();
   const StepEntry &e = entry_of(table, blockIdx.x);
-  const Place q = place_of(e, blockIdx.x);
+  const Place q = place_of<kStepTile>(e, blockIdx.x);
   if (q.base >= q.n) return;
   Eight<A> p, m, v;
   Eight<T> g;
@@ -335,12 +336,12 @@ __device__ __forceinline__ F2 second_pair(const uint32_t (&c)[2], int j, F2 unit
 
 // Asks for the tile that this CTA's successor on the SM will work on: the loads of a short-lived CTA with many instructions
 // between them otherwise leave the memory idle while its warps compute.
-constexpr uint32_t kTilesAhead = 4 * kNumSM_B200;
-__device__ __forceinline__ void prefetch_ahead(const void *base, size_t esz, const StepEntry &e, uint32_t tile) {
-  const int64_t at = (int64_t)(tile - e.first_tile + kTilesAhead) * kStepTile;
+constexpr uint32_t kTilesAhead = 8 * kNumSM_B200;
+__device__ __forceinline__ void prefetch_ahead(const void *base, uint32_t esz, const StepEntry &e, uint32_t tile) {
+  const int64_t at = (int64_t)(tile - e.first_tile + kTilesAhead) * kCodeTile;
   const char *p = (const char *)base + at * esz;
-  if (at + kStepTile <= e.n && ((uintptr_t)p & 15) == 0)
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p), "r"((uint32_t)(kStepTile * esz)) : "memory");
+  if (at + kCodeTile <= e.n && ((uintptr_t)p & 15) == 0)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p), "r"(kCodeTile * esz) : "memory");
 }
 
 __device__ __forceinline__ float pick(const F2 (&x)[kStepItems / 2], int j) {      // element j, without an indexed register
@@ -351,12 +352,12 @@ __device__ __forceinline__ float pick(const F2 (&x)[kStepItems / 2], int j) {   
 }
 
 template <typename T, bool MASTER, int N>
-__global__ void __launch_bounds__(kStepThreads, 4)
+__global__ void __launch_bounds__(kCodeThreads, 8)
 adamw8_kernel(const __grid_constant__ StepTable<N> table, const __grid_constant__ StepPairs c) {
   pdl_prologue();
   const StepEntry &e = entry_of(table, blockIdx.x);
-  const Place q = place_of(e, blockIdx.x);
-  const int64_t block = (int64_t)(blockIdx.x - e.first_tile) * (kStepThreads / 32) + (threadIdx.x >> 5);
+  const Place q = place_of<kCodeTile>(e, blockIdx.x);
+  const int64_t block = (int64_t)(blockIdx.x - e.first_tile) * (kCodeThreads / 32) + (threadIdx.x >> 5);
   if (block * kUnitItems >= e.n) return;      // whole warps
   Eight<float> p;
   Eight<T> g;
@@ -365,10 +366,10 @@ adamw8_kernel(const __grid_constant__ StepTable<N> table, const __grid_constant_
   load_eight(g, (const T *)e.grad, q);
   load_codes(cm, (const int8_t *)e.m, q);
   load_codes(cv, (const uint8_t *)e.v, q);
-  if (threadIdx.x == 0) prefetch_ahead(MASTER ? e.master : e.param, MASTER ? 4 : sizeof(T), e, blockIdx.x);
-  if (threadIdx.x == 64) prefetch_ahead(e.grad, sizeof(T), e, blockIdx.x);
-  if (threadIdx.x == 128) prefetch_ahead(e.m, 1, e, blockIdx.x);
-  if (threadIdx.x == 192) prefetch_ahead(e.v, 1, e, blockIdx.x);
+  if (threadIdx.x < 4) {
+    const void *base = threadIdx.x == 0 ? (MASTER ? e.master : e.param) : threadIdx.x == 1 ? e.grad : threadIdx.x == 2 ? e.m : e.v;
+    prefetch_ahead(base, threadIdx.x == 0 ? (MASTER ? 4u : (uint32_t)sizeof(T)) : threadIdx.x == 1 ? (uint32_t)sizeof(T) : 1u, e, blockIdx.x);
+  }
   const F2 mu = both(e.m_unit[block]), vu = both(e.v_unit[block]);
   cm[0] ^= 0x80808080u;                       // signed codes as 128 + c
   cm[1] ^= 0x80808080u;
@@ -462,7 +463,7 @@ __global__ void __launch_bounds__(kStepThreads)
 adamw_values_kernel(const __grid_constant__ StepTable<N> table, const __grid_constant__ StepPairs c) {
   pdl_prologue();
   const StepEntry &e = entry_of(table, blockIdx.x);
-  const Place q = place_of(e, blockIdx.x);
+  const Place q = place_of<kStepTile>(e, blockIdx.x);
   const int64_t block = (int64_t)(blockIdx.x - e.first_tile) * (kStepThreads / 32) + (threadIdx.x >> 5);
   if (block * kUnitItems >= e.n) return;
   uint32_t cm[2], cv[2];
@@ -550,7 +551,7 @@ int launch_table(const thcb200_adamw_tensor *t, int count, size_t esz, StepKind 
     uint64_t tiles = 0;
     for (; i < count && table.count < N; ++i) {
       if (t[i].numel == 0) continue;
-      const uint64_t need = ((uint64_t)t[i].numel + kStepTile - 1) / kStepTile;
+      const uint64_t tile = kind == kStep8 ? kCodeTile : kStepTile, need = ((uint64_t)t[i].numel + tile - 1) / tile;
       if (need >= (1ull << 31)) { set_error("adamw: tensor %d is too large", i); return THCB200_ERR_LIMIT; }
       if (tiles + need >= (1ull << 31)) break;
       StepEntry &e = table.e[table.count++];
@@ -612,7 +613,7 @@ int run_step(const thcb200_adamw_tensor *t, int count, int bits, const thcb200_a
     });
   if constexpr (sizeof(T) < 8)
     return launch_table<N>(t, count, sizeof(T), kStep8, [&, pairs = step_pairs(s)](const StepTable<N> &table, unsigned tiles) {
-      launch_pdl(adamw8_kernel<T, MASTER, N>, tiles, kStepThreads, 0, st, table, pairs);
+      launch_pdl(adamw8_kernel<T, MASTER, N>, tiles, kCodeThreads, 0, st, table, pairs);
     });
   return THCB200_ERR_UNSUPPORTED;
 }
