@@ -555,6 +555,18 @@ template <typename R> StorageT<R> *storage_new(THCState *state, ptrdiff_t size) 
   return s;
 }
 
+// A storage over memory that is there already, on the device the memory is on.
+template <typename R> StorageT<R> *storage_over(THCState *state, R *data, ptrdiff_t size) {
+  StorageT<R> *s = storage_new<R>(state, 0);
+  s->data = data;
+  s->size = size;
+  if (data) {
+    cudaPointerAttributes attr;
+    if (cudaPointerGetAttributes(&attr, data) == cudaSuccess) s->device = attr.device; else cudaGetLastError();
+  }
+  return s;
+}
+
 template <typename R> void storage_free(THCState *, StorageT<R> *s) {
   if (!s) return;
   if (!(s->flag & TH_STORAGE_REFCOUNTED)) return;

@@ -273,19 +273,14 @@ class Tensor:
                 run *= n
         if storage_elems is None:
             storage_elems = 1 + sum((n - 1) * s for n, s in zip(sizes, strides))
-        nw = state.fn(kind, "newWithData", "Storage")
-        nw.restype = C.c_void_p
-        nw.argtypes = [C.c_void_p, C.c_void_p, C.c_ssize_t]
-        storage = C.c_void_p(nw(state.ptr, C.c_void_p(device_ptr), storage_elems))
-        clear = state.fn(kind, "clearFlag", "Storage")
-        clear.argtypes = [C.c_void_p, C.c_void_p, C.c_char]
-        clear(state.ptr, storage, bytes([4 | 2]))  # TH_STORAGE_FREEMEM | TH_STORAGE_RESIZABLE
-        t = cls.new(state, kind)
-        t._set_storage(storage, 0, sizes, strides)
-        free = state.fn(kind, "free", "Storage")
-        free.argtypes = [C.c_void_p, C.c_void_p]
-        free(state.ptr, storage)
-        return t
+        f = state.fn(kind, "newBorrowed")
+        if f.argtypes is None:
+            f.restype = C.c_void_p
+            f.argtypes = [C.c_void_p, C.c_void_p, C.c_ssize_t, C.c_int, C.c_void_p, C.c_void_p]
+        longs = C.c_long * len(sizes)
+        p = f(state.ptr, device_ptr, storage_elems, len(sizes), longs(*sizes), longs(*strides))
+        state.check()
+        return cls(state, kind, p)
 
     @staticmethod
     def _long_storage(state, values):

@@ -97,6 +97,9 @@ THC_API THLongStorage *THCTensor_(newStrideOf)(THCState *state, THCTensor *self)
 THC_API real *THCTensor_(data)(THCState *state, const THCTensor *self);
 
 THC_API THCTensor *THCTensor_(new)(THCState *state);
+/* a tensor over `elements` elements at `data` that somebody else owns: its storage is neither freed nor resized (an
+ * addition; one call for newWithData, clearFlag and setStorage) */
+THC_API THCTensor *THCTensor_(newBorrowed)(THCState *state, real *data, ptrdiff_t elements, int nDimension, const long *size, const long *stride);
 THC_API THCTensor *THCTensor_(newWithTensor)(THCState *state, THCTensor *tensor);
 THC_API THCTensor *THCTensor_(newWithStorage)(THCState *state, THCStorage *storage_, ptrdiff_t storageOffset_,
                                               THLongStorage *size_, THLongStorage *stride_);
