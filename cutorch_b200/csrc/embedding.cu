@@ -144,8 +144,10 @@ __device__ __forceinline__ void store_sums(typename TypeTraits<T>::Acc *p, const
 // CTAs 0 .. chunks-1 sum the rows named in their chunk of the sorted tokens; the ones behind clear the rows no token
 // names (accumulate = 0).
 // FEW: every CTA puts all tokens (at most kFewTokens) in order itself, and a row is summed by the chunk it begins in however
-// long it is: no sort before and no join behind.
-constexpr int kFewTokens = 128;
+// long it is: no sort before and no join behind.  One launch for three saves 1.2 to 2.4 us on rows that hardly repeat (64
+// tokens of 1024 halves 6.7 -> 5.4, of 1001 floats 6.5 -> 4.1), but a row's tokens are then added one after another, 0.28 us
+// each: all 64 the same 8.1 -> 18.8 us, all 128 9.9 -> 36.4.  64 bounds what that can cost.
+constexpr int kFewTokens = 64;
 
 template <typename T, int V, bool ADD, bool FEW>
 __global__ void __launch_bounds__(kGradThreads, 4)
@@ -374,9 +376,10 @@ int run_embedding(thcb200_ctx *ctx, const MatView &out, const MatView &w, const 
 }
 
 uint32_t grad_chunk(int64_t tokens, uint32_t groups, int64_t slabs) {
-  // long chunks leave fewer partial sums, short ones give every SM several CTAs
+  // long chunks leave fewer partial sums, short ones give every SM several CTAs (8, 6, 4 and 2 of them: 65536 tokens of 2048
+  // halves 156.5, 152.6, 152.7, 152.7 us, 5003 of 1001 floats 29.1, 29.1, 31.1, 38.5, 10562 of 2368 42.3, 38.7, 38.7, 41.2)
   uint32_t c = kGradMaxChunk;
-  while (c > 8 && (c * groups > kGradKeys || tokens / (c * groups) * slabs < 8 * kNumSM_B200)) c >>= 1;
+  while (c > 8 && (c * groups > kGradKeys || tokens / (c * groups) * slabs < 6 * kNumSM_B200)) c >>= 1;
   return c;
 }
 

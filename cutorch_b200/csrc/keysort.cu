@@ -12,6 +12,8 @@
 
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "core.cuh"
 #include "plan.h"
 
@@ -468,10 +470,41 @@ int launch_cluster(const SortInput &in, uint32_t *tkey, uint32_t *tpos, uint32_t
 
 }  // namespace
 
+// Items that one cluster takes on the current device: all kClusterItems where it grants clusters of kClusterMany CTAs, which
+// not every partition of a GPU need do; the portable size otherwise.
+static int64_t cluster_items() {
+  static std::atomic<int> granted[64];              // per device: 0 not asked, 1 yes, 2 no
+  int d = 0;
+  if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= 64) { cudaGetLastError(); return kClusterFew * kClusterThreads; }
+  int g = granted[d].load(std::memory_order_relaxed);
+  if (g == 0) {
+    auto kernel = cluster_sort_kernel<false, kClusterMaxRounds>;
+    const size_t smem = (size_t)kClusterMaxRounds * kClusterThreads * 8;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = kClusterMany;
+    cfg.blockDim = kClusterThreads;
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kClusterMany;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    const bool ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) == cudaSuccess &&
+                    cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                    cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0;
+    if (!ok) cudaGetLastError();
+    g = ok ? 1 : 2;
+    granted[d].store(g, std::memory_order_relaxed);
+  }
+  return g == 1 ? kClusterItems : (int64_t)kClusterFew * kClusterThreads;
+}
+
 size_t sort_by_key_bytes(int64_t n, int64_t) {
   if (n <= kPairItems) return 0;
   const size_t bins = 1u << kMaxDigitBits, items = 2 * align256(((size_t)n + 1) * 4);
-  return n <= kClusterItems ? items : align256((size_t)tiles_of(n) * bins * 4) + align256(bins * 4) + items;
+  return n <= cluster_items() ? items : align256((size_t)tiles_of(n) * bins * 4) + align256(bins * 4) + items;
 }
 
 int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, void *ws, cudaStream_t st) {
@@ -487,7 +520,7 @@ int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, uint3
   const uint32_t bins = 1u << digit_bits;
   const int64_t tiles = tiles_of(in.n);
   char *w = (char *)ws;
-  if (in.n <= kClusterItems) {
+  if (in.n <= cluster_items()) {
     uint32_t *tkey = (uint32_t *)w, *tpos = (uint32_t *)(w + align256(((size_t)in.n + 1) * 4));
     return launch_cluster<false>(in, tkey, tpos, out_key, out_pos, zero, nullptr, nullptr, nullptr, passes, digit_bits, st);
   }
@@ -518,7 +551,7 @@ int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, uint3
 }
 
 size_t sort_to_slots_bytes(int64_t n, int64_t limit) {
-  if (n <= kPairItems || (n <= kClusterItems && limit < kClusterBins)) return 0;
+  if (n <= kPairItems || (n <= cluster_items() && limit < kClusterBins)) return 0;
   const size_t bins = pow2_at_least((uint32_t)limit + 1);
   return align256((size_t)tiles_of(n) * bins * 4) + align256(bins * 4);
 }
@@ -532,7 +565,7 @@ int sort_to_slots(const SortInput &in, int64_t *slot, int64_t *order, int64_t *o
     return 0;
   }
   const int bits = bits_of(in.limit);
-  if (in.n <= kClusterItems && in.limit < kClusterBins)
+  if (in.n <= cluster_items() && in.limit < kClusterBins)
     return launch_cluster<true>(in, nullptr, nullptr, nullptr, nullptr, nullptr, slot, order, offsets, 1, bits, st);
   const uint32_t bins = pow2_at_least((uint32_t)in.limit + 1);
   const int64_t tiles = tiles_of(in.n);
