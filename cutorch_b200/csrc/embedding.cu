@@ -89,6 +89,7 @@ template <typename T, int V> constexpr bool kGradCopies = V > 1;
 template <typename T, int V> constexpr size_t kGradRing = kGradCopies<T, V> ? kGradStages * kGradBatch<T, V> * kGradThreads * sizeof(T) * V : 0;
 constexpr int kGradMaxChunk = 64;    // sorted tokens per CTA
 constexpr int kGradKeys = 1024;      // sorted tokens per CTA where rows are narrow and it takes several chunks
+constexpr uint32_t kJoinChunks = 64; // partial sums that one CTA joins
 
 template <typename T> struct GradArgs {
   T *table;
@@ -97,7 +98,7 @@ template <typename T> struct GradArgs {
   SortInput index;                           // the positions themselves, for few tokens
   typename TypeTraits<T>::Acc *partial;      // [chunk][head, tail][width]
   uint32_t *start_count;                     // rows that lie across more than two chunks
-  uint4 *starts;                             // for each: the chunk it begins in, the chunks behind that, its key
+  uint4 *starts;                             // for each, or each section: the chunk it begins in, the chunks behind that, its key, the section
   int64_t tokens, width, rows;
   int64_t grad_stride, grad_col, table_stride;
   uint32_t chunk, chunks;
@@ -118,14 +119,19 @@ __device__ __forceinline__ void write_row(const GradArgs<T> &a, uint32_t key, in
 
 // Partial sums lie in rows of `width` accumulators, on 16-byte boundaries where the rows' elements are taken in vectors.
 template <typename T, int V>
-__device__ __forceinline__ void add_partial(typename TypeTraits<T>::Acc (&acc)[V], const typename TypeTraits<T>::Acc *p) {
+__device__ __forceinline__ void add_partial(typename TypeTraits<T>::Acc (&acc)[V], const typename TypeTraits<T>::Acc *p) {   // past L1
   using Acc = typename TypeTraits<T>::Acc;
   constexpr int W = V > 1 ? 16 / sizeof(Acc) : 1;
 #pragma unroll
   for (int e = 0; e < V; e += W) {
-    const Pack<Acc, W> x = *reinterpret_cast<const Pack<Acc, W> *>(p + e);
+    if constexpr (V > 1) {
+      const int4 raw = __ldcg(reinterpret_cast<const int4 *>(p + e));
+      const Pack<Acc, W> x = *reinterpret_cast<const Pack<Acc, W> *>(&raw);
 #pragma unroll
-    for (int k = 0; k < W; ++k) acc[e + k] += x.e[k];
+      for (int k = 0; k < W; ++k) acc[e + k] += x.e[k];
+    } else {
+      acc[e] += __ldcg(p + e);
+    }
   }
 }
 template <typename T, int V>
@@ -305,13 +311,22 @@ embedding_grad_kernel(GradArgs<T> a) {
       const int64_t mid = (lo + hi) >> 1;
       if (a.key[mid * a.chunk] == last) lo = mid + 1; else hi = mid;
     }
-    a.starts[atomicAdd(a.start_count, 1u)] = make_uint4(index, (uint32_t)(lo - 1 - (int64_t)index), last, 0);
+    const uint32_t count = (uint32_t)(lo - 1 - (int64_t)index), sections = (count + kJoinChunks - 1) / kJoinChunks;
+    if (sections > 1) {
+      // the next chunk is this row's throughout and leaves its second place free: it counts the sections that are done
+      uint32_t *done = reinterpret_cast<uint32_t *>(a.partial + ((int64_t)index * 2 + 3) * a.width);
+      for (int64_t p = 0; p < (a.width + 32 * V - 1) / (32 * V); ++p) done[p] = 0;
+    }
+    const uint32_t at = atomicAdd(a.start_count, sections);
+    for (uint32_t s = 0; s < sections; ++s) a.starts[at + s] = make_uint4(index, count, last, s);
   }
 }
 
 // Joins the rows whose tokens cross chunks.  `starts` lists the chunks in which such a row begins (in the order their CTAs came
 // by, which no result depends on); a CTA takes a row and a piece of its columns, its warps take runs of the row's chunks, and
-// the warps' sums are added in chunk order.
+// the warps' sums are added in chunk order.  A row of more than kJoinChunks chunks is listed once for each section of that
+// many; the CTA that ends last adds the sections' sums, in their order.  (One row for all tokens, by one CTA and by sections:
+// 65536 of 64 halves 165 -> 34 us, 200000 of 2048 halves 300 -> 201.)
 constexpr int kJoinWarps = kGradThreads / 32;
 
 template <typename T, int V, bool ADD>
@@ -320,33 +335,57 @@ embedding_grad_join_kernel(GradArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
   pdl_prologue();
   __shared__ Acc part[kJoinWarps][32 * V];
+  __shared__ uint32_t ended;
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t rows = *a.start_count, pieces = (uint32_t)((a.width + 32 * V - 1) / (32 * V));
-  for (uint64_t job = blockIdx.x; job < (uint64_t)rows * pieces; job += gridDim.x) {
+  const uint32_t entries = *a.start_count, pieces = (uint32_t)((a.width + 32 * V - 1) / (32 * V));
+  for (uint64_t job = blockIdx.x; job < (uint64_t)entries * pieces; job += gridDim.x) {
     const uint4 row = a.starts[job / pieces];
-    const int64_t chunk = row.x, count = row.y, col = ((int64_t)(job % pieces) * 32 + lane) * V;
-    const int64_t per = (count + kJoinWarps - 1) / kJoinWarps;
-    const int64_t from = chunk + 1 + min(warp * per, count), to = chunk + 1 + min((warp + 1) * per, count);
-    Pack<T, V> old;
+    const uint32_t piece = (uint32_t)(job % pieces), sections = (row.y + kJoinChunks - 1) / kJoinChunks;
+    const int64_t col = ((int64_t)piece * 32 + lane) * V, stride = 2 * a.width;
     Acc acc[V];
+    // the sum of the n partial sums from p on, `step` apart, and of `more`: complete in the first warp
+    const auto join = [&](const Acc *p, int64_t step, uint32_t n, const Acc *more) {
+      const uint32_t per = (n + kJoinWarps - 1) / kJoinWarps, from = min(warp * per, n), to = min(from + per, n);
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] = 0;
-    if (col < a.width) {
-      if (ADD && warp == 0) old = load_pack<T, V>(a.table + (int64_t)row.z * a.table_stride + col);
-      if (warp == 0) add_partial<T, V>(acc, a.partial + (chunk * 2 + 1) * a.width + col);
+      for (int e = 0; e < V; ++e) acc[e] = 0;
+      if (col < a.width) {
+        if (more && warp == 0) add_partial<T, V>(acc, more);
 #pragma unroll 8
-      for (int64_t c = from; c < to; ++c) add_partial<T, V>(acc, a.partial + c * 2 * a.width + col);
+        for (uint32_t c = from; c < to; ++c) add_partial<T, V>(acc, p + c * step);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) part[warp][lane * V + e] = acc[e];
+      __syncthreads();
+      if (warp == 0 && col < a.width) {
+#pragma unroll
+        for (int w = 1; w < kJoinWarps; ++w)
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[e] += part[w][lane * V + e];
+      }
+    };
+    Pack<T, V> old;
+    if (ADD && warp == 0 && col < a.width) old = load_pack<T, V>(a.table + (int64_t)row.z * a.table_stride + col);
+    Acc *const behind = a.partial + ((int64_t)row.x + 1) * stride + col;      // the first chunk after the one it begins in
+    const uint32_t first = row.w * kJoinChunks;
+    join(behind + first * stride, stride, min(row.y - first, kJoinChunks), row.w == 0 ? behind - a.width : nullptr);
+    if (sections > 1) {
+      if (warp == 0) {
+        if (col < a.width) store_sums<T, V>(behind + first * stride, acc);
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) ended = atomicAdd(reinterpret_cast<uint32_t *>(a.partial + ((int64_t)row.x * 2 + 3) * a.width) + piece, 1u) + 1;
+      }
+      __syncthreads();
+      const bool all = ended == sections;
+      if (all) {
+        __threadfence();
+        join(behind, kJoinChunks * stride, sections, nullptr);
+      } else {
+        __syncthreads();           // `ended` is read before the next job
+        continue;
+      }
     }
-#pragma unroll
-    for (int e = 0; e < V; ++e) part[warp][lane * V + e] = acc[e];
-    __syncthreads();
-    if (warp == 0 && col < a.width) {
-#pragma unroll
-      for (int w = 1; w < kJoinWarps; ++w)
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] += part[w][lane * V + e];
-      write_row<T, V, ADD>(a, row.z, col, acc, old);
-    }
+    if (warp == 0 && col < a.width) write_row<T, V, ADD>(a, row.z, col, acc, old);
     __syncthreads();
   }
 }

@@ -140,6 +140,19 @@ def test_gradient_sums_tokens_of_a_row(state, tokens, how):
         check_grad(state, kind, rows, width, ix, 0.75, 0, accumulate)
 
 
+# rows with so many tokens that their partial sums are joined in sections, next to rows with few
+@pytest.mark.parametrize("kind", FP_KINDS)
+@pytest.mark.parametrize("width", [5, 72, 1040])
+@pytest.mark.parametrize("accumulate", [0, 1])
+def test_gradient_of_rows_with_very_many_tokens(state, kind, width, accumulate):
+    r = rng("sections", width, accumulate)
+    ix = r.integers(1, 41, 12011)
+    ix[r.random(ix.size) < 0.5] = 17
+    ix[r.random(ix.size) < 0.2] = 18
+    got = check_grad(state, kind, 40, width, ix, 1.5, 0, accumulate)
+    assert_bit_equal(check_grad(state, kind, 40, width, ix, 1.5, 0, accumulate), got, "the same call again")
+
+
 @pytest.mark.parametrize("kind", FP_KINDS)
 @pytest.mark.parametrize("width", [1, 3, 64, 1001, 2056])
 @pytest.mark.parametrize("accumulate", [0, 1])
