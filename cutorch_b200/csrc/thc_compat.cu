@@ -1770,6 +1770,12 @@ void check_apart(int arg, Span out, std::initializer_list<Span> others) {
     if (s.lo && out.lo < s.hi && s.lo < out.hi) th_arg_error(arg, "the result shares memory with another argument");
 }
 
+// A result that is one of the arguments: refused before anything is resized.
+void check_distinct(int arg, const void *out, std::initializer_list<const void *> others) {
+  for (const void *o : others)
+    if (out && out == o) th_arg_error(arg, "the result shares memory with another argument");
+}
+
 void resize2(THCState *state, TensorT<long> *t, long a) { tensor_raw_resize<long>(state, t, 1, &a, nullptr); }
 
 template <typename R> void embedding(THCState *state, TensorT<R> *result, TensorT<R> *weight, LongT *index, double scale) {
@@ -1778,6 +1784,7 @@ template <typename R> void embedding(THCState *state, TensorT<R> *result, Tensor
   THArgCheck(weight->nDimension == 2, 3, "expecting a matrix of rows");
   THArgCheck(index->nDimension >= 1, 4, "expecting a tensor of positions");
   THArgCheck(index->nDimension < THCB200_MAX_DIMS, 4, CUTORCH_DIM_WARNING);
+  check_distinct(2, result, {weight});
   long sz[THCB200_MAX_DIMS];
   for (int d = 0; d < index->nDimension; ++d) sz[d] = index->size[d];
   sz[index->nDimension] = weight->size[1];
@@ -1847,6 +1854,7 @@ template <typename R, typename A> void expert_dispatch(THCState *state, TensorT<
   check_slot(slot, 4);
   THArgCheck(slot->size[0] == src->size[0], 4, "slot must have a row for each row of src");
   check_weight<A>(weight, slot, 5);
+  check_distinct(2, rows, {src, weight});
   const long n = (long)tensor_nelement<long>(slot);
   if (rows->nDimension != 2 || rows->size[1] != src->size[1] || rows->size[0] < n) {
     const long sz[2] = {n, src->size[1]};
@@ -1873,6 +1881,7 @@ template <typename R, typename A> void expert_combine(THCState *state, TensorT<R
   THArgCheck(rows->nDimension == 2, 3, "expecting a matrix of rows");
   check_slot(slot, 4);
   check_weight<A>(weight, slot, 5);
+  check_distinct(2, result, {rows, weight});
   const long sz[2] = {slot->size[0], rows->size[1]};
   tensor_raw_resize<R>(state, result, 2, sz, nullptr);
   check_apart(2, span_of<R>(result), {span_of<R>(rows), span_of<long>(slot), span_of<A>(weight)});
@@ -1900,6 +1909,8 @@ void expert_combine_grad(THCState *state, TensorT<R> *grad_rows, TensorT<A> *gra
   check_slot(slot, 6);
   THArgCheck(slot->size[0] == grad_result->size[0], 6, "slot must have a row for each row of gradResult");
   check_weight<A>(weight, slot, 7);
+  check_distinct(2, grad_rows, {grad_weight, grad_result, rows, weight});
+  check_distinct(3, grad_weight, {grad_result, rows, weight});
   if (grad_rows) tensor_resize_as<R>(state, grad_rows, rows);
   if (grad_weight) tensor_raw_resize<A>(state, grad_weight, slot->nDimension, slot->size, nullptr);
   const Span gr = span_of<R>(grad_rows), gw = span_of<A>(grad_weight);
@@ -1954,6 +1965,53 @@ template <typename R> struct HeldList {
   void finish() { for (Held<R> &h : v) h.finish(); }
 };
 
+// Strided tensors of a list go to the step as copies, so what they share with others shows in the tensors themselves only.
+struct Piece {
+  const char *base, *lo, *hi;       // first element; the bytes from the lowest to the highest
+  ptrdiff_t esz;
+  int dims;
+  const long *size, *stride;
+  bool written, dense;
+};
+template <typename R> void add_pieces(std::vector<Piece> &out, TensorT<R> **list, int n, bool written) {
+  for (int i = 0; list && i < n; ++i) {
+    const TensorT<R> *t = list[i];
+    const Span s = span_of<R>(t);
+    if (!s.lo) continue;
+    out.push_back(Piece{(const char *)(t->storage->data + t->storageOffset), s.lo, s.hi, (ptrdiff_t)sizeof(R), t->nDimension, t->size, t->stride,
+                        written, tensor_is_contiguous<R>(t)});
+  }
+}
+// Whether two tensors surely have no byte in common.  Counted modulo a stride L, the dims whose strides are multiples of L
+// stay where they are, so all that a tensor takes lies in one window as long as its other dims reach; two windows that do not
+// meet are enough (columns of one matrix, slices of an inner dim).
+bool surely_apart(const Piece &a, const Piece &b) {
+  if (a.hi <= b.lo || b.hi <= a.lo) return true;
+  const Piece *both[2] = {&a, &b};
+  const auto window = [](const Piece &p, ptrdiff_t l) {
+    ptrdiff_t w = p.esz;
+    for (int d = 0; d < p.dims; ++d)
+      if (p.stride[d] < 0) return l + 1;
+      else if (p.size[d] > 1 && p.stride[d] * p.esz % l != 0) w += (p.size[d] - 1) * p.stride[d] * p.esz;
+    return w;
+  };
+  for (const Piece *p : both)
+    for (int d = 0; d < p->dims; ++d) {
+      const ptrdiff_t l = p->stride[d] * p->esz;
+      if (p->size[d] <= 1 || l <= 0) continue;
+      const ptrdiff_t at = ((b.base - a.base) % l + l) % l;
+      if (window(a, l) <= at && at + window(b, l) <= l) return true;
+    }
+  return false;
+}
+void check_pieces(std::vector<Piece> &p) {
+  std::sort(p.begin(), p.end(), [](const Piece &a, const Piece &b) { return a.lo < b.lo; });
+  for (size_t i = 0; i < p.size(); ++i)
+    for (size_t j = i + 1; j < p.size() && p[j].lo < p[i].hi; ++j)
+      if ((p[i].written || p[j].written) && !(p[i].dense && p[j].dense) && !surely_apart(p[i], p[j]))
+        th_arg_error(2, "a tensor that is written shares memory with another (each may be listed once)");
+}
+
 long unit_count(ptrdiff_t n) { return (long)((n + THCB200_ADAMW_BLOCK - 1) / THCB200_ADAMW_BLOCK); }
 
 template <typename R, typename A>
@@ -1973,6 +2031,15 @@ void adamw(THCState *state, TensorT<R> **param, TensorT<R> **grad, TensorT<A> **
     t.m = ha.add(state, m[i], k, true, 4, i);
     t.v = ha.add(state, v[i], k, true, 5, i);
     if (master) t.master = ha.add(state, master[i], k, true, 6, i);
+  }
+  if (!hp.v.empty() || !ha.v.empty()) {
+    std::vector<Piece> p;
+    add_pieces<R>(p, param, n, true);
+    add_pieces<R>(p, grad, n, false);
+    add_pieces<A>(p, m, n, true);
+    add_pieces<A>(p, v, n, true);
+    add_pieces<A>(p, master, n, true);
+    check_pieces(p);
   }
   check_core(thcb200_adamw(state_ctx(state), RealTraits<R>::dtype, 32, list.data(), n, &args, (void *)state_stream(state)));
   hp.finish();
@@ -2002,6 +2069,17 @@ void adamw8bit(THCState *state, TensorT<R> **param, TensorT<R> **grad, TensorT<c
     t.m_unit = hu.add(state, m_unit[i], unit_count(k), true, 6, i);
     t.v_unit = hu.add(state, v_unit[i], unit_count(k), true, 7, i);
     if (master) t.master = ha.add(state, master[i], k, true, 8, i);
+  }
+  if (!hp.v.empty() || !ha.v.empty() || !hm.v.empty() || !hv.v.empty() || !hu.v.empty()) {
+    std::vector<Piece> p;
+    add_pieces<R>(p, param, n, true);
+    add_pieces<R>(p, grad, n, false);
+    add_pieces<char>(p, m, n, true);
+    add_pieces<unsigned char>(p, v, n, true);
+    add_pieces<float>(p, m_unit, n, true);
+    add_pieces<float>(p, v_unit, n, true);
+    add_pieces<A>(p, master, n, true);
+    check_pieces(p);
   }
   check_core(thcb200_adamw(state_ctx(state), RealTraits<R>::dtype, 8, list.data(), n, &args, (void *)state_stream(state)));
   hp.finish();
@@ -2033,6 +2111,16 @@ void adamw_values(THCState *state, TensorT<float> **m_value, TensorT<float> **v_
     t.v = hv.add(state, v[i], k, false, 5, i);
     t.m_unit = hf.add(state, m_unit[i], unit_count(k), false, 6, i);
     t.v_unit = hf.add(state, v_unit[i], unit_count(k), false, 7, i);
+  }
+  if (!hf.v.empty() || !hm.v.empty() || !hv.v.empty()) {
+    std::vector<Piece> p;
+    add_pieces<float>(p, m_value, n, true);
+    add_pieces<float>(p, v_value, n, true);
+    add_pieces<char>(p, m, n, false);
+    add_pieces<unsigned char>(p, v, n, false);
+    add_pieces<float>(p, m_unit, n, false);
+    add_pieces<float>(p, v_unit, n, false);
+    check_pieces(p);
   }
   check_core(thcb200_adamw_values(state_ctx(state), list.data(), n, (void *)state_stream(state)));
   hf.finish();

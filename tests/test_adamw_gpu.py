@@ -283,3 +283,32 @@ def test_refusals(state):
         P.adamw(one(*G.tensors * 2), M, V, step=1, **HYPER)
     assert_bit_equal(t.numpy(), p)
     assert_bit_equal(M.tensors[0].numpy(), m)
+
+
+def test_strided_tensors_of_one_matrix(state):
+    """Strided tensors go to the step as copies: columns of one matrix beside one another are a list, the same column twice or
+    two that meet are not, nor is a moment or a gradient inside the parameter."""
+    r = rng("columns")
+    mats = {k: r.standard_normal((33, 12)).astype(np.float32) ** (2 if k == "v" else 1) for k in "pgmv"}
+    dev = {k: to_device(state, a) for k, a in mats.items()}
+    one = lambda *a: thc.TensorList(a)  # noqa: E731
+    column = lambda k, at, n: dev[k].narrow(1, at, n)  # noqa: E731
+    split = lambda k: one(column(k, 7, 5), column(k, 0, 4), column(k, 4, 3))  # noqa: E731
+    twice = lambda k, *at: one(*[column(k, a, 4) for a in at])  # noqa: E731
+    dense = lambda k, n: one(*[to_device(state, mats[k][:, :4]) for _ in range(n)])  # noqa: E731
+    own = dense("p", 1)
+    for refused in (lambda: twice("p", 0, 0).adamw(dense("g", 2), dense("m", 2), dense("v", 2), step=1, **HYPER),
+                    lambda: twice("p", 0, 3).adamw(dense("g", 2), dense("m", 2), dense("v", 2), step=1, **HYPER),
+                    lambda: dense("p", 2).adamw(dense("g", 2), twice("m", 2, 5), dense("v", 2), step=1, **HYPER),
+                    lambda: twice("p", 0).adamw(dense("g", 1), twice("p", 1), dense("v", 1), step=1, **HYPER),
+                    lambda: twice("p", 0).adamw(twice("p", 0), dense("m", 1), dense("v", 1), step=1, **HYPER),
+                    lambda: one(dev["p"]).adamw(one(dev["g"]), one(dev["m"]), one(dev["p"].transpose(0, 1)), step=1, **HYPER)):
+        with pytest.raises(thc.THCError, match="shares memory"):
+            refused()
+    assert all((dev[k].numpy() == a).all() for k, a in mats.items())
+    own.adamw(dense("g", 1), dense("m", 1), dense("v", 1), step=3, **HYPER)
+    twice("p", 0).adamw(twice("g", 0), twice("m", 0), twice("v", 0), step=3, **HYPER)
+    assert_bit_equal(dev["p"].numpy()[:, :4].copy(), own.tensors[0].numpy(), "one column list beside a contiguous one")
+    dev = {k: to_device(state, a) for k, a in mats.items()}
+    split("p").adamw(split("g"), split("m"), split("v"), step=3, **HYPER)
+    check_param(dev["p"].numpy().ravel(), *(mats[k].ravel() for k in "pgmv"), 3, "Float")

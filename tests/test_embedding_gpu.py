@@ -260,3 +260,10 @@ def test_refusals(state):
     with pytest.raises(TypeError, match="Long"):
         out.embedding(w, go, 1.0)
     assert_bit_equal(w.numpy(), np.ones((4, 6), np.float32))
+
+
+def test_a_result_that_is_the_table_is_refused_as_it_was(state):
+    w = to_device(state, np.arange(24, dtype=np.float32).reshape(4, 6))
+    with pytest.raises(thc.THCError, match="shares memory"):
+        w.embedding(w, to_device(state, np.array([1, 2, 3, 4, 1])), 1.0)
+    assert_bit_equal(w.numpy(), np.arange(24, dtype=np.float32).reshape(4, 6))

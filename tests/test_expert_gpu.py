@@ -243,3 +243,16 @@ def test_refusals(state):
         expert.expertSort(long(), long(), expert, 3)
     with pytest.raises(TypeError, match="Float"):
         thc.Tensor.new(state, "Half").expertCombine(to_device(state, np.ones((4, 8), np.float16)), slot, to_device(state, np.ones((2, 2))))
+
+
+def test_a_result_that_is_an_argument_is_refused_as_it_was(state):
+    a = np.arange(16, dtype=np.float32).reshape(2, 8)
+    x, rows, w = to_device(state, a), to_device(state, np.ones((4, 8), np.float32)), to_device(state, np.ones((2, 2), np.float32))
+    slot = to_device(state, np.array([[1, 2], [3, 4]]))
+    for call in (lambda: x.expertDispatch(x, slot, None), lambda: w.expertDispatch(x, slot, w), lambda: rows.expertCombine(rows, slot, None),
+                 lambda: w.expertCombine(rows, slot, w), lambda: x.expertCombineGrad(w, x, rows, slot, w),
+                 lambda: rows.expertCombineGrad(None, x, rows, slot, w), lambda: thc.Tensor.new(state, "Float").expertCombineGrad(x, x, rows, slot, w)):
+        with pytest.raises(thc.THCError, match="shares memory"):
+            call()
+    for t, want in ((x, a), (rows, np.ones((4, 8), np.float32)), (w, np.ones((2, 2), np.float32))):
+        assert_bit_equal(t.numpy(), want)
