@@ -539,12 +539,51 @@ class Tensor:
         self.state.check()
 
 
+_DIRECT = {        # per argument code: when an argument can go to C as it is, and what goes there
+    "T": ("type({a}) is Tensor and {a}.kind == kind", "{a}.ptr"),
+    "L": ("type({a}) is Tensor and {a}.kind == 'Long'", "{a}.ptr"),
+    "B": ("type({a}) is Tensor and {a}.kind == 'Byte'", "{a}.ptr"),
+    "A": ("({a} is None or type({a}) is Tensor and {a}.kind == ACC_KIND.get(kind))", "None if {a} is None else {a}.ptr"),
+    "f": ("type({a}) is float", "{a}"),
+    "l": ("type({a}) is int", "{a}"),
+    "i": ("type({a}) is int", "{a}"),
+}
+
+
 def _method(name):
-    # tensor methods in the Lua style: the receiver is the first C argument
-    def method(self, *args):
+    """A tensor method in the Lua style: the receiver is the first C argument.  A step of small tensors is bound by what its
+    calls take on the host, so arguments that need no conversion go to C from here (a lookup of one row 4.6 -> 4.0 us);
+    everything else, refusals among it, goes through `call`."""
+    ret, spec = SIGNATURES[name]
+
+    def general(self, *args):
         return self.call(name, self, *args)
-    method.__name__ = name
-    return method
+
+    general.__name__ = name
+    if ret == "R" or spec[0] != "T" or any(c not in _DIRECT for c in spec):
+        return general
+    names = [f"a{k}" for k in range(1, len(spec))]
+    fits = [_DIRECT[c][0].format(a=a) for c, a in zip(spec[1:], names)]
+    passed = ["state.ptr", "self.ptr"] + [_DIRECT[c][1].format(a=a) for c, a in zip(spec[1:], names)]
+    unpack = f"{', '.join(names)}, = args" if names else "pass"
+    source = f"""
+def {name}(self, *args):
+    state, kind = self.state, self.kind
+    f = ready.get(kind)
+    if f is not None and len(args) == {len(names)}:
+        {unpack}
+        if {' and '.join(fits) or 'True'}:
+            r = f({', '.join(passed)})
+            if state._failed():
+                state.check()
+            return r
+    r = self.call(name, self, *args)
+    ready[kind] = state._calls[kind, name][0]
+    return r
+"""
+    scope = {"Tensor": Tensor, "ACC_KIND": ACC_KIND, "ready": {}, "name": name}
+    exec(source, scope)
+    return scope[name]
 
 
 for _name in SIGNATURES:
@@ -564,41 +603,53 @@ class TensorList:
         if any(t.kind != self.kind for t in self.tensors):
             raise TypeError("tensors of different kinds in one list")
         self.array = (C.c_void_p * len(self.tensors))(*[t.ptr for t in self.tensors])
+        self.handles = C.c_void_p(C.addressof(self.array))
 
     def __len__(self):
         return len(self.tensors)
 
     def _call(self, name, lists, kinds, scalars=(), scalar_types=()):
+        """`name` of these tensors and `lists`, which are of `kinds` (None: no list), and the scalars behind the count."""
+        state, n = self.state, len(self.tensors)
+        args = [state.ptr, self.handles]
         for what, want in zip(lists, kinds):
-            if what is None:
-                continue
-            if not isinstance(what, TensorList):
+            if type(what) is TensorList and what.kind == want and len(what.tensors) == n:
+                args.append(what.handles)
+            elif what is None:
+                args.append(None)
+            elif not isinstance(what, TensorList):
                 raise TypeError(f"{name}: expected a TensorList")
-            if what.kind != want:
+            elif what.kind != want:
                 raise TypeError(f"{name}: expected {want} tensors, got {what.kind}")
-            if len(what) != len(self):
-                raise ValueError(f"{name}: lists of {len(self)} and {len(what)} tensors")
-        f = self.state.fn(self.kind, name)
-        if not hasattr(f, "prototype"):
-            f.argtypes = [C.c_void_p] * (1 + len(lists)) + [C.c_int, *scalar_types]
+            else:
+                raise ValueError(f"{name}: lists of {n} and {len(what)} tensors")
+        f = state._calls.get((self.kind, name, "list"))
+        if f is None:
+            f = state._calls[self.kind, name, "list"] = state.fn(self.kind, name)
+            f.argtypes = [C.c_void_p] * (2 + len(lists)) + [C.c_int, *scalar_types]
             f.restype = None
-            f.prototype = name
-        f(self.state.ptr, *[None if x is None else x.array for x in lists], len(self), *scalars)
-        self.state.check()
+        f(*args, n, *scalars)
+        if state._failed():
+            state.check()
 
     def adamw(self, grad, m, v, *, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, grad_scale=1.0, master=None):
         """One AdamW step of these parameters (THCTensor_(adamw)); m, v and master are of the parameters' accreal."""
         acc = ACC_KIND.get(self.kind)
-        self._call("adamw", (self, grad, m, v, master), (self.kind, self.kind, acc, acc, acc),
-                   (step, lr, beta1, beta2, eps, weight_decay, grad_scale), (C.c_long, *[C.c_double] * 6))
+        self._call("adamw", (grad, m, v, master), (self.kind, acc, acc, acc),
+                   (step, lr, beta1, beta2, eps, weight_decay, grad_scale), _STEP_SCALARS)
 
     def adamw8bit(self, grad, m, v, m_unit, v_unit, *, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, grad_scale=1.0,
                   master=None):
         """The same with the moments in 8 bits (THCTensor_(adamw8bit)): Char and Byte codes, a float unit per 256 elements."""
-        self._call("adamw8bit", (self, grad, m, v, m_unit, v_unit, master),
-                   (self.kind, self.kind, "Char", "Byte", "Float", "Float", ACC_KIND.get(self.kind)),
-                   (step, lr, beta1, beta2, eps, weight_decay, grad_scale), (C.c_long, *[C.c_double] * 6))
+        self._call("adamw8bit", (grad, m, v, m_unit, v_unit, master),
+                   (self.kind, "Char", "Byte", "Float", "Float", ACC_KIND.get(self.kind)),
+                   (step, lr, beta1, beta2, eps, weight_decay, grad_scale), _STEP_SCALARS)
 
     def adamwValues(self, v_value, m, v, m_unit, v_unit):
         """The floats that 8-bit moments stand for: these tensors receive the first moment's, v_value's the second's."""
-        self._call("adamwValues", (self, v_value, m, v, m_unit, v_unit), ("Float", "Float", "Char", "Byte", "Float", "Float"))
+        if self.kind != "Float":
+            raise TypeError(f"adamwValues: expected Float tensors, got {self.kind}")
+        self._call("adamwValues", (v_value, m, v, m_unit, v_unit), ("Float", "Char", "Byte", "Float", "Float"))
+
+
+_STEP_SCALARS = (C.c_long, *[C.c_double] * 6)      # step, lr, beta1, beta2, eps, weight decay, scale of the gradients
