@@ -310,18 +310,39 @@ template <typename T> struct CombineGradArgs {
   unsigned int *errors;
 };
 
+// A single element by a load that stays where it is written: the compiler otherwise sinks a batch's loads to their uses.
+template <typename T> __device__ __forceinline__ T load_single(const T *p) {
+  T x;
+  if constexpr (sizeof(T) == 2) {
+    uint16_t b;
+    asm volatile("ld.global.u16 %0, [%1];" : "=h"(b) : "l"(p));
+    memcpy(&x, &b, 2);
+  } else if constexpr (sizeof(T) == 4) {
+    uint32_t b;
+    asm volatile("ld.global.u32 %0, [%1];" : "=r"(b) : "l"(p));
+    memcpy(&x, &b, 4);
+  } else {
+    uint64_t b;
+    asm volatile("ld.global.u64 %0, [%1];" : "=l"(b) : "l"(p));
+    memcpy(&x, &b, 8);
+  }
+  return x;
+}
+
 // A warp (for narrow rows, a team of 4, 8 or 16 lanes) per (token, choice): the token's gradient row is read by the warps of its
 // choices, which sit side by side in the CTA, so all but the first find it in the L1.  16384 tokens x 4 of 2048 halves, 577 MB:
 // 88 us, 6.5 TB/s (116 us while the compiler kept two vectors in flight).  Rows of single elements are bound by instructions: a
 // step between loads that is added, not multiplied out in 64 bits, took 29625 x 2 x 151 halves from 72 to 36 us.
-template <typename T, int V, bool ROWS, bool DOT, bool TEAMS>
+// Of those, rows of more than 8 elements per lane have 8 in flight: 4 and 8 take 8.5 and 6.7 us (1003 x 3 x 1021 floats), 112.5 and
+// 98 us (20000 x 2 x 2047 halves), but 18.4 and 21.0 us (29625 x 2 x 151 halves); doubles 51.0 and 56.8 us (5000 x 4 x 777).
+template <typename T, int V, bool ROWS, bool DOT, bool TEAMS, bool LONG>
 __global__ void __launch_bounds__(kRowThreads)
 combine_grad_kernel(CombineGradArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
   using Math = typename TypeTraits<T>::Math;
   // vectors of each row in flight per lane (2 of 32 bytes 140 us, 4 157 us, 16384 x 4 x 2048 half; doubles, whose few pairs leave
   // few warps, 127 us with 4 and 140 us with 2 at 567 x 8 x 5632)
-  constexpr int B = V == 1 || (V * sizeof(T) == 32 && sizeof(T) == 8) ? 4 : 2;
+  constexpr int B = LONG ? 8 : V == 1 || (V * sizeof(T) == 32 && sizeof(T) == 8) ? 4 : 2;
   pdl_prologue();
   const uint32_t team_bits = TEAMS ? a.team_bits : 5, team = 1u << team_bits, lane = threadIdx.x & (team - 1);
   const uint64_t pair = ((uint64_t)blockIdx.x * kRowThreads + threadIdx.x) >> team_bits;
@@ -340,8 +361,13 @@ combine_grad_kernel(CombineGradArgs<T> a) {
 #pragma unroll
       for (int u = 0; u < B; ++u) {
         if (left <= (int32_t)team * u) continue;
-        x[u] = load_kept<T, V>(g + u * g_step);
-        if (DOT) y[u] = load_pack<T, V>(r + u * r_step);
+        if constexpr (V == 1) {
+          x[u].e[0] = load_single(g + u * g_step);
+          if (DOT) y[u].e[0] = load_single(r + u * r_step);
+        } else {
+          x[u] = load_kept<T, V>(g + u * g_step);
+          if (DOT) y[u] = load_pack<T, V>(r + u * r_step);
+        }
       }
 #pragma unroll
       for (int u = 0; u < B; ++u) {
@@ -490,15 +516,16 @@ int run_combine_grad(thcb200_ctx *ctx, const MatView *out, void *grad_weight, co
   const uint64_t per_cta = kRowThreads >> a.team_bits;
   const unsigned blocks = (unsigned)((a.pairs + per_cta - 1) / per_cta);
   auto launch = [&](auto kernel) { launch_pdl(kernel, blocks, kRowThreads, 0, st, a); };
-#define THCB_GRAD(V, TEAMS) \
+#define THCB_GRAD(V, TEAMS, LONG) \
   do { \
-    if (out && grad_weight) launch(combine_grad_kernel<T, V, true, true, TEAMS>); \
-    else if (out) launch(combine_grad_kernel<T, V, true, false, TEAMS>); \
-    else launch(combine_grad_kernel<T, V, false, true, TEAMS>); \
+    if (out && grad_weight) launch(combine_grad_kernel<T, V, true, true, TEAMS, LONG>); \
+    else if (out) launch(combine_grad_kernel<T, V, true, false, TEAMS, LONG>); \
+    else launch(combine_grad_kernel<T, V, false, true, TEAMS, LONG>); \
   } while (0)
-  if (bytes == 32) THCB_GRAD(32 / sizeof(T), false);
-  else if (bytes == 16) THCB_GRAD(16 / sizeof(T), true);
-  else THCB_GRAD(1, true);
+  if (bytes == 32) THCB_GRAD(32 / sizeof(T), false, false);
+  else if (bytes == 16) THCB_GRAD(16 / sizeof(T), true, false);
+  else if (sizeof(T) == 8 || a.vecs <= 8 * 32) THCB_GRAD(1, true, false);
+  else THCB_GRAD(1, false, sizeof(T) < 8);
 #undef THCB_GRAD
   count_launch();
   THCB_CUDA_TRY(cudaGetLastError());
