@@ -5,8 +5,8 @@
 // kClusterItems one cluster does all radix passes in one launch; beyond, each pass is three kernels: digit counts of
 // every tile, a scan of those counts over the tiles, and the scatter.  One pass, B200, us back to back in a graph:
 //   items        300   4096   8192  16384  32768  65536  131072  262144
-//   cluster      4.0    4.6    4.6    5.0    7.1    8.8    13.3    22.1    (64 keys; 500 keys: 4.9 .. 26)
-//   tiles                           10.8   10.6   10.9   11.1    11.7    15.7    (500 keys: 12 .. 17)
+//   cluster      3.2    3.5    4.4    5.0    5.9    8.1    13.3    22.1    (64 keys; 500 keys: 4.0 .. 26)
+//   tiles                           10.8   10.6   10.9    11.7    15.6    (500 keys: 12 .. 17)
 // (one CTA's shared memory instead of the cluster: 5.4 at 300 items, 10.8 at 4096.)
 #include "keysort.h"
 
@@ -298,54 +298,68 @@ pair_sort_kernel(KeySource src, uint32_t *out_key, uint32_t *out_pos, uint32_t *
 // ---- one cluster -------------------------------------------------------------------------------
 // Up to kClusterItems items: eight or sixteen CTAs that wait for one another in hardware, so that all passes fit one launch.
 // Sixteen (more than every GPU grants a cluster, hence the function attribute) where eight would take a second round: a pass is
-// bound by its instructions, about 100 per warp and round.  Items
-// go through global memory between the passes (they stay in the L2), digit counts through distributed shared memory.
-// A CTA first puts its items in order in its own shared memory and then writes each digit's run side by side: with eight
-// or sixteen SMs the rate of scattered stores is part of what a pass waits for.
+// bound by its instructions, about 100 per warp and round.  Each CTA holds an equal share of the items; between the passes
+// they go straight to the shared memory of the CTA that holds their place, digit counts are read from there as well.  (With
+// the items in global memory between the passes, and 1024 to a CTA however few there were, lookup gradients took 19.1 us in place
+// of 16.8 for 1419 tokens of 3008 halves, 29.2 in place of 27.8 for 5003 of 1001 floats.)
+// In the last pass a CTA first puts its items in order in its own shared memory and then writes each digit's run side by
+// side: with eight or sixteen SMs the rate of scattered stores is part of what a pass waits for.
 constexpr int kClusterFew = 8, kClusterMany = 16;
-constexpr int kClusterThreads = 1024;
-constexpr int kClusterWarps = kClusterThreads / 32;
+constexpr int kClusterThreads = 1024;      // or half as many, where they have no more items than that
 constexpr int kClusterMaxRounds = 4;
 constexpr int64_t kClusterItems = (int64_t)kClusterMany * kClusterThreads * kClusterMaxRounds;
 constexpr int kClusterBins = 1 << kMaxDigitBits;
+static_assert(kClusterBins <= kClusterThreads / 2, "a thread per bin");
 
 template <bool SLOTS, int ROUNDS>
 __global__ void __launch_bounds__(kClusterThreads)
-cluster_sort_kernel(KeySource src, uint32_t *tkey, uint32_t *tpos, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, int64_t *slot, int64_t *order,
-                    int64_t *offsets, uint32_t n, int passes, int digit_bits) {
+cluster_sort_kernel(KeySource src, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, int64_t *slot, int64_t *order, int64_t *offsets, uint32_t n,
+                    FastDiv32 share, int passes, int digit_bits) {
   pdl_prologue();
   cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
   extern __shared__ uint4 cluster_smem[];
-  uint32_t *skey = reinterpret_cast<uint32_t *>(cluster_smem), *spos = skey + ROUNDS * kClusterThreads;
-  __shared__ __align__(16) uint16_t count[kClusterWarps * kClusterBins];   // at most 4096 equal digits in a CTA
+  const uint32_t threads = blockDim.x, warps = threads >> 5, per_cta = share.d;
+  uint64_t *const held = reinterpret_cast<uint64_t *>(cluster_smem);          // items that came from the pass before: position above key
+  uint32_t *const skey = reinterpret_cast<uint32_t *>(held + (SLOTS ? 0 : ROUNDS * threads)), *const spos = skey + ROUNDS * threads;
+  __shared__ __align__(16) uint16_t count[kClusterThreads / 32 * kClusterBins];   // at most 4096 equal digits in a CTA
   __shared__ uint32_t total[kClusterBins], base[kClusterBins], local[kClusterBins], warp_sums[2][32];
   const uint32_t cta = cluster.block_rank(), ctas = cluster.num_blocks(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t bins = 1u << digit_bits;
-  const uint32_t first = (cta * kClusterWarps + warp) * (ROUNDS * 32) + lane;   // a warp's items are consecutive
-  for (int p = 0; p < passes; ++p) {
+  const uint32_t begin = min(cta * per_cta, n), end = min(begin + per_cta, n);
+  const uint32_t first = begin + warp * (ROUNDS * 32) + lane;                  // a warp's items are consecutive
+  for (int p = 0;; ++p) {
     const int shift = p * digit_bits;
-    const bool last = p == passes - 1, from_out = ((passes - 1 - p) & 1) != 0;
-    const uint32_t *in_key = from_out ? out_key : tkey, *in_pos = from_out ? out_pos : tpos;
-    uint32_t key[ROUNDS], rank[ROUNDS];
-    if (p > 0) src.key = in_key;
-    source_keys<ROUNDS>(key, src, first, 32, n);
-    for (uint32_t i = threadIdx.x; i < kClusterWarps * bins / 8; i += kClusterThreads) reinterpret_cast<uint4 *>(count)[i] = make_uint4(0, 0, 0, 0);
+    const bool last = p == passes - 1;
+    uint32_t key[ROUNDS], pos[ROUNDS], rank[ROUNDS];
+    if (p == 0) {
+      source_keys<ROUNDS>(key, src, first, 32, end);
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r) pos[r] = first + r * 32;
+    } else {
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r) {
+        const uint64_t x = first + r * 32 < end ? held[first - begin + r * 32] : 0;
+        key[r] = (uint32_t)x;
+        pos[r] = (uint32_t)(x >> 32);
+      }
+    }
+    for (uint32_t i = threadIdx.x; i < warps * bins / 8; i += threads) reinterpret_cast<uint4 *>(count)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     uint16_t *mine = count + warp * bins;
-    warp_ranks<ROUNDS>(key, shift, digit_bits, first, n, rank, mine, 1);
+    warp_ranks<ROUNDS>(key, shift, digit_bits, first, end, rank, mine, 1);
     __syncthreads();
     const uint32_t b = threadIdx.x;
     if (b < bins) {
       uint32_t run = 0;
 #pragma unroll 8
-      for (int w = 0; w < kClusterWarps; ++w) {
+      for (uint32_t w = 0; w < warps; ++w) {
         const uint32_t c = count[w * bins + b];
         count[w * bins + b] = (uint16_t)run;
         run += c;
       }
       total[b] = run;
     }
-    cluster.sync();
+    cluster.sync();                 // totals are there, and what each CTA held is in its registers
     uint32_t before = 0, all = 0, here = 0;
     if (b < bins) {
       here = total[b];
@@ -375,6 +389,7 @@ cluster_sort_kernel(KeySource src, uint32_t *tkey, uint32_t *tpos, uint32_t *out
       warp_sums[1][warp] = incl_here;
     }
     __syncthreads();
+    if (last) cluster.barrier_arrive();             // nobody reads the others' totals any more
     uint32_t front = 0, front_here = 0;
 #pragma unroll
     for (int w = 0; w < kClusterBins / 32; ++w) {
@@ -384,37 +399,48 @@ cluster_sort_kernel(KeySource src, uint32_t *tkey, uint32_t *tpos, uint32_t *out
     if (b < bins) {
       const uint32_t start = front + incl - all;
       local[b] = front_here + incl_here - here;
-      base[b] = start + before - local[b];            // place of the CTA's item at local place x of this bin: base + x
-      if (SLOTS && last && cta == 0 && b <= (uint32_t)src.limit) offsets[b] = (int64_t)start;
+      base[b] = start + before - (last ? local[b] : 0);   // place of the CTA's first item of this bin; last: less its place here
+      if (SLOTS && cta == 0 && b <= (uint32_t)src.limit) offsets[b] = (int64_t)start;
     }
     __syncthreads();
+    if (!last) {
+#pragma unroll
+      for (int r = 0; r < ROUNDS; ++r) {
+        if (first + r * 32 >= end) continue;
+        const uint32_t d = (key[r] >> shift) & (bins - 1);
+        uint32_t owner, at;
+        share.divmod(base[d] + mine[d] + rank[r], owner, at);
+        cluster.map_shared_rank(held, owner)[at] = (uint64_t)pos[r] << 32 | key[r];
+      }
+      cluster.sync();               // everything is in place for the next pass, and nobody reads this CTA's totals any more
+      continue;
+    }
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
       const uint32_t i = first + r * 32;
-      if (i >= n) continue;
+      if (i >= end) continue;
       const uint32_t d = (key[r] >> shift) & (bins - 1), x = local[d] + mine[d] + rank[r];
       skey[x] = key[r];
-      spos[x] = p == 0 ? i : __ldcg(in_pos + i);
+      spos[x] = pos[r];
       if constexpr (SLOTS) slot[i] = key[r] < (uint32_t)src.limit ? (int64_t)(base[d] + x) + 1 : 0;   // a single pass: item i is choice i
     }
     __syncthreads();
-    const uint32_t start_item = cta * (ROUNDS * kClusterThreads), items = start_item < n ? min(n - start_item, (uint32_t)(ROUNDS * kClusterThreads)) : 0;
-    for (uint32_t x = threadIdx.x; x < items; x += kClusterThreads) {
+    for (uint32_t x = threadIdx.x; x < end - begin; x += threads) {
       const uint32_t k = skey[x], q = base[(k >> shift) & (bins - 1)] + x;
       if constexpr (SLOTS) {
         order[q] = k < (uint32_t)src.limit ? (int64_t)spos[x] + 1 : 0;
       } else {
-        (from_out ? tkey : out_key)[q] = k;
-        (from_out ? tpos : out_pos)[q] = spos[x];
+        out_key[q] = k;
+        out_pos[q] = spos[x];
       }
     }
-    // the items are in place for the next pass, and nobody reads this CTA's totals any more
-    cluster.sync();
+    break;
   }
   if (!SLOTS && cta == 0 && threadIdx.x == 0) {
     out_key[n] = 0xffffffffu;
     *zero = 0;
   }
+  cluster.barrier_wait();
 }
 
 int bits_of(int64_t max_key) {
@@ -445,24 +471,23 @@ size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 int64_t tiles_of(int64_t n) { return (n + kTileItems - 1) / kTileItems; }
 
 template <bool SLOTS>
-int launch_cluster(const SortInput &in, uint32_t *tkey, uint32_t *tpos, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, int64_t *slot, int64_t *order,
-                   int64_t *offsets, int passes, int digit_bits, cudaStream_t st) {
+int launch_cluster(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, int64_t *slot, int64_t *order, int64_t *offsets, int passes,
+                   int digit_bits, cudaStream_t st) {
   const KeySource src = first_source(in, true);
-  const unsigned ctas = in.n <= kClusterFew * kClusterThreads ? kClusterFew : kClusterMany;
-  const int64_t rounds = (in.n + ctas * kClusterThreads - 1) / (ctas * kClusterThreads);
-#define THCB_CLUSTER(R) \
-  do { \
-    auto kernel = cluster_sort_kernel<SLOTS, R>; \
-    const size_t smem = (size_t)(R) * kClusterThreads * 8; \
-    if (smem + 40960 > 48 * 1024) THCB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
-    if (ctas > kClusterFew) THCB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)); \
-    THCB_CUDA_TRY(launch_pdl_cluster(kernel, ctas, ctas, kClusterThreads, smem, st, src, tkey, tpos, out_key, out_pos, zero, slot, order, offsets, \
-                                     (uint32_t)in.n, passes, digit_bits)); \
-  } while (0)
-  if (rounds <= 1) { THCB_CLUSTER(1); }
-  else if (rounds <= 2) { THCB_CLUSTER(2); }
-  else { THCB_CLUSTER(4); }
-#undef THCB_CLUSTER
+  const uint32_t n = (uint32_t)in.n, ctas = n <= kClusterFew * kClusterThreads ? kClusterFew : kClusterMany;
+  const uint32_t each = (n + ctas - 1) / ctas, threads = each <= kClusterThreads / 2 ? kClusterThreads / 2 : kClusterThreads;
+  auto launch = [&](auto kernel, uint32_t rounds) -> int {
+    const uint32_t share = (each + 32 * rounds - 1) / (32 * rounds) * (32 * rounds);
+    const size_t smem = (size_t)rounds * threads * (SLOTS ? 8 : 16);
+    if (smem + 40960 > 48 * 1024) THCB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (ctas > kClusterFew) THCB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    THCB_CUDA_TRY(launch_pdl_cluster(kernel, ctas, ctas, threads, smem, st, src, out_key, out_pos, zero, slot, order, offsets, n, FastDiv32(share), passes,
+                                     digit_bits));
+    return 0;
+  };
+  const int rc = each <= kClusterThreads ? launch(cluster_sort_kernel<SLOTS, 1>, 1) : each <= 2 * kClusterThreads ? launch(cluster_sort_kernel<SLOTS, 2>, 2)
+                                                                                                            : launch(cluster_sort_kernel<SLOTS, 4>, 4);
+  if (rc) return rc;
   count_launch();
   THCB_CUDA_TRY(cudaGetLastError());
   return 0;
@@ -479,7 +504,7 @@ static int64_t cluster_items() {
   int g = granted[d].load(std::memory_order_relaxed);
   if (g == 0) {
     auto kernel = cluster_sort_kernel<false, kClusterMaxRounds>;
-    const size_t smem = (size_t)kClusterMaxRounds * kClusterThreads * 8;
+    const size_t smem = (size_t)kClusterMaxRounds * kClusterThreads * 16;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = kClusterMany;
     cfg.blockDim = kClusterThreads;
@@ -503,8 +528,8 @@ static int64_t cluster_items() {
 
 size_t sort_by_key_bytes(int64_t n, int64_t) {
   if (n <= kPairItems) return 0;
-  const size_t bins = 1u << kMaxDigitBits, items = 2 * align256(((size_t)n + 1) * 4);
-  return n <= cluster_items() ? items : align256((size_t)tiles_of(n) * bins * 4) + align256(bins * 4) + items;
+  const size_t bins = 1u << kMaxDigitBits;
+  return n <= cluster_items() ? 0 : align256((size_t)tiles_of(n) * bins * 4) + align256(bins * 4) + 2 * align256(((size_t)n + 1) * 4);
 }
 
 int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, uint32_t *zero, void *ws, cudaStream_t st) {
@@ -520,10 +545,7 @@ int sort_by_key(const SortInput &in, uint32_t *out_key, uint32_t *out_pos, uint3
   const uint32_t bins = 1u << digit_bits;
   const int64_t tiles = tiles_of(in.n);
   char *w = (char *)ws;
-  if (in.n <= cluster_items()) {
-    uint32_t *tkey = (uint32_t *)w, *tpos = (uint32_t *)(w + align256(((size_t)in.n + 1) * 4));
-    return launch_cluster<false>(in, tkey, tpos, out_key, out_pos, zero, nullptr, nullptr, nullptr, passes, digit_bits, st);
-  }
+  if (in.n <= cluster_items()) return launch_cluster<false>(in, out_key, out_pos, zero, nullptr, nullptr, nullptr, passes, digit_bits, st);
   uint32_t *hist = (uint32_t *)w;
   w += align256((size_t)tiles * (1u << kMaxDigitBits) * 4);
   uint32_t *totals = (uint32_t *)w;
@@ -566,7 +588,7 @@ int sort_to_slots(const SortInput &in, int64_t *slot, int64_t *order, int64_t *o
   }
   const int bits = bits_of(in.limit);
   if (in.n <= cluster_items() && in.limit < kClusterBins)
-    return launch_cluster<true>(in, nullptr, nullptr, nullptr, nullptr, nullptr, slot, order, offsets, 1, bits, st);
+    return launch_cluster<true>(in, nullptr, nullptr, nullptr, slot, order, offsets, 1, bits, st);
   const uint32_t bins = pow2_at_least((uint32_t)in.limit + 1);
   const int64_t tiles = tiles_of(in.n);
   uint32_t *hist = (uint32_t *)ws, *totals = (uint32_t *)((char *)ws + align256((size_t)tiles * bins * 4));
