@@ -89,23 +89,27 @@ dispatch_kernel(RouteArgs<T> a) {
 
 // Rows of single elements: a warp takes kLaneItems elements per lane, 32 apart, of a token's row, and its lanes read the
 // token's slots and weights, one each: 1003 x 3 of 1021 floats 5.8 us with one element and its own slots per thread, 3.9 us so.
-constexpr int kLaneItems = 4;
+// Halves go by 8, as a lane moves few bytes otherwise (4 and 8: dispatch of 20000 x 2 of 2047 halves 72 and 62 us, 29625 x 2 of 151
+// 13.1 and 9.9 us, combine 103 and 95, 15.6 and 13.9 us); 8 floats are too many (3.9 and 4.7 us; combine of 20000 x 4 of 2047 182 and
+// 198 us).
+template <typename T> constexpr int kLaneItems = sizeof(T) == 2 ? 8 : 4;
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
 dispatch_single_kernel(RouteArgs<T> a) {
   using Math = typename TypeTraits<T>::Math;
+  constexpr int G = kLaneItems<T>;
   pdl_prologue();
   const uint32_t lane = threadIdx.x & 31;
   const uint64_t unit = (uint64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
   if (unit >= a.items) return;
   int64_t token, stretch;
   split_item(a, unit, &token, &stretch);
-  const int32_t col0 = (int32_t)stretch * (32 * kLaneItems) + (int32_t)lane, width = (int32_t)a.vecs;
+  const int32_t col0 = (int32_t)stretch * (32 * G) + (int32_t)lane, width = (int32_t)a.vecs;
   const T *src = a.src + token * a.src_stride + col0 * a.src_col;
   const int64_t step = 32 * a.src_col;
-  T x[kLaneItems];
+  T x[G];
 #pragma unroll
-  for (int g = 0; g < kLaneItems; ++g)
+  for (int g = 0; g < G; ++g)
     if (col0 + 32 * g < width) x[g] = src[g * step];
   for (int k0 = 0; k0 < a.chosen; k0 += 32) {
     const int k = k0 + (int)lane;
@@ -122,7 +126,7 @@ dispatch_single_kernel(RouteArgs<T> a) {
       if (p < 0) continue;
       T *q = a.dst + p * a.dst_stride + col0;
 #pragma unroll
-      for (int g = 0; g < kLaneItems; ++g)
+      for (int g = 0; g < G; ++g)
         if (col0 + 32 * g < width) q[32 * g] = a.weight ? from_math<T>(to_math(x[g]) * w) : x[g];
     }
   }
@@ -251,7 +255,7 @@ template <typename T, int BATCH>
 __global__ void __launch_bounds__(kRowThreads)
 combine_kernel(RouteArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
-  constexpr int G = kLaneItems;
+  constexpr int G = kLaneItems<T>;
   pdl_prologue();
   const uint32_t lane = threadIdx.x & 31;
   const uint64_t unit = (uint64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
@@ -448,7 +452,7 @@ int run_route(thcb200_ctx *ctx, bool dispatch, const MatView &dst, const MatView
   a.vecs = vec ? dst.cols / VB : dst.cols;
   const int batch = s.chosen <= 1 ? 1 : s.chosen <= 2 ? 2 : s.chosen <= 4 ? 4 : 8;
   a.team = vec && a.vecs <= 8 ? 8 : vec && a.vecs <= 16 ? 16 : 32;
-  const int64_t lane_vecs = vec ? kRingSlots / batch : kLaneItems;        // G of the combine kernels
+  const int64_t lane_vecs = vec ? kRingSlots / batch : kLaneItems<T>;     // G of the combine kernels
   const bool by_vector = dispatch && vec;
   a.per = by_vector ? (uint64_t)a.vecs : (uint64_t)((a.vecs + a.team * lane_vecs - 1) / (a.team * lane_vecs));
   a.items = a.per * (uint64_t)s.tokens;
