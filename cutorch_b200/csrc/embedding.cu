@@ -81,12 +81,15 @@ embedding_kernel(T *out, const T *weight, const int64_t *index, FastDiv32 vecs32
 
 // ---- gradient ----------------------------------------------------------------------------------
 constexpr int kGradThreads = 256;
-// Rows on their way while others are added: vectors by asynchronous copies into shared
-// memory, kGradStages batches of them; single elements, whose copies cost more instructions than they save, by loads of a batch.
+// Rows on their way while others are added, kGradBatch at a time: vectors by asynchronous copies into shared memory,
+// kGradStages batches of them; single elements, whose copies cost more instructions than they save, by loads.  A thread takes
+// kGradCols single elements of a row: 9979 tokens of 545 halves, 5003 of 1001 floats and 6000 of 2047 halves take 29.9, 27.5 and 42.3 us
+// by one (8 rows in a batch), 26.7, 24.6 and 36.8 by two, 27.6, 24.8 and 33.1 by four (of 2 rows).
 constexpr int kGradStages = 3;
-template <typename T, int V> constexpr int kGradBatch = V > 1 ? 4 : 8;
+constexpr int kGradBatch = 4;
 template <typename T, int V> constexpr bool kGradCopies = V > 1;
-template <typename T, int V> constexpr size_t kGradRing = kGradCopies<T, V> ? kGradStages * kGradBatch<T, V> * kGradThreads * sizeof(T) * V : 0;
+template <typename T, int V> constexpr int kGradCols = V > 1 ? 1 : 2;
+template <typename T, int V> constexpr size_t kGradRing = kGradCopies<T, V> ? kGradStages * kGradBatch * kGradThreads * sizeof(T) * V : 0;
 constexpr int kGradMaxChunk = 64;    // sorted tokens per CTA
 constexpr int kGradKeys = 1024;      // sorted tokens per CTA where rows are narrow and it takes several chunks
 constexpr uint32_t kJoinChunks = 64; // partial sums that one CTA joins
@@ -159,10 +162,11 @@ template <typename T, int V, bool ADD, bool FEW>
 __global__ void __launch_bounds__(kGradThreads, 4)
 embedding_grad_kernel(GradArgs<T> a) {
   using Acc = typename TypeTraits<T>::Acc;
-  constexpr int B = kGradBatch<T, V>;
+  constexpr int B = kGradBatch;
   pdl_prologue();
   const uint32_t group = 1u << a.group_bits, groups = kGradThreads >> a.group_bits, mine = threadIdx.x >> a.group_bits, member = threadIdx.x & (group - 1);
-  const int64_t col = ((int64_t)blockIdx.y * group + member) * V;
+  constexpr int G = kGradCols<T, V>;
+  const int64_t col = ((int64_t)blockIdx.y * (G * group) + member) * V, apart = group * V;      // column g of the thread: col + g * apart
   extern __shared__ Bytes16 grad_dynamic[];
   Pack<T, V> *grad_ring = reinterpret_cast<Pack<T, V> *>(grad_dynamic);
   uint32_t *grad_smem = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(grad_dynamic) + kGradRing<T, V>);
@@ -203,7 +207,11 @@ embedding_grad_kernel(GradArgs<T> a) {
 #pragma unroll
     for (int e = 0; e < V; ++e) zero.e[e] = round_from<T>((Acc)0);
     for (uint32_t r = mine; r < a.zero_rows; r += groups)
-      if (!grad_smem[r]) store_pack<T, V>(a.table + (row0 + r) * a.table_stride + col, zero);
+      if (!grad_smem[r]) {
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+          if (g == 0 || col + g * apart < a.width) store_pack<T, V>(a.table + (row0 + r) * a.table_stride + col + g * apart, zero);
+      }
     return;
   }
   const uint32_t index = blockIdx.x * groups + mine;            // the group's chunk
@@ -239,26 +247,39 @@ embedding_grad_kernel(GradArgs<T> a) {
     while (to < seen && skey[to + 1] == last) ++to;
   if (last == none)                                    // items without a row come last
     for (to = from; to < own && skey[to + 1] != none;) ++to;
-  Acc acc[V];
+  Acc acc[G][V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) acc[e] = 0;
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[g][e] = 0;
+  const auto there = [&](int g) { return g == 0 || col + g * apart < a.width; };
   const auto row_ends = [&](uint32_t i) { return i + 1 >= to || skey[i + 2] != skey[i + 1]; };
   // Adds token i; the sum of a row that ends there goes to the table, over `old` or not, or to the partial sums.
-  const auto add = [&](const Pack<T, V> &x, uint32_t i, const Pack<T, V> &old) {
+  const auto add = [&](const Pack<T, V> *x, uint32_t i, const Pack<T, V> *old) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] += (Acc)to_math(x.e[e]);
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[g][e] += (Acc)to_math(x[g].e[e]);
     if (!row_ends(i)) return;
     const uint32_t key = skey[i + 1];
     const bool in_head = head_long && key == first, in_tail = tail_long && key == last;
-    if (in_head || in_tail) store_sums<T, V>(a.partial + ((int64_t)index * 2 + (in_head ? 0 : 1)) * a.width + col, acc);
-    else write_row<T, V, ADD>(a, key, col, acc, old);
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] = 0;
+    for (int g = 0; g < G; ++g) {
+      if (there(g)) {
+        if (in_head || in_tail) store_sums<T, V>(a.partial + ((int64_t)index * 2 + (in_head ? 0 : 1)) * a.width + col + g * apart, acc[g]);
+        else write_row<T, V, ADD>(a, key, col + g * apart, acc[g], old[g]);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[g][e] = 0;
+    }
   };
-  Pack<T, V> old[ADD ? B : 1];
+  Pack<T, V> old[ADD ? B : 1][G];
   // what the sum of a row that ends at token i is added to comes with the token's batch
-  const auto read_old = [&](Pack<T, V> (&o)[ADD ? B : 1], uint32_t i, int u) {
-    if (ADD && row_ends(i)) o[ADD ? u : 0] = load_pack<T, V>(a.table + (int64_t)skey[i + 1] * a.table_stride + col);
+  const auto read_old = [&](Pack<T, V> (&o)[ADD ? B : 1][G], uint32_t i, int u) {
+    if (!ADD || !row_ends(i)) return;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      if (there(g)) o[ADD ? u : 0][g] = load_pack<T, V>(a.table + (int64_t)skey[i + 1] * a.table_stride + col + g * apart);
   };
   if constexpr (kGradCopies<T, V>) {
     // every thread copies what it will add itself, so that no barrier is needed: two batches on their way while one is added
@@ -281,18 +302,20 @@ embedding_grad_kernel(GradArgs<T> a) {
 #pragma unroll
       for (int u = 0; u < B; ++u) {
         if (i + u >= to) break;
-        add(grad_ring[(stage * B + u) * kGradThreads + threadIdx.x], i + u, old[ADD ? u : 0]);
+        add(&grad_ring[(stage * B + u) * kGradThreads + threadIdx.x], i + u, old[ADD ? u : 0]);
       }
       stage = stage == 2 ? 0 : stage + 1;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
   } else {
     for (uint32_t i = from; i < to; i += B) {
-      Pack<T, V> x[B];
+      Pack<T, V> x[B][G];
 #pragma unroll
       for (int u = 0; u < B; ++u) {
         if (i + u >= to) continue;
-        x[u] = load_pack<T, V>(a.grad + (int64_t)spos[i + u] * a.grad_stride + col * a.grad_col);
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+          if (there(g)) x[u][g] = load_pack<T, V>(a.grad + (int64_t)spos[i + u] * a.grad_stride + (col + g * apart) * a.grad_col);
         read_old(old, i + u, u);
       }
 #pragma unroll
@@ -430,9 +453,10 @@ int run_embedding_grad(thcb200_ctx *ctx, const MatView &table, const MatView &gr
   const bool vec = mat_vec(table, sizeof(T), 16) && mat_vec(grad, sizeof(T), 16);
   const int64_t vecs = vec ? table.cols / VB : table.cols;
   uint32_t group_bits = 8;
-  while (group_bits > 2 && (1 << (group_bits - 1)) >= vecs) --group_bits;
+  const int cols = vec ? kGradCols<T, VB> : kGradCols<T, 1>;
+  while (group_bits > 2 && (cols << (group_bits - 1)) >= vecs) --group_bits;
   const uint32_t group = 1u << group_bits, groups = kGradThreads >> group_bits, zero_rows = groups >= 8 ? kGradThreads : 32;
-  const int64_t slabs = (vecs + group - 1) / group;
+  const int64_t slabs = (vecs + cols * group - 1) / (cols * group);
   const uint32_t chunk = grad_chunk(in.n, groups, slabs);
   const int64_t chunks = (in.n + chunk - 1) / chunk, sum_ctas = (chunks + groups - 1) / groups;
   const int64_t zero = accumulate ? 0 : (table.rows + zero_rows - 1) / zero_rows;
