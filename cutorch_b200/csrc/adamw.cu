@@ -338,11 +338,11 @@ __device__ __forceinline__ F2 second_pair(const uint32_t (&c)[2], int j, F2 unit
 // Asks for the tile that this CTA's successor on the SM will work on: the loads of a short-lived CTA with many instructions
 // between them otherwise leave the memory idle while its warps compute.
 constexpr uint32_t kTilesAhead = 8 * kNumSM_B200;
-__device__ __forceinline__ void prefetch_ahead(const void *base, uint32_t esz, const StepEntry &e, uint32_t tile) {
-  const int64_t at = (int64_t)(tile - e.first_tile + kTilesAhead) * kCodeTile;
+template <int TILE> __device__ __forceinline__ void prefetch_ahead(const void *base, uint32_t esz, const StepEntry &e, uint32_t tile) {
+  const int64_t at = (int64_t)(tile - e.first_tile + kTilesAhead) * TILE;
   const char *p = (const char *)base + at * esz;
-  if (at + kCodeTile <= e.n && ((uintptr_t)p & 15) == 0)
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p), "r"(kCodeTile * esz) : "memory");
+  if (at + TILE <= e.n && ((uintptr_t)p & 15) == 0)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(p), "r"(TILE * esz) : "memory");
 }
 
 __device__ __forceinline__ float pick(const F2 (&x)[kStepItems / 2], int j) {      // element j, without an indexed register
@@ -369,7 +369,7 @@ adamw8_kernel(const __grid_constant__ StepTable<N> table, const __grid_constant_
   load_codes(cv, (const uint8_t *)e.v, q);
   if (threadIdx.x < 4) {
     const void *base = threadIdx.x == 0 ? (MASTER ? e.master : e.param) : threadIdx.x == 1 ? e.grad : threadIdx.x == 2 ? e.m : e.v;
-    prefetch_ahead(base, threadIdx.x == 0 ? (MASTER ? 4u : (uint32_t)sizeof(T)) : threadIdx.x == 1 ? (uint32_t)sizeof(T) : 1u, e, blockIdx.x);
+    prefetch_ahead<kCodeTile>(base, threadIdx.x == 0 ? (MASTER ? 4u : (uint32_t)sizeof(T)) : threadIdx.x == 1 ? (uint32_t)sizeof(T) : 1u, e, blockIdx.x);
   }
   const F2 mu = both(e.m_unit[block]), vu = both(e.v_unit[block]);
   cm[0] ^= 0x80808080u;                       // signed codes as 128 + c
@@ -458,7 +458,8 @@ adamw8_kernel(const __grid_constant__ StepTable<N> table, const __grid_constant_
   }
 }
 
-// What the codes stand for: param and master of the entry are the float results for the first and second moment.
+// What the codes stand for: param and master of the entry are the float results for the first and second moment.  200 M elements,
+// 2 GB: 307 us, the copy rate; 362 us without the prefetch, 341 and 387 us with two and four blocks a warp.
 template <int N>
 __global__ void __launch_bounds__(kStepThreads)
 adamw_values_kernel(const __grid_constant__ StepTable<N> table, const __grid_constant__ StepPairs c) {
@@ -469,6 +470,7 @@ adamw_values_kernel(const __grid_constant__ StepTable<N> table, const __grid_con
   if (block * kUnitItems >= e.n) return;
   uint32_t cm[2], cv[2];
   Eight<float> m, v;
+  if (threadIdx.x < 2) prefetch_ahead<kStepTile>(threadIdx.x ? e.v : e.m, 1, e, blockIdx.x);
   load_codes(cm, (const int8_t *)e.m, q);
   load_codes(cv, (const uint8_t *)e.v, q);
   const F2 mu = both(e.m_unit[block]), vu = both(e.v_unit[block]);
