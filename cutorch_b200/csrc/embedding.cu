@@ -79,16 +79,18 @@ embedding_kernel(T *out, const T *weight, const int64_t *index, FastDiv32 vecs32
 }
 
 // Rows of single elements: a warp, or a team of 4, 8 or 16 lanes for narrow rows, takes kLookItems elements per lane, a team's width
-// apart, of a token's row, and reads its position once: 20000 tokens of 2047 halves 55 us, 5003 of 1001 floats 6.8 us, where elements
-// taken one by one took 103 and 13.4 (4 floats a lane 7.6; 8 doubles 12.7 us, 4 12.2 us for 9000 of 777).
+// apart, of a token's row, and reads its position once: 20000 tokens of 2047 halves 34 us, 5003 of 1001 floats 5.3 us, where elements
+// taken one by one took 103 and 13.4.  It is bound by instructions (79 % of the issue slots before addresses were constants apart, 55 us).
 template <typename T> constexpr int kLookItems = sizeof(T) == 8 ? 4 : 8;
-template <typename T>
+// PLAIN: whole warps and neighbouring columns, so that a lane's addresses are one and constants.
+template <typename T, bool PLAIN>
 __global__ void __launch_bounds__(kLookThreads)
-embedding_single_kernel(T *out, const T *weight, const int64_t *index, FastDiv32 per32, uint64_t per, uint64_t items, uint32_t team_bits, int64_t width,
+embedding_single_kernel(T *out, const T *weight, const int64_t *index, FastDiv32 per32, uint64_t per, uint64_t items, uint32_t bits, int64_t width,
                         int64_t index_stride, int64_t rows, int64_t row_stride, int64_t col_stride, int64_t out_stride, typename TypeTraits<T>::Math scale,
                         unsigned int *errors) {
   constexpr int G = kLookItems<T>;
   pdl_prologue();
+  const uint32_t team_bits = PLAIN ? 5 : bits;
   const uint64_t unit = ((uint64_t)blockIdx.x * kLookThreads + threadIdx.x) >> team_bits;
   if (unit >= items) return;
   uint64_t token, stretch;
@@ -107,16 +109,18 @@ embedding_single_kernel(T *out, const T *weight, const int64_t *index, FastDiv32
     if (col0 == 0) atomicAdd(errors, 1u);
     return;
   }
-  const T *p = weight + row * row_stride + col0 * col_stride;
+  const T *p = weight + row * row_stride + (PLAIN ? col0 : col0 * col_stride);
   T *q = out + (int64_t)token * out_stride + col0;
-  const int64_t step = team * col_stride;
+  const int64_t step = PLAIN ? 32 : team * col_stride;
+  if (width <= col0) return;
+  const uint32_t left = (uint32_t)min(width - col0, (int64_t)(G * 32));       // columns from the lane's first on
   T x[G];
 #pragma unroll
   for (int g = 0; g < G; ++g)
-    if (col0 + g * team < width) x[g] = p[g * step];
+    if (g * team < left) x[g] = p[g * step];
 #pragma unroll
   for (int g = 0; g < G; ++g)
-    if (col0 + g * team < width) q[g * team] = from_math<T>(to_math(x[g]) * scale);
+    if (g * team < left) q[g * team] = from_math<T>(to_math(x[g]) * scale);
 }
 
 // ---- gradient ----------------------------------------------------------------------------------
@@ -467,8 +471,9 @@ int run_embedding(thcb200_ctx *ctx, const MatView &out, const MatView &w, const 
     const uint64_t per = ((uint64_t)out.cols + (G << team_bits) - 1) / (G << team_bits), items = per * (uint64_t)out.rows;
     const uint64_t per_cta = kLookThreads >> team_bits, blocks = (items + per_cta - 1) / per_cta;
     if (blocks >= (1ull << 31) || per >= (1ull << 31)) { set_error("embedding: tensor too large"); return THCB200_ERR_LIMIT; }
-    launch_pdl(embedding_single_kernel<T>, (unsigned)blocks, kLookThreads, 0, st, (T *)out.data, (const T *)w.data, index, FastDiv32((uint32_t)per), per,
-               items, team_bits, out.cols, index_stride, w.rows, w.row_stride, w.col_stride, out.row_stride, (Math)scale, errors);
+    launch_pdl(team_bits == 5 && w.col_stride == 1 ? embedding_single_kernel<T, true> : embedding_single_kernel<T, false>, (unsigned)blocks, kLookThreads, 0,
+               st, (T *)out.data, (const T *)w.data, index, FastDiv32((uint32_t)per), per, items, team_bits, out.cols, index_stride, w.rows, w.row_stride,
+               w.col_stride, out.row_stride, (Math)scale, errors);
     count_launch();
     THCB_CUDA_TRY(cudaGetLastError());
     return 0;
