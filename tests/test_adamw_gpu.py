@@ -312,3 +312,9 @@ def test_strided_tensors_of_one_matrix(state):
     dev = {k: to_device(state, a) for k, a in mats.items()}
     split("p").adamw(split("g"), split("m"), split("v"), step=3, **HYPER)
     check_param(dev["p"].numpy().ravel(), *(mats[k].ravel() for k in "pgmv"), 3, "Float")
+
+
+@pytest.mark.parametrize("count", [79, 80, 81])
+def test_tables_of_every_size(state, count):
+    test_lists_of_every_length(state, count, 32)
+    test_lists_of_every_length(state, count, 8)

@@ -267,3 +267,41 @@ def test_a_result_that_is_the_table_is_refused_as_it_was(state):
     with pytest.raises(thc.THCError, match="shares memory"):
         w.embedding(w, to_device(state, np.array([1, 2, 3, 4, 1])), 1.0)
     assert_bit_equal(w.numpy(), np.arange(24, dtype=np.float32).reshape(4, 6))
+
+
+# the shares of one cluster's CTAs and the rounds they take, at their borders, and the first size beyond one cluster
+@pytest.mark.parametrize("tokens", [4096, 4097, 8192, 8193, 16384, 16385, 32768, 32769, 65536, 65537])
+@pytest.mark.parametrize("rows", [300, 131072])
+def test_gradient_at_the_borders_of_the_sort(state, tokens, rows):
+    r = rng("borders", tokens, rows)
+    ix = positions(r, tokens, rows, "frequencies")
+    ix[::7] = 0                                        # no row: counted
+    check_grad(state, "Float", rows, 4, ix, 1.0, 0, 0)
+    check_grad(state, "Half", rows, 3, ix, 0.5, int(ix[1]), 1)
+
+
+@pytest.mark.parametrize("tokens", [63, 64, 65])
+@pytest.mark.parametrize("how", ["uniform", "same", "frequencies"])
+@pytest.mark.parametrize("kind", FP_KINDS)
+def test_gradient_of_few_tokens(state, tokens, how, kind):
+    for width, accumulate in ((7, 0), (257, 1), (1024, 0)):
+        check_grad(state, kind, 200, width, positions(rng("few", tokens, how), tokens, 200, how), 1.25, 3, accumulate)
+
+
+# single elements: narrow teams of lanes, whole warps, columns apart
+@pytest.mark.parametrize("kind", FP_KINDS)
+@pytest.mark.parametrize("width", [1, 2, 15, 17, 31, 33, 63, 65, 127, 129, 255, 257, 515])
+def test_lookup_of_single_elements(state, kind, width):
+    r = rng("single", kind, width)
+    w = r.standard_normal((50, 2 * width)).astype(NP_OF_KIND[kind])
+    ix = r.integers(-1, 53, 77)
+    bad = (ix < 1) | (ix > 50)
+    rows = np.clip(ix, 1, 50) - 1
+    apart = w.reshape(50, width, 2)
+    for view, host in ((to_device(state, w).narrow(1, 1, width), w[:, 1:1 + width]), (to_device(state, apart).select(2, 1), apart[:, :, 1])):
+        out = to_device(state, np.full((77, width), 5, host.dtype))
+        take_errors(state)
+        out.embedding(view, to_device(state, ix), 2.0)              # a product with a power of two is exact
+        want = np.where(bad[:, None], np.array(5, host.dtype), host[rows] * host.dtype.type(2))
+        assert_bit_equal(out.numpy(), want.astype(host.dtype))
+        assert take_errors(state) == int(bad.sum())

@@ -256,3 +256,49 @@ def test_a_result_that_is_an_argument_is_refused_as_it_was(state):
             call()
     for t, want in ((x, a), (rows, np.ones((4, 8), np.float32)), (w, np.ones((2, 2), np.float32))):
         assert_bit_equal(t.numpy(), want)
+
+
+@pytest.mark.parametrize("n", [4096, 4097, 8192, 8193, 16385, 32769, 65536, 65537])
+@pytest.mark.parametrize("experts", [1, 2, 300, 511, 512])
+def test_sort_at_its_borders(state, n, experts):
+    expert = rng("sort borders", n, experts).integers(0, experts + 1, n)
+    long = lambda: thc.Tensor.new(state, "Long")  # noqa: E731
+    slot, order, offsets = long(), long(), long()
+    slot.expertSort(order, offsets, to_device(state, expert), experts)
+    routed = np.argsort(np.where(expert == 0, experts + 1, expert), kind="stable")[:np.count_nonzero(expert)]
+    want = np.zeros(n, np.int64)
+    want[routed] = np.arange(1, routed.size + 1)
+    assert (slot.numpy() == want).all()
+    assert (order.numpy() == np.concatenate([routed + 1, np.zeros(n - routed.size, np.int64)])).all()
+    assert (offsets.numpy() == np.array([np.count_nonzero((expert > 0) & (expert <= e)) for e in range(experts + 1)])).all()
+
+
+# rows of single elements: dispatch, combine and its gradient at the borders of a lane's elements, with strided token rows
+@pytest.mark.parametrize("kind", ["Half", "Float", "Double"])
+@pytest.mark.parametrize("width", [1, 31, 127, 129, 255, 257, 261, 515])
+@pytest.mark.parametrize("chosen", [1, 3, 9])
+def test_rows_of_single_elements(state, kind, width, chosen):
+    r = rng("single rows", kind, width, chosen)
+    dt, wt = {"Half": (np.float16, np.float32), "Float": (np.float32, np.float32), "Double": (np.float64, np.float64)}[kind]
+    tokens = 11
+    slot = r.permutation(tokens * chosen).reshape(tokens, chosen) + 1
+    slot[r.random(slot.shape) < 0.2] = 0
+    x, rows = r.integers(-4, 5, (tokens, 2 * width)).astype(dt), r.integers(-4, 5, (tokens * chosen, width)).astype(dt)
+    weight = r.integers(1, 4, slot.shape).astype(wt)                       # small whole numbers: every product and sum is exact
+    dslot, dweight = to_device(state, slot), to_device(state, weight)
+    for how in ("narrow", "every other"):
+        dx = to_device(state, x).narrow(1, 0, width) if how == "narrow" else to_device(state, x.reshape(tokens, width, 2)).select(2, 0)
+        hx = x[:, :width] if how == "narrow" else x.reshape(tokens, width, 2)[:, :, 0]
+        out = to_device(state, np.full_like(rows, 7))
+        out.expertDispatch(dx, dslot, dweight)
+        want = np.full_like(rows, 7)
+        want[slot[slot > 0] - 1] = (hx[:, None, :] * weight[:, :, None].astype(dt))[slot > 0]
+        assert (out.numpy() == want).all()
+        gr, gw = to_device(state, np.full_like(rows, 7)), thc.Tensor.new(state, "Double" if kind == "Double" else "Float")
+        gr.expertCombineGrad(gw, dx, to_device(state, rows), dslot, dweight)
+        assert (gr.numpy() == want).all()
+        full = rows[np.maximum(slot, 1) - 1].astype(np.float64) * (slot > 0)[:, :, None]
+        assert (gw.numpy() == (full * hx[:, None, :].astype(np.float64)).sum(-1)).all()
+    y = thc.Tensor.new(state, kind)
+    y.expertCombine(to_device(state, rows), dslot, dweight)
+    assert (y.numpy() == (full * weight[:, :, None]).sum(1)).all()
