@@ -137,6 +137,11 @@ template <typename T, int V> constexpr size_t kGradRing = kGradCopies<T, V> ? kG
 constexpr int kGradMaxChunk = 64;    // sorted tokens per CTA
 constexpr int kGradKeys = 1024;      // sorted tokens per CTA where rows are narrow and it takes several chunks
 constexpr uint32_t kJoinChunks = 64; // partial sums that one CTA joins
+constexpr uint32_t kGradMinChunk = 8, kGradMinGroup = 4;
+// Words a CTA's groups hold their tokens' keys and places in, and at most: kGradKeys tokens, or the shortest chunk for every group.
+constexpr uint32_t grad_words(uint32_t groups, uint32_t chunk) { return groups * (4 * chunk + 2); }
+constexpr uint32_t kGradMaxWords = 4 * kGradKeys + 2 * kGradThreads / kGradMinGroup;
+static_assert(kGradMinChunk * kGradThreads / kGradMinGroup <= kGradKeys && kGradMaxWords >= kGradThreads, "also the flags of the rows a CTA clears");
 
 template <typename T> struct GradArgs {
   T *table;
@@ -498,7 +503,7 @@ uint32_t grad_chunk(int64_t tokens, uint32_t groups, int64_t slabs) {
   // long chunks leave fewer partial sums, short ones give every SM several CTAs (8, 6, 4 and 2 of them: 65536 tokens of 2048
   // halves 156.5, 152.6, 152.7, 152.7 us, 5003 of 1001 floats 29.1, 29.1, 31.1, 38.5, 10562 of 2368 42.3, 38.7, 38.7, 41.2)
   uint32_t c = kGradMaxChunk;
-  while (c > 8 && (c * groups > kGradKeys || tokens / (c * groups) * slabs < 6 * kNumSM_B200)) c >>= 1;
+  while (c > kGradMinChunk && (c * groups > kGradKeys || tokens / (c * groups) * slabs < 6 * kNumSM_B200)) c >>= 1;
   return c;
 }
 
@@ -511,7 +516,7 @@ int run_embedding_grad(thcb200_ctx *ctx, const MatView &table, const MatView &gr
   const int64_t vecs = vec ? table.cols / VB : table.cols;
   uint32_t group_bits = 8;
   const int cols = vec ? kGradCols<T, VB> : kGradCols<T, 1>;
-  while (group_bits > 2 && (cols << (group_bits - 1)) >= vecs) --group_bits;
+  while ((1u << group_bits) > kGradMinGroup && (cols << (group_bits - 1)) >= vecs) --group_bits;
   const uint32_t group = 1u << group_bits, groups = kGradThreads >> group_bits, zero_rows = groups >= 8 ? kGradThreads : 32;
   const int64_t slabs = (vecs + cols * group - 1) / (cols * group);
   const uint32_t chunk = grad_chunk(in.n, groups, slabs);
@@ -549,12 +554,14 @@ int run_embedding_grad(thcb200_ctx *ctx, const MatView &table, const MatView &gr
   a.zero_rows = zero_rows;
   a.scale = (Acc)scale;
   const dim3 grid((unsigned)(sum_ctas + zero), (unsigned)slabs);
-  const size_t smem = (vec ? kGradRing<T, VB> : kGradRing<T, 1>) + std::max((size_t)groups * (4 * chunk + 2), (size_t)zero_rows) * sizeof(uint32_t);   // at most 66 KiB
+  const size_t ring = vec ? kGradRing<T, VB> : kGradRing<T, 1>, smem = ring + std::max(grad_words(groups, chunk), zero_rows) * sizeof(uint32_t);
+  const size_t most = ring + kGradMaxWords * sizeof(uint32_t);             // 64.5 KiB
   const int64_t piece = vec ? 32 * VB : 32, pieces = (table.cols + piece - 1) / piece;
   const unsigned join = (unsigned)(chunks * pieces < 8 * kNumSM_B200 ? chunks * pieces : 8 * kNumSM_B200);
   const bool joined = !few && chunks > 2;      // a row across more than two chunks needs three
   auto sum = [&](auto kernel) -> int {
-    if (smem + 2048 > 48 * 1024) THCB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // the limit is the kernel's, not the call's: what one call needs would be below what another thread's is about to launch with
+    if (most + 2048 > 48 * 1024) THCB_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
     launch_pdl(kernel, grid, kGradThreads, smem, st, a);
     return 0;
   };

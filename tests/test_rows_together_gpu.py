@@ -244,6 +244,46 @@ def test_host_threads_with_a_stream_each():
     own.shutdown()
 
 
+def test_host_threads_whose_gradients_need_different_shared_memory():
+    """One kernel, rows of 4 floats on half of the threads and of 1024 on the others: 57856 and 49288 bytes of shared memory.  What a
+    thread asks for must not take away what another is about to launch with."""
+    import torch
+    own = thc.State()
+    failures = []
+    ready = threading.Barrier(4)
+
+    def work(k):
+        try:
+            torch.cuda.set_device(0)
+            stream = torch.cuda.Stream()
+            own.set_stream(stream.cuda_stream, 0)
+            r = rng("shared memory", k)
+            width, tokens = (4, 3000) if k % 2 else (1024, 300)
+            index = r.integers(1, 60, tokens)
+            go = r.standard_normal((tokens, width)).astype(np.float32)
+            dgo, dindex, table = to_device(own, go), to_device(own, index), to_device(own, np.zeros((60, width), np.float32))
+            table.embeddingAccGrad(dgo, dindex, 1.0, 0, 0)
+            first = table.numpy()
+            ready.wait(60)
+            for _ in range(3000):
+                table.embeddingAccGrad(dgo, dindex, 1.0, 0, 0)
+            assert_bit_equal(table.numpy(), first)
+            total, size, count = ro.embedding_grad(np.zeros((60, width), np.float32), go, index, 1.0, 0, 0)
+            assert (np.abs(first - total) <= 2.0 ** -24 * np.abs(total) + count[:, None] * 2.0 ** -52 * size).all()
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001
+            failures.append(f"thread {k}: {e!r}")
+            ready.abort()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
+    own.shutdown()
+
+
 # one pass and three of the tiled sort, its first size and others
 @pytest.mark.parametrize("tokens", [8193, 16385, 65536, 65537, 150001])
 @pytest.mark.parametrize("rows", [200, 70000, 3000000])
