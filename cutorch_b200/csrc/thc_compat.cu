@@ -2097,11 +2097,28 @@ void adamw_values(THCState *state, TensorT<float> **m_value, TensorT<float> **v_
   HeldList<float> hf(current);
   HeldList<char> hm(current);
   HeldList<unsigned char> hv(current);
+  // Every result gets its size before any address is taken: a storage that grows moves, with all tensors that share it.  A result
+  // that would be resized while the call names it once more is refused as it is.
+  std::vector<std::pair<TensorT<float> *, int>> grow;
   for (int i = 0; i < n; ++i) {
     THArgCheck(m[i] != nullptr && v[i] != nullptr && m_value[i] != nullptr && v_value[i] != nullptr, 2, "tensor %d is missing", i + 1);
     const ptrdiff_t k = tensor_nelement<char>(m[i]);
-    if (tensor_nelement<float>(m_value[i]) != k) tensor_raw_resize<float>(state, m_value[i], m[i]->nDimension, m[i]->size, nullptr);
-    if (tensor_nelement<float>(v_value[i]) != k) tensor_raw_resize<float>(state, v_value[i], m[i]->nDimension, m[i]->size, nullptr);
+    if (tensor_nelement<float>(m_value[i]) != k) grow.emplace_back(m_value[i], i);
+    if (tensor_nelement<float>(v_value[i]) != k) grow.emplace_back(v_value[i], i);
+  }
+  if (!grow.empty()) {
+    std::vector<const void *> named;
+    for (int i = 0; i < n; ++i)
+      for (const void *t : {(const void *)m_value[i], (const void *)v_value[i], (const void *)m_unit[i], (const void *)v_unit[i]}) named.push_back(t);
+    std::sort(named.begin(), named.end());
+    for (const auto &g : grow) {
+      const auto at = std::lower_bound(named.begin(), named.end(), (const void *)g.first);
+      if (at + 1 != named.end() && at[1] == *at) th_arg_error(2, "the result shares memory with another argument");
+    }
+    for (const auto &g : grow) tensor_raw_resize<float>(state, g.first, m[g.second]->nDimension, m[g.second]->size, nullptr);
+  }
+  for (int i = 0; i < n; ++i) {
+    const ptrdiff_t k = tensor_nelement<char>(m[i]);
     thcb200_adamw_tensor &t = list[(size_t)i];
     t = thcb200_adamw_tensor{};
     t.numel = k;

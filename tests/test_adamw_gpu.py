@@ -318,3 +318,35 @@ def test_strided_tensors_of_one_matrix(state):
 def test_tables_of_every_size(state, count):
     test_lists_of_every_length(state, count, 32)
     test_lists_of_every_length(state, count, 8)
+
+
+def test_values_that_share_a_storage_which_grows(state):
+    """The results are windows of one storage, a unit too, and the last of them has to grow: the memory moves, and every tensor of the
+    call with it."""
+    r = rng("values in one storage")
+    sizes = (300, 5000)
+    cm, cv = [r.integers(-127, 128, n).astype(np.int8) for n in sizes], [r.integers(0, 256, n).astype(np.uint8) for n in sizes]
+    um, uv = ([(r.random(-(-n // 256)) * 1e-5).astype(np.float32) for n in sizes] for _ in range(2))
+    m, v, mu, vu = lists(state, cm, cv, um, uv)
+    base = to_device(state, np.concatenate([um[0], np.zeros(310, np.float32)]))
+    firsts = base.narrow(0, 2, 300), base.narrow(0, 302, 10)
+    seconds = [thc.Tensor.new(state, "Float") for _ in sizes]
+    units = thc.TensorList([base.narrow(0, 0, 2), mu.tensors[1]])
+    thc.TensorList(firsts).adamwValues(thc.TensorList(seconds), m, v, units, vu)
+    for t, c, u, value in ((firsts[0], cm[0], um[0], ro.first_value), (firsts[1], cm[1], um[1], ro.first_value),
+                           (seconds[0], cv[0], uv[0], ro.second_value), (seconds[1], cv[1], uv[1], ro.second_value)):
+        assert_bit_equal(t.numpy(), ro.decode(c, u, value))
+    assert_bit_equal(base.numpy()[:302], np.concatenate([um[0], ro.decode(cm[0], um[0], ro.first_value)]))
+
+
+def test_values_over_an_argument_are_refused_as_it_was(state):
+    r = rng("values refused")
+    um, uv = (r.random(3).astype(np.float32) for _ in range(2))
+    m, v, mu, vu = lists(state, [r.integers(-127, 128, 600).astype(np.int8)], [r.integers(0, 256, 600).astype(np.uint8)], [um], [uv])
+    other = thc.TensorList([thc.Tensor.new(state, "Float")])
+    for first, second in ((mu, other), (other, mu), (vu, other), (other, vu), (other, other)):
+        with pytest.raises(thc.THCError, match="shares memory"):
+            first.adamwValues(second, m, v, mu, vu)
+    assert_bit_equal(mu.tensors[0].numpy(), um)
+    assert_bit_equal(vu.tensors[0].numpy(), uv)
+    assert other.tensors[0].numpy().ndim == 0, "an empty tensor still"
