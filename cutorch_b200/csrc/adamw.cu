@@ -23,6 +23,7 @@
 // instructions, IEEE roots and byte conversions, 925 us packed, 890 us with 1024 threads per SM, 860 us with the next tile
 // prefetched into the L2, 840 us with the rare exact codes apart, 795 us with CTAs of 128 threads.
 #include <cuda_fp16.h>
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -310,6 +311,9 @@ __device__ __forceinline__ F2 codes_near(F2 x, F2 root, F2 dither, float &rare, 
 constexpr float kFirstTop = (float)(1.0 / 16129.0), kSecondTop = (float)(1.0 / (255.0 * 255.0 * 255.0 * 255.0));
 // Blocks whose largest value is below these (where a unit would leave the normal floats) are stored as zero.
 constexpr float kFirstLeast = 1e-30f, kSecondLeast = 1e-28f;
+// A block whose largest value is not finite has no unit: NaN, and with it the whole block (an infinite one would leave its element
+// an infinity of either sign, as the codes of NaN fall, beside NaN for the code 0).
+__device__ __forceinline__ float unit_of(float most, float least, float top) { return most < least ? 0.0f : most <= FLT_MAX ? most * top : NAN; }
 
 // The thread's eight codes, as two words.
 template <typename T>
@@ -405,8 +409,7 @@ adamw8_kernel(const __grid_constant__ StepTable<N> table, const __grid_constant_
   // over the warp by the bits: a NaN's are above infinity's and win
   mmost = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(mmost)));
   vmost = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(vmost)));
-  // not (x < least): a NaN stays
-  const float nmu = mmost < kFirstLeast ? 0.0f : mmost * kFirstTop, nvu = vmost < kSecondLeast ? 0.0f : vmost * kSecondTop;
+  const float nmu = unit_of(mmost, kFirstLeast, kFirstTop), nvu = unit_of(vmost, kSecondLeast, kSecondTop);
   const float mi = nmu > 0 ? 1.0f / nmu : 0.0f, vi = nvu > 0 ? 1.0f / nvu : 0.0f;
   const uint32_t h = (uint32_t)q.at(0) * kDitherPlace + c.dither, hstep = q.wide ? kDitherPlace : 32u * kDitherPlace;
   F2 km[kStepItems / 2], kv[kStepItems / 2];

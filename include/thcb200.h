@@ -455,8 +455,9 @@ THCB200_API int thcb200_expert_combine_grad(thcb200_ctx *ctx, const thcb200_tens
  * dtype: the type of param and grad.  bits = 32: m and v are float (double for F64).  bits = 8 (F16, F32): m holds int8 and
  * v uint8 codes, and every THCB200_ADAMW_BLOCK elements share one float in m_unit and one in v_unit; all zero is the start.
  * A code c of m stands for c|c| * unit, one of v for c^4 * unit; values between two codes are rounded up or down by a hash of
- * the element's place and the step, so that averages keep their expectation.  A NaN or infinite gradient makes its
- * block's moments NaN.  master (F16; all tensors or none): float copies the step is computed from.
+ * the element's place and the step, so that averages keep their expectation.  A first moment that is NaN or infinite makes its
+ * block's first moments NaN, a second moment the second ones: a NaN or infinite gradient does both.  A block whose largest first
+ * moment is below 1e-30 (second: 1e-28) is stored as zeros.  master (F16; all tensors or none): float copies the step is computed from.
  * A list in which an array that is written shares memory with another is refused.  The arguments, step among them, are
  * fixed when a call is captured into a graph. */
 #define THCB200_ADAMW_BLOCK 256

@@ -118,7 +118,7 @@ def adamw8(p, g, cm, cv, um, uv, step, lr, beta1, beta2, eps, weight_decay, grad
         padded = np.zeros(-(-n // BLOCK) * BLOCK, _F)
         padded[:n] = x
         most = padded.reshape(-1, BLOCK).max(1)
-        unit = np.where(most < least, _F(0), most * _F(1.0 / float(value(np.array([top]))[0])))
+        unit = np.where(most < least, _F(0), np.where(most <= np.finfo(_F).max, most * _F(1.0 / float(value(np.array([top]))[0])), _F(np.nan)))
         inverse = np.where(unit > 0, _F(1) / np.where(unit > 0, unit, _F(1)), _F(0))
         out.append((_encode(x * np.repeat(inverse, BLOCK)[:n], dith, value, top), unit))
     (km, nmu), (kv, nvu) = out

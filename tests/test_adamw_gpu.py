@@ -350,3 +350,31 @@ def test_values_over_an_argument_are_refused_as_it_was(state):
     assert_bit_equal(mu.tensors[0].numpy(), um)
     assert_bit_equal(vu.tensors[0].numpy(), uv)
     assert other.tensors[0].numpy().ndim == 0, "an empty tensor still"
+
+
+@pytest.mark.parametrize("kind", ["Half", "Float"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_a_block_whose_moments_are_not_finite_is_not_a_number(state, kind, bad):
+    """A unit cannot stand beside an infinite moment: the whole block's moments become NaN, not infinities of either sign beside
+    zeros.  Where only the square of a gradient is beyond float, the second moments do."""
+    r = rng("not finite")
+    n = 1300
+    g = r.standard_normal(n).astype(NP_OF_KIND[kind])
+    g[300], g[1290] = bad, bad                                  # a block of vectors, and the ragged last one
+    if kind == "Float":
+        g[600] = 1e25
+    one = lists(state, [np.ones(n, g.dtype)], [g], [np.zeros(n, np.int8)], [np.zeros(n, np.uint8)], [np.zeros(6, np.float32)], [np.zeros(6, np.float32)])
+    one[0].adamw8bit(*one[1:], step=1, **{**HYPER, "grad_scale": 1.0})
+    mv, vv = (thc.TensorList([thc.Tensor.new(state, "Float")]) for _ in range(2))
+    mv.adamwValues(vv, *one[2:])
+    m, v = mv.tensors[0].numpy(), vv.tensors[0].numpy()
+    lost = np.isin(np.arange(n) // 256, [1, 5])
+    squares = lost | (np.arange(n) // 256 == 2) if kind == "Float" else lost
+    assert np.isnan(m[lost]).all() and np.isfinite(m[~lost]).all()
+    assert np.isnan(v[squares]).all() and np.isfinite(v[~squares]).all()
+    w = ro.adamw8(np.ones(n, g.dtype), g, *(np.zeros(k, t) for k, t in ((n, np.int8), (n, np.uint8), (6, np.float32), (6, np.float32))), 1,
+                  **{**HYPER, "grad_scale": 1.0})
+    for got, want in ((one[4], w[6]), (one[5], w[7])):
+        np.testing.assert_array_equal(got.tensors[0].numpy(), want)
+    assert_bit_equal(one[2].tensors[0].numpy()[~lost], w[4][~lost])
+    assert_bit_equal(one[3].tensors[0].numpy()[~squares], w[5][~squares])
