@@ -1752,22 +1752,52 @@ struct Positions : Held<long> {
   }
 };
 
-// Results must not share memory with anything else a call is given.
-struct Span { const char *lo, *hi; };
-template <typename R> Span span_of(const TensorT<R> *t) {
-  if (!t || !t->storage || !t->storage->data || tensor_nelement<R>(t) == 0) return Span{nullptr, nullptr};
+// The bytes a tensor takes; lo = null: none.
+struct Piece {
+  const char *base, *lo, *hi;       // first element; the bytes from the lowest to the highest
+  ptrdiff_t esz;
+  int dims;
+  const long *size, *stride;
+  bool written, dense;
+};
+template <typename R> Piece piece_of(const TensorT<R> *t, bool written = false) {
+  if (!t || !t->storage || !t->storage->data || tensor_nelement<R>(t) == 0) return Piece{};
   ptrdiff_t lo = 0, hi = 0;
   for (int d = 0; d < t->nDimension; ++d) {
     const ptrdiff_t reach = (ptrdiff_t)(t->size[d] - 1) * t->stride[d];
     if (reach > 0) hi += reach; else lo += reach;
   }
   const R *p = t->storage->data + t->storageOffset;
-  return Span{(const char *)(p + lo), (const char *)(p + hi + 1)};
+  return Piece{(const char *)p, (const char *)(p + lo), (const char *)(p + hi + 1), (ptrdiff_t)sizeof(R), t->nDimension, t->size, t->stride,
+               written, tensor_is_contiguous<R>(t)};
 }
-void check_apart(int arg, Span out, std::initializer_list<Span> others) {
+// Whether two tensors surely have no byte in common.  Counted modulo a stride L, the dims whose strides are multiples of L
+// stay where they are, so all that a tensor takes lies in one window as long as its other dims reach; two windows that do not
+// meet are enough (columns of one matrix, slices of an inner dim).
+bool surely_apart(const Piece &a, const Piece &b) {
+  if (a.hi <= b.lo || b.hi <= a.lo) return true;
+  const Piece *both[2] = {&a, &b};
+  const auto window = [](const Piece &p, ptrdiff_t l) {
+    ptrdiff_t w = p.esz;
+    for (int d = 0; d < p.dims; ++d)
+      if (p.stride[d] < 0) return l + 1;
+      else if (p.size[d] > 1 && p.stride[d] * p.esz % l != 0) w += (p.size[d] - 1) * p.stride[d] * p.esz;
+    return w;
+  };
+  for (const Piece *p : both)
+    for (int d = 0; d < p->dims; ++d) {
+      const ptrdiff_t l = p->stride[d] * p->esz;
+      if (p->size[d] <= 1 || l <= 0) continue;
+      const ptrdiff_t at = ((b.base - a.base) % l + l) % l;
+      if (window(a, l) <= at && at + window(b, l) <= l) return true;
+    }
+  return false;
+}
+// Results must not share memory with anything else a call is given.
+void check_apart(int arg, const Piece &out, std::initializer_list<Piece> others) {
   if (!out.lo) return;
-  for (const Span &s : others)
-    if (s.lo && out.lo < s.hi && s.lo < out.hi) th_arg_error(arg, "the result shares memory with another argument");
+  for (const Piece &p : others)
+    if (p.lo && !surely_apart(out, p)) th_arg_error(arg, "the result shares memory with another argument");
 }
 
 // A result that is one of the arguments: refused before anything is resized.
@@ -1789,7 +1819,7 @@ template <typename R> void embedding(THCState *state, TensorT<R> *result, Tensor
   for (int d = 0; d < index->nDimension; ++d) sz[d] = index->size[d];
   sz[index->nDimension] = weight->size[1];
   tensor_raw_resize<R>(state, result, index->nDimension + 1, sz, nullptr);
-  check_apart(2, span_of<R>(result), {span_of<R>(weight), span_of<long>(index)});
+  check_apart(2, piece_of<R>(result), {piece_of<R>(weight), piece_of<long>(index)});
   if (tensor_nelement<R>(result) == 0) return;
   RowsOut<R> out(state, result, 2);
   RowsIn<R> w(state, weight);
@@ -1809,7 +1839,7 @@ void embedding_acc_grad(THCState *state, TensorT<R> *grad_weight, TensorT<R> *gr
   for (int d = 0; d < index->nDimension; ++d)
     THArgCheck(grad_output->size[d] == index->size[d], 3, "gradOutput must have the sizes of index and the table's columns");
   THArgCheck(grad_output->size[index->nDimension] == grad_weight->size[1], 3, "gradOutput must have the sizes of index and the table's columns");
-  check_apart(2, span_of<R>(grad_weight), {span_of<R>(grad_output), span_of<long>(index)});
+  check_apart(2, piece_of<R>(grad_weight), {piece_of<R>(grad_output), piece_of<long>(index)});
   if (tensor_nelement<R>(grad_weight) == 0) return;
   RowsOut<R> table(state, grad_weight, 2);
   RowsIn<R> grad(state, grad_output);
@@ -1828,7 +1858,7 @@ void expert_sort(THCState *state, LongT *slot, LongT *order, LongT *offsets, Lon
   tensor_resize_as<long>(state, slot, expert);
   resize2(state, order, (long)tensor_nelement<long>(expert));
   resize2(state, offsets, experts + 1);
-  const Span s = span_of<long>(slot), o = span_of<long>(order), f = span_of<long>(offsets), e = span_of<long>(expert);
+  const Piece s = piece_of<long>(slot), o = piece_of<long>(order), f = piece_of<long>(offsets), e = piece_of<long>(expert);
   check_apart(2, s, {o, f, e});
   check_apart(3, o, {f, e});
   check_apart(4, f, {e});
@@ -1860,7 +1890,7 @@ template <typename R, typename A> void expert_dispatch(THCState *state, TensorT<
     const long sz[2] = {n, src->size[1]};
     tensor_raw_resize<R>(state, rows, 2, sz, nullptr);
   }
-  check_apart(2, span_of<R>(rows), {span_of<R>(src), span_of<long>(slot), span_of<A>(weight)});
+  check_apart(2, piece_of<R>(rows), {piece_of<R>(src), piece_of<long>(slot), piece_of<A>(weight)});
   if (n == 0 || src->size[1] == 0) return;
   RowsOut<R> out(state, rows, 2);
   RowsIn<R> in(state, src);
@@ -1884,7 +1914,7 @@ template <typename R, typename A> void expert_combine(THCState *state, TensorT<R
   check_distinct(2, result, {rows, weight});
   const long sz[2] = {slot->size[0], rows->size[1]};
   tensor_raw_resize<R>(state, result, 2, sz, nullptr);
-  check_apart(2, span_of<R>(result), {span_of<R>(rows), span_of<long>(slot), span_of<A>(weight)});
+  check_apart(2, piece_of<R>(result), {piece_of<R>(rows), piece_of<long>(slot), piece_of<A>(weight)});
   if (sz[0] == 0 || sz[1] == 0) return;
   RowsOut<R> out(state, result, 2);
   RowsIn<R> in(state, rows);
@@ -1913,9 +1943,9 @@ void expert_combine_grad(THCState *state, TensorT<R> *grad_rows, TensorT<A> *gra
   check_distinct(3, grad_weight, {grad_result, rows, weight});
   if (grad_rows) tensor_resize_as<R>(state, grad_rows, rows);
   if (grad_weight) tensor_raw_resize<A>(state, grad_weight, slot->nDimension, slot->size, nullptr);
-  const Span gr = span_of<R>(grad_rows), gw = span_of<A>(grad_weight);
-  check_apart(2, gr, {gw, span_of<R>(grad_result), span_of<R>(rows), span_of<long>(slot), span_of<A>(weight)});
-  check_apart(3, gw, {span_of<R>(grad_result), span_of<R>(rows), span_of<long>(slot), span_of<A>(weight)});
+  const Piece gr = piece_of<R>(grad_rows), gw = piece_of<A>(grad_weight);
+  check_apart(2, gr, {gw, piece_of<R>(grad_result), piece_of<R>(rows), piece_of<long>(slot), piece_of<A>(weight)});
+  check_apart(3, gw, {piece_of<R>(grad_result), piece_of<R>(rows), piece_of<long>(slot), piece_of<A>(weight)});
   if (tensor_nelement<long>(slot) == 0) return;
   if (rows->size[1] == 0 || rows->size[0] == 0) {   // no rows to multiply with
     if (grad_weight) pointwise<A>(state, THCB200_OP_FILL, grad_weight, nullptr, nullptr, nullptr, kZero, kZero);
@@ -1966,43 +1996,11 @@ template <typename R> struct HeldList {
 };
 
 // Strided tensors of a list go to the step as copies, so what they share with others shows in the tensors themselves only.
-struct Piece {
-  const char *base, *lo, *hi;       // first element; the bytes from the lowest to the highest
-  ptrdiff_t esz;
-  int dims;
-  const long *size, *stride;
-  bool written, dense;
-};
 template <typename R> void add_pieces(std::vector<Piece> &out, TensorT<R> **list, int n, bool written) {
   for (int i = 0; list && i < n; ++i) {
-    const TensorT<R> *t = list[i];
-    const Span s = span_of<R>(t);
-    if (!s.lo) continue;
-    out.push_back(Piece{(const char *)(t->storage->data + t->storageOffset), s.lo, s.hi, (ptrdiff_t)sizeof(R), t->nDimension, t->size, t->stride,
-                        written, tensor_is_contiguous<R>(t)});
+    const Piece p = piece_of<R>(list[i], written);
+    if (p.lo) out.push_back(p);
   }
-}
-// Whether two tensors surely have no byte in common.  Counted modulo a stride L, the dims whose strides are multiples of L
-// stay where they are, so all that a tensor takes lies in one window as long as its other dims reach; two windows that do not
-// meet are enough (columns of one matrix, slices of an inner dim).
-bool surely_apart(const Piece &a, const Piece &b) {
-  if (a.hi <= b.lo || b.hi <= a.lo) return true;
-  const Piece *both[2] = {&a, &b};
-  const auto window = [](const Piece &p, ptrdiff_t l) {
-    ptrdiff_t w = p.esz;
-    for (int d = 0; d < p.dims; ++d)
-      if (p.stride[d] < 0) return l + 1;
-      else if (p.size[d] > 1 && p.stride[d] * p.esz % l != 0) w += (p.size[d] - 1) * p.stride[d] * p.esz;
-    return w;
-  };
-  for (const Piece *p : both)
-    for (int d = 0; d < p->dims; ++d) {
-      const ptrdiff_t l = p->stride[d] * p->esz;
-      if (p->size[d] <= 1 || l <= 0) continue;
-      const ptrdiff_t at = ((b.base - a.base) % l + l) % l;
-      if (window(a, l) <= at && at + window(b, l) <= l) return true;
-    }
-  return false;
 }
 void check_pieces(std::vector<Piece> &p) {
   std::sort(p.begin(), p.end(), [](const Piece &a, const Piece &b) { return a.lo < b.lo; });

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from cutorch_b200 import thc
-from common import assert_bit_equal, rng, to_device
+from common import NP_OF_KIND, assert_bit_equal, rng, to_device
 from oracle import rows_oracle as ro
 from test_embedding_gpu import check_grad
 from test_expert_gpu import check_sort
@@ -298,6 +298,61 @@ def test_long_sorts(state, tokens, rows):
 @pytest.mark.parametrize("choices,experts", [(8193, 64), (65536, 500), (65537, 9), (70000, 2047), (300000, 128), (16384, 511), (16384, 512)])
 def test_long_expert_sorts(state, choices, experts):
     check_sort(state, rng("long experts", choices, experts).integers(0, experts + 1, choices), experts)
+
+
+@pytest.mark.parametrize("kind", ["Half", "Float", "Double"])
+@pytest.mark.parametrize("width", [8, 7, 1])
+def test_results_beside_their_sources_in_one_matrix(state, kind, width):
+    """Neighbouring columns of one matrix share no memory, whatever the spans from their first to their last bytes: the calls take
+    them, give what they give on tensors of their own and leave the other columns alone.  Windows that meet are refused."""
+    r = rng("windows", kind, width)
+    dt, wide = NP_OF_KIND[kind], np.float64 if kind == "Double" else np.float32
+    T, K, E, V = 9, 2, 3, 12
+    N, gap = T * K, 2                                           # rows of every matrix; columns between two windows
+    index, expert = r.integers(1, V + 1, T), r.integers(0, E + 1, (T, K))
+    slot = ro.expert_sort(expert, E)[0]
+    data = {k: r.standard_normal((n, width)).astype(dt) for k, n in
+            dict(table=V, x=T, grad_x=T, grad_table=V, rows=N, answers=N, y=T, grad_y=T, grad_answers=N).items()}
+    weight, grad_weight = r.random((T, K)).astype(wide), np.zeros((T, K), wide)
+    one = lambda a: to_device(state, a)  # noqa: E731
+    dindex, dslot, dweight = one(index), one(slot), one(weight)
+
+    calls = (
+        (("x", "table"), lambda t: t["x"].embedding(t["table"], dindex, 1.5)),
+        (("grad_table", "grad_x"), lambda t: t["grad_table"].embeddingAccGrad(t["grad_x"], dindex, 1.5, 0, 0)),
+        (("grad_table", "grad_x"), lambda t: t["grad_table"].embeddingAccGrad(t["grad_x"], dindex, 1.5, 0, 1)),
+        (("rows", "x"), lambda t: t["rows"].expertDispatch(t["x"], dslot, None)),
+        (("rows", "x"), lambda t: t["rows"].expertDispatch(t["x"], dslot, dweight)),
+        (("y", "answers"), lambda t: t["y"].expertCombine(t["answers"], dslot, dweight)),
+        (("grad_answers", "grad_y", "answers"), lambda t: t["grad_answers"].expertCombineGrad(one(grad_weight), t["grad_y"], t["answers"], dslot, dweight)),
+    )
+    step = width + gap
+    for names, call in calls:
+        alone = {k: one(data[k]) for k in names}
+        call(alone)
+        wide_matrix = r.standard_normal((N, step * len(names))).astype(dt)
+        for j, k in enumerate(names):
+            wide_matrix[:len(data[k]), j * step:j * step + width] = data[k]
+        matrix = one(wide_matrix)
+        call({k: matrix.narrow(1, j * step, width).narrow(0, 0, len(data[k])) for j, k in enumerate(names)})
+        want = wide_matrix.copy()
+        want[:len(data[names[0]]), :width] = alone[names[0]].numpy().reshape(len(data[names[0]]), width)
+        assert_bit_equal(matrix.numpy(), want, names)
+        if width > 1:
+            with pytest.raises(thc.THCError, match="shares memory"):
+                call({k: matrix.narrow(1, min(j, 1) * (width - 1), width).narrow(0, 0, len(data[k])) for j, k in enumerate(names)})
+            assert_bit_equal(matrix.numpy(), want, names)
+    # weights beside their gradient, slots beside the experts they come from
+    both = one(np.concatenate([grad_weight, weight], 1))
+    alone = one(grad_weight)
+    thc.Tensor.new(state, kind).expertCombineGrad(alone, one(data["grad_y"]), one(data["answers"]), dslot, dweight)
+    thc.Tensor.new(state, kind).expertCombineGrad(both.narrow(1, 0, K), one(data["grad_y"]), one(data["answers"]), dslot, both.narrow(1, K, K))
+    assert_bit_equal(both.numpy(), np.concatenate([alone.numpy(), weight], 1))
+    longs = one(np.concatenate([expert, np.full((T, K), 7), np.full((T, 1), 9)], 1))
+    longs.narrow(1, K, K).expertSort(thc.Tensor.new(state, "Long"), thc.Tensor.new(state, "Long"), longs.narrow(1, 0, K), E)
+    assert_bit_equal(longs.numpy(), np.concatenate([expert, slot, np.full((T, 1), 9)], 1))
+    with pytest.raises(thc.THCError, match="shares memory"):
+        longs.narrow(1, 1, K).expertSort(thc.Tensor.new(state, "Long"), thc.Tensor.new(state, "Long"), longs.narrow(1, 0, K), E)
 
 
 def torch_handle(state, t, kind):
