@@ -272,7 +272,7 @@ class Tensor:
                 strides.insert(0, run)
                 run *= n
         if storage_elems is None:
-            storage_elems = 1 + sum((n - 1) * s for n, s in zip(sizes, strides))
+            storage_elems = max(0, 1 + sum((n - 1) * s for n, s in zip(sizes, strides)))     # below 1 where a size is 0
         f = state.fn(kind, "newBorrowed")
         if f.argtypes is None:
             f.restype = C.c_void_p

@@ -361,6 +361,29 @@ def torch_handle(state, t, kind):
     return w
 
 
+def test_empty_windows_of_padded_rows(state):
+    """An expert without tokens, a batch without words: views of no rows whose strides reach further than the other dims do."""
+    import torch
+    rows = torch.arange(50, device="cuda", dtype=torch.float32).view(5, 10)
+    longs = torch.ones(5, 4, device="cuda", dtype=torch.int64)
+    x, one, two = torch_handle(state, rows[5:, :8], "Float"), torch_handle(state, longs[5:, 0], "Long"), torch_handle(state, longs[5:, :2], "Long")
+    table = to_device(state, np.ones((3, 8), np.float32))
+    table.embeddingAccGrad(x, one, 1.0, 0, 1)
+    assert_bit_equal(table.numpy(), np.ones((3, 8), np.float32))
+    table.embeddingAccGrad(x, one, 1.0, 0, 0)
+    assert_bit_equal(table.numpy(), np.zeros((3, 8), np.float32))
+    x.embedding(table, one, 1.0)
+    table.expertDispatch(x, two, None)
+    x.expertCombine(table, two, None)
+    slot, order, offsets = (thc.Tensor.new(state, "Long") for _ in range(3))
+    slot.expertSort(order, offsets, two, 3)
+    assert_bit_equal(offsets.numpy(), np.zeros(4, np.int64))
+    state.synchronize()
+    assert torch.equal(rows, torch.arange(50, device="cuda", dtype=torch.float32).view(5, 10))
+    empty = torch_handle(state, rows[:, 10:], "Float")            # rows of no elements
+    assert empty.numpy().shape == (5, 0)
+
+
 def test_offsets_beyond_32_bits(state):
     """A table of 2^32 + elements: rows on both sides of the border, looked up, and their gradients added."""
     import torch
