@@ -66,6 +66,7 @@ template <int N> struct StepTable {
 constexpr int kFewTensors = 16, kSomeTensors = 80, kManyTensors = 320;   // 1, 6 and 22.5 KiB of arguments: a launch with the last takes 2 us longer
 
 template <typename A> struct StepScalars { A beta1, one_minus_beta1, beta2, one_minus_beta2, keep, size, root, eps, grad_scale; uint32_t dither; };
+constexpr size_t kArgumentBytes = 32764;                                 // of a kernel launch
 
 // The entry a tile belongs to: the last one whose first tile is not behind it.
 template <int N> __device__ __forceinline__ const StepEntry &entry_of(const StepTable<N> &t, uint32_t tile) {
@@ -241,6 +242,7 @@ struct StepPairs {
   F2 minus_zero;
   uint32_t dither;
 };
+static_assert(sizeof(StepTable<kManyTensors>) + std::max(sizeof(StepPairs), sizeof(StepScalars<double>)) + alignof(StepPairs) <= kArgumentBytes);
 __device__ __forceinline__ F2 sub2(F2 a, F2 b) { return fma2(b, both(-1.0f), a); }   // no instruction for the sign
 __device__ __forceinline__ F2 fma2_down(F2 a, F2 b, F2 c) { F2 r; asm("fma.rm.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 

@@ -53,12 +53,11 @@ template <typename T, int V> __device__ __forceinline__ void store_pack(T *p, co
   }
 }
 
-// Asynchronous copy of V elements (4, 8 or 16 bytes) into shared memory.
+// Asynchronous copy of a 16-byte vector into shared memory.
 template <typename T, int V> __device__ __forceinline__ void copy_async(void *shared, const T *p) {
+  static_assert(sizeof(T) * V == 16, "a vector");
   const uint32_t s = (uint32_t)__cvta_generic_to_shared(shared);
-  if constexpr (sizeof(T) * V == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(s), "l"(p) : "memory");
-  else if constexpr (sizeof(T) * V == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" :: "r"(s), "l"(p) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(s), "l"(p) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(s), "l"(p) : "memory");
 }
 
 // An accumulator rounded once to the element type.
