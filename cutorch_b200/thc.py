@@ -625,9 +625,10 @@ class TensorList:
                 raise ValueError(f"{name}: lists of {n} and {len(what)} tensors")
         f = state._calls.get((self.kind, name, "list"))
         if f is None:
-            f = state._calls[self.kind, name, "list"] = state.fn(self.kind, name)
+            f = state.fn(self.kind, name)
             f.argtypes = [C.c_void_p] * (2 + len(lists)) + [C.c_int, *scalar_types]
             f.restype = None
+            state._calls[self.kind, name, "list"] = f          # other host threads find it there
         f(*args, n, *scalars)
         if state._failed():
             state.check()

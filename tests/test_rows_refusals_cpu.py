@@ -150,3 +150,39 @@ def test_large_kernel_arguments_fit():
     """The list of an AdamW launch travels in the kernel's arguments, of which CUDA takes 32764 bytes."""
     entry = 9 * 8
     assert 8 + 320 * entry + 10 * 8 <= 32764
+
+
+def test_list_calls_are_prepared_before_other_threads_see_them():
+    """A function without its C prototype takes no numbers (ctypes.ArgumentError): it may not be in the table of prepared calls yet
+    when its prototype is set, or another host thread's first step finds it there."""
+    from cutorch_b200 import thc
+
+    class Function:
+        prepared = None
+
+        def __setattr__(self, name, value):
+            if name in ("argtypes", "restype"):
+                assert not state._calls, f"{name} is set on a call that other threads may take"
+            object.__setattr__(self, name, value)
+
+        def __call__(self, *args):
+            self.prepared = len(self.argtypes)
+
+    class State:
+        ptr, _calls, function = 1, {}, Function()
+
+        def fn(self, kind, name):
+            return self.function
+
+        def _failed(self):
+            return 0
+
+    class Handle:
+        def __init__(self, kind):
+            self.state, self.kind, self.ptr = state, kind, 8
+
+    state = State()
+    lists = [thc.TensorList([Handle(k)]) for k in ("Float", "Float", "Char", "Byte", "Float", "Float")]
+    lists[0].adamwValues(*lists[1:])
+    assert state.function.prepared == 8 and list(state._calls.values()) == [state.function]
+    lists[0].adamwValues(*lists[1:])
