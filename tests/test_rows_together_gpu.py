@@ -355,6 +355,60 @@ def test_results_beside_their_sources_in_one_matrix(state, kind, width):
         longs.narrow(1, 1, K).expertSort(thc.Tensor.new(state, "Long"), thc.Tensor.new(state, "Long"), longs.narrow(1, 0, K), E)
 
 
+def test_captured_calls_over_strided_tensors(state):
+    """Results and lists that go through copies for the length of a call: in a graph the copies are the graph's own, made anew from what
+    the tensors hold at each replay."""
+    import torch
+    own = thc.State()
+    side = torch.cuda.Stream()
+    own.set_stream(side.cuda_stream, 0)
+    r = rng("captured strided")
+    T, K, E, V, W = 300, 2, 5, 40, 24
+    data = dict(index=r.integers(1, V + 1, T), weight=r.random((K, T)).astype(np.float32), gw=np.zeros((K, T), np.float32),
+                table=r.standard_normal((W, V)).astype(np.float32), x=np.zeros((W, T), np.float32), go=r.standard_normal((W, T)).astype(np.float32),
+                grad=np.zeros((V, 2 * W), np.float32), rows=r.standard_normal((T * K, W)).astype(np.float32),
+                grad_rows=np.zeros((W, T * K), np.float32), slot=ro.expert_sort(r.integers(0, E + 1, (T, K)), E)[0].T.copy(),
+                m=np.zeros((V, 2 * W), np.float32), v=np.zeros((V, 2 * W), np.float32))
+
+    class Set:
+        def __init__(self):
+            self.base = {k: to_device(own, a) for k, a in data.items()}
+            flip = lambda k: self.base[k].transpose(0, 1)  # noqa: E731
+            every_other = lambda k: self.base[k].narrow(1, 3, W)  # noqa: E731
+            self.t = {k: flip(k) for k in ("weight", "gw", "table", "x", "go", "grad_rows", "slot")}
+            self.t |= {k: every_other(k) for k in ("grad", "m", "v")}
+            self.lists = [thc.TensorList([self.t[k]]) for k in ("table", "grad", "m", "v")]
+
+        def run(self):
+            t = self.t
+            t["x"].embedding(t["table"], self.base["index"], 1.5)
+            t["grad"].embeddingAccGrad(t["go"], self.base["index"], 1.0, 0, 1)
+            t["grad_rows"].expertCombineGrad(t["gw"], t["x"], self.base["rows"], t["slot"], t["weight"])
+            self.lists[0].adamw(*self.lists[1:], step=2, **HYPER)
+
+        def check(self, other):
+            for k in data:
+                assert_bit_equal(self.base[k].numpy(), other.base[k].numpy(), k)
+
+    plain, replayed = Set(), Set()
+    with torch.cuda.stream(side):
+        replayed.run()
+        for k, a in data.items():
+            replayed.base[k].copy_from(to_device(own, a))
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            replayed.run()
+        replayed.check(plain)                               # capturing runs nothing
+        for _ in range(3):
+            graph.replay()
+            plain.run()
+            side.synchronize()
+            replayed.check(plain)
+    del graph
+    own.shutdown()
+
+
 def torch_handle(state, t, kind):
     w = thc.Tensor.wrap(state, kind, t.data_ptr(), tuple(t.shape), tuple(t.stride()))
     w.owner = t
