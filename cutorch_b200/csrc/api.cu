@@ -12,13 +12,13 @@ namespace thcb {
 int64_t launch_count();
 void arm_allocation_failure(int nth);
 
-void *ctx_workspace(thcb200_ctx *ctx, size_t bytes) {
-  if (bytes <= ctx->ws_bytes) return ctx->ws;
+static void *grown(void **ws, size_t *have, size_t bytes) {
+  if (bytes <= *have) return *ws;
   // grow: wait for work that may still read the old buffer
   if (cudaDeviceSynchronize() != cudaSuccess) { set_error("workspace: device synchronize failed"); return nullptr; }
-  if (ctx->ws) cudaFree(ctx->ws);
-  ctx->ws = nullptr;
-  ctx->ws_bytes = 0;
+  if (*ws) cudaFree(*ws);
+  *ws = nullptr;
+  *have = 0;
   size_t want = 1 << 20;
   while (want < bytes) want <<= 1;
   void *p = nullptr;
@@ -27,10 +27,12 @@ void *ctx_workspace(thcb200_ctx *ctx, size_t bytes) {
     set_error("workspace: cannot allocate %zu bytes", want);
     return nullptr;
   }
-  ctx->ws = p;
-  ctx->ws_bytes = want;
+  *ws = p;
+  *have = want;
   return p;
 }
+void *ctx_workspace(thcb200_ctx *ctx, size_t bytes) { return grown(&ctx->ws, &ctx->ws_bytes, bytes); }
+void *ctx_rows_workspace(thcb200_ctx *ctx, size_t bytes) { return grown(&ctx->rows_ws, &ctx->rows_ws_bytes, bytes); }
 
 namespace {
 
@@ -174,6 +176,8 @@ int thcb200_ctx_create(thcb200_ctx **out, int device) {
   if (e == cudaSuccess) e = cudaHostGetDevicePointer(&c->host_slot_dev, c->host_slot, 0);
   if (e == cudaSuccess) e = cudaMalloc(&c->ws, 1 << 20);
   if (e == cudaSuccess) c->ws_bytes = 1 << 20;
+  if (e == cudaSuccess) e = cudaMalloc(&c->rows_ws, 1 << 20);
+  if (e == cudaSuccess) c->rows_ws_bytes = 1 << 20;
   cudaSetDevice(prev);
   if (e != cudaSuccess) {
     set_error("ctx_create: %s", cudaGetErrorString(e));
@@ -194,6 +198,7 @@ void thcb200_ctx_destroy(thcb200_ctx *c) {
   if (c->dev_slot) cudaFree(c->dev_slot);
   if (c->host_slot) cudaFreeHost(c->host_slot);
   if (c->ws) cudaFree(c->ws);
+  if (c->rows_ws) cudaFree(c->rows_ws);
   if (c->mask_ws) cudaFree(c->mask_ws);
   cudaSetDevice(prev);
   delete c;

@@ -25,6 +25,10 @@ struct thcb200_ctx {
   int max_smem_optin;
   void *ws;               // device workspace for partial results, grown on demand
   size_t ws_bytes;
+  // the same for the calls over rows (rows.cuh), which may need gigabytes: apart from `ws`, whose address captured reductions and
+  // callers of thcb200_ctx_workspace keep and which must not move for them
+  void *rows_ws;
+  size_t rows_ws_bytes;
   unsigned int *tickets;  // kNumTickets counters, zero between launches (kernels reset them)
   int *status;            // device word: kernels record bounded-wait failures here
   void *host_slot;        // pinned, mapped, 64 bytes
@@ -52,6 +56,7 @@ namespace thcb {
 // Returns a device buffer of at least `bytes` (256-byte aligned), valid until the next call
 // that asks for more.  Growing synchronises the device; nullptr on allocation failure.
 void *ctx_workspace(thcb200_ctx *ctx, size_t bytes);
+void *ctx_rows_workspace(thcb200_ctx *ctx, size_t bytes);
 
 // Every device allocation the library makes for itself (workspaces, dense temporaries) goes through
 // these two, so that a test can make the n-th one fail the way an exhausted GPU would, without

@@ -100,7 +100,7 @@ inline bool dense_rows(const MatView &m) {
 // The context's count of positions out of range (thcb200_take_index_errors reads it).
 inline unsigned int *index_errors(thcb200_ctx *ctx) { return reinterpret_cast<unsigned int *>(ctx->status) + 1; }
 
-// Scratch of one call: the context's workspace, or, while the stream is being captured into a graph, an allocation that
+// Scratch of one call: the context's workspace for rows, or, while the stream is being captured into a graph, an allocation that
 // becomes part of that graph: a graph that outlives the call must not hold the address of a buffer that later calls share
 // and may replace.  The caller holds the context's lock.
 struct Workspace {
@@ -115,7 +115,7 @@ struct Workspace {
       return;
     }
     if (status == cudaStreamCaptureStatusNone) {
-      data = (char *)ctx_workspace(ctx, bytes);
+      data = (char *)ctx_rows_workspace(ctx, bytes);
     } else if (device_alloc_async(&owned_, bytes, st) == cudaSuccess) {
       data = (char *)owned_;
     } else {

@@ -423,8 +423,10 @@ THCB200_API int thcb200_embedding(thcb200_ctx *ctx, const thcb200_tensor *result
                       const thcb200_tensor *index, double scale, void *stream);
 /* grad_weight[r, :] = scale * sum over t with index[t] = r of grad_output[t, :], in token order; rows no token names
  * become zero.  accumulate != 0 adds the sums to what is there and leaves the other rows alone.  Tokens whose position is
- * padding_index (0: none) are left out.  Uses the context's workspace: about 24 bytes per token and the partial sums of
- * rows whose tokens are cut by a chunk boundary. */
+ * padding_index (0: none) are left out.  Beyond 64 tokens it uses a workspace of the context, apart from the one that
+ * thcb200_ctx_workspace gives out: 8 to 24 bytes per token and, whether or not a row is cut by a chunk boundary,
+ * 2 * ceil(tokens / chunk) * columns sums (F16: float, otherwise double) of chunks of 8 to 64 tokens.  It grows by powers of two, which
+ * waits for the device, and is kept until the context goes. */
 THCB200_API int thcb200_embedding_grad(thcb200_ctx *ctx, const thcb200_tensor *grad_weight, const thcb200_tensor *grad_output,
                            const thcb200_tensor *index, double scale, int64_t padding_index, int accumulate, void *stream);
 

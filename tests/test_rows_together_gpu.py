@@ -1,5 +1,6 @@
 """Embedding, expert routing and AdamW used together: a small model's training steps against the same model in 64 bits, recorded
 into graphs, on streams of their own, from several host threads, and at sizes whose offsets pass 32 bits."""
+import ctypes as C
 import threading
 
 import numpy as np
@@ -405,6 +406,37 @@ def test_captured_calls_over_strided_tensors(state):
             plain.run()
             side.synchronize()
             replayed.check(plain)
+    del graph
+    own.shutdown()
+
+
+def test_the_scratch_of_reductions_stays_where_it_is():
+    """A gradient that needs hundreds of megabytes leaves the scratch of the context's other calls alone: its address is in the hands of
+    captured reductions and of callers of THCState_getCurrentDeviceScratchSpace."""
+    import torch
+    own = thc.State()
+    side = torch.cuda.Stream()
+    own.set_stream(side.cuda_stream, 0)
+    scratch = own.lib.THCState_getCurrentDeviceScratchSpace
+    scratch.restype, scratch.argtypes = C.c_void_p, [C.c_void_p]
+    r = rng("scratch")
+    a = r.integers(-8, 9, (4, 200000)).astype(np.float32)
+    x, out = to_device(own, a), to_device(own, np.zeros((4, 1), np.float32))
+    with torch.cuda.stream(side):
+        out.sum(x, 1, 1)
+        before = scratch(own.ptr)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out.sum(x, 1, 1)
+        index = r.integers(1, 9, 60000)
+        table = to_device(own, np.zeros((8, 600), np.float32))
+        table.embeddingAccGrad(to_device(own, np.ones((60000, 600), np.float32)), to_device(own, index), 1.0, 0, 0)
+        assert scratch(own.ptr) == before
+        out.copy_from(to_device(own, np.zeros((4, 1), np.float32)))
+        graph.replay()
+        side.synchronize()
+    assert_bit_equal(out.numpy(), a.sum(1, keepdims=True))
+    assert_bit_equal(table.numpy(), np.repeat(np.bincount(index, minlength=9)[1:, None], 600, 1).astype(np.float32))
     del graph
     own.shutdown()
 
