@@ -19,9 +19,10 @@
 // depend on the compiler's choice of fused operations; the 8-bit form's parameter takes the approximate root and reciprocal.
 //
 // Both are bound by HBM in principle.  200 M float elements in 290 tensors, B200: 32-bit moments 800 us, 5.6 GB, 7000 GB/s (the
-// box's copy: 6558).  8-bit moments, 3.2 GB: 795 us, 4.0 TB/s, bound by instruction issue (89 per element): 1310 us with scalar
-// instructions, IEEE roots and byte conversions, 925 us packed, 890 us with 1024 threads per SM, 860 us with the next tile
-// prefetched into the L2, 840 us with the rare exact codes apart, 795 us with CTAs of 128 threads.
+// box's copy: 6558).  8-bit moments, 3.2 GB: 795 us, 4.0 TB/s, bound by instruction issue (about 90 per element): 1310 us with
+// scalar instructions, IEEE roots and byte conversions, 925 us packed, 890 us with 1024 threads per SM, 860 us with the next tile
+// prefetched into the L2, 840 us with the rare exact codes apart, 795 us with CTAs of 128 threads (a loop of 1500; 695 us before the
+// power limit holds the clocks back).  Half parameters issue as many: 806 us for 2.0 GB, with masters 850 us for 3.2 GB.
 #include <cuda_fp16.h>
 #include <float.h>
 #include <math.h>

@@ -5,8 +5,8 @@
 // kClusterItems one cluster does all radix passes in one launch; beyond, each pass is three kernels: digit counts of
 // every tile, a scan of those counts over the tiles, and the scatter.  One pass, B200, us back to back in a graph:
 //   items        300   4096   8192  16384  32768  65536  131072  262144
-//   cluster      3.2    3.5    4.4    5.0    5.9    8.1    13.3    22.1    (64 keys; 500 keys: 4.0 .. 26)
-//   tiles                           10.8   10.6   10.9    11.7    15.6    (500 keys: 12 .. 17)
+//   cluster      3.2    3.5    4.4    5.0    5.9    8.1                    (64 keys; 500 keys: 4.0 .. 10.4)
+//   tiles                           10.8   10.6   10.9    11.7    15.7    (500 keys: 12 .. 17)
 // (one CTA's shared memory instead of the cluster: 5.4 at 300 items, 10.8 at 4096.)
 #include "keysort.h"
 
